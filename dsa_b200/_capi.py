@@ -45,6 +45,25 @@ class TdsaRescue(C.Structure):
                 ("use_threshold", i32)]
 
 
+class TdsaPagedCache(C.Structure):
+    """struct tdsa_paged_cache (include/tdsa.h)."""
+    _fields_ = [("keys", vp), ("values", vp), ("page_stride", i64), ("row_stride", i64),
+                ("head_stride", i64), ("pages", C.c_int32), ("page_size", C.c_int32),
+                ("kv_heads", C.c_int32), ("head_dim", C.c_int32), ("dtype", C.c_int32)]
+
+
+class TdsaPagedBatch(C.Structure):
+    """struct tdsa_paged_batch (include/tdsa.h)."""
+    _fields_ = [("page_table", vp), ("table_stride", i64), ("query_starts", vp), ("lengths", vp),
+                ("batch", C.c_int32), ("max_pages", C.c_int32), ("tokens", C.c_int32),
+                ("max_new", C.c_int32)]
+
+
+class TdsaTokenRows(C.Structure):
+    """struct tdsa_token_rows (include/tdsa.h)."""
+    _fields_ = [("data", vp), ("token_stride", i64), ("head_stride", i64)]
+
+
 TDSA_ORDER_ADDRESS, TDSA_ORDER_PREVIOUS_MAX = 0, 1
 TDSA_ORDER_BUCKET, TDSA_ORDER_ORACLE_CURRENT = 2, 3
 TDSA_RISK_LAST_MAX, TDSA_RISK_EMA = 0, 1
@@ -122,6 +141,12 @@ SIGNATURES: dict[str, tuple] = {
     "tdsa_block_key_norms": (i32, [vp, i32, i32, i32, i32, vp, vp]),
     "tdsa_temporal_radius": (i32, [vp, vp, vp, vp, vp, i32, i32, i32, vp, vp, vp]),
     "tdsa_relu_index_score": (i32, [vp, vp, vp, i32, i32, i32, vp, vp]),
+    # struct arguments by address (vp): C.byref of the structures above
+    "tdsa_paged_append": (i32, [vp, vp, vp, vp, vp, vp, i32, vp, i32, i32, vp, vp]),
+    "tdsa_paged_workspace_bytes": (sz, [i32]),
+    "tdsa_paged_attention": (i32, [vp, vp, vp, i32, C.c_float, i32, vp, vp, vp, sz, vp]),
+    "tdsa_selected_attention": (i32, [vp, vp, vp, i32, C.c_float, vp, i32, i64, i32, vp, vp, vp,
+                                      sz, vp]),
     "tdsa_query_prep": (i32, [vp, i64, vp, i64, i32, vp, vp, vp, i64, vp, i64, i32, i32, i32,
                               C.c_float, C.c_float, vp]),
 }

@@ -1,4 +1,5 @@
 // extern "C" entry points of libtdsa: argument checks on the host, then the launchers.
+#include <algorithm>
 #include <mutex>
 #include <string>
 #include <utility>
@@ -6,6 +7,7 @@
 
 #include "common.cuh"
 #include "kernels.cuh"
+#include "paged.cuh"
 
 namespace tdsa {
 
@@ -208,6 +210,97 @@ int block_setup(const void* q, int64_t q_bs, const float* w, int64_t w_bs, const
   a.w_stride = w_bs;
   a.status = device_status_ptr();
   if (!a.status) return fail(TDSA_ERR_CUDA, "device status word not available");
+  return TDSA_OK;
+}
+
+// Shared checks of the paged entry points; fills the device view.
+int paged_setup(const tdsa_paged_cache* c, const tdsa_paged_batch* b, PagedView& p) {
+  if (!c || !b) return fail(TDSA_ERR_INVALID, "cache or batch is null");
+  if (c->dtype != TDSA_BF16 && c->dtype != TDSA_F16)
+    return fail(TDSA_ERR_UNSUPPORTED, "paged caches are TDSA_BF16 or TDSA_F16");
+  if (c->head_dim != 64 && c->head_dim != 128)
+    return fail(TDSA_ERR_UNSUPPORTED, "head_dim must be 64 or 128");
+  if (c->page_size < 16 || c->page_size > 1024 || (c->page_size & (c->page_size - 1)))
+    return fail(TDSA_ERR_UNSUPPORTED, "page_size must be a power of two from 16 to 1024");
+  if (c->pages < 1 || c->kv_heads < 1 || c->kv_heads > 1024)
+    return fail(TDSA_ERR_INVALID, "pages must be >= 1 and kv_heads in [1, 1024]");
+  if (!c->keys || !c->values) return fail(TDSA_ERR_INVALID, "cache pointers are null");
+  if (!aligned16(c->keys) || !aligned16(c->values) || c->page_stride % 8 || c->row_stride % 8 ||
+      c->head_stride % 8)
+    return fail(TDSA_ERR_ALIGN,
+                "cache bases must be 16-byte aligned, strides multiples of 8 elements");
+  if (c->page_stride < 0 || c->row_stride < c->head_dim ||
+      (c->kv_heads > 1 && c->head_stride < c->head_dim))
+    return fail(TDSA_ERR_INVALID, "cache strides overlap the rows");
+  if (b->batch < 1 || b->batch > 65535)
+    return fail(TDSA_ERR_INVALID, "batch must be in [1, 65535]");
+  if (b->tokens < 0 || b->max_new < 0 || b->max_pages < 1)
+    return fail(TDSA_ERR_INVALID, "tokens, max_new must be >= 0 and max_pages >= 1");
+  if (static_cast<int64_t>(b->max_pages) * c->page_size > (int64_t(1) << 30))
+    return fail(TDSA_ERR_UNSUPPORTED, "max_pages * page_size must be at most 2^30");
+  if (!b->page_table || !b->query_starts || !b->lengths)
+    return fail(TDSA_ERR_INVALID, "batch pointers are null");
+  if (b->batch > 1 && b->table_stride < b->max_pages)
+    return fail(TDSA_ERR_INVALID, "table_stride must be >= max_pages");
+  p.keys = static_cast<const uint16_t*>(c->keys);
+  p.values = static_cast<const uint16_t*>(c->values);
+  p.page_stride = c->page_stride;
+  p.row_stride = c->row_stride;
+  p.head_stride = c->head_stride;
+  p.pages = c->pages;
+  p.page_shift = __builtin_ctz(static_cast<unsigned>(c->page_size));
+  p.kv_heads = c->kv_heads;
+  p.table = b->page_table;
+  p.table_stride = b->table_stride;
+  p.starts = b->query_starts;
+  p.lengths = b->lengths;
+  p.batch = b->batch;
+  p.max_pages = b->max_pages;
+  p.tokens = b->tokens;
+  return TDSA_OK;
+}
+
+int check_token_rows(const tdsa_token_rows* r, int heads, int dim, const char* name) {
+  if (!r || !r->data) return fail(TDSA_ERR_INVALID, std::string(name) + " is null");
+  if (!aligned16(r->data) || r->token_stride % 8 || r->head_stride % 8)
+    return fail(TDSA_ERR_ALIGN, std::string(name) +
+                                    " must be 16-byte aligned with strides that are multiples "
+                                    "of 8 elements");
+  if (r->token_stride < 0 || (heads > 1 && r->head_stride < 0) || dim < 1)
+    return fail(TDSA_ERR_INVALID, std::string(name) + " has a negative stride");
+  return TDSA_OK;
+}
+
+int paged_query(const tdsa_paged_cache* c, const tdsa_token_rows* q, int q_heads, float scale,
+                const tdsa_token_rows* out, float* lse, void* ws, size_t ws_bytes,
+                PagedQuery& d) {
+  if (q_heads < 1 || q_heads % c->kv_heads)
+    return fail(TDSA_ERR_INVALID, "q_heads must be a multiple of kv_heads");
+  int rc = check_token_rows(q, q_heads, c->head_dim, "q");
+  if (!rc) rc = check_token_rows(out, q_heads, c->head_dim, "out");
+  if (rc) return rc;
+  if (!(scale > 0.f) || scale > 1e30f)
+    return fail(TDSA_ERR_INVALID, "scale must be positive and finite");
+  if (!ws || ws_bytes < tdsa_paged_workspace_bytes(c->head_dim) ||
+      (reinterpret_cast<uintptr_t>(ws) & 255u))
+    return fail(TDSA_ERR_WORKSPACE,
+                "workspace missing, smaller than tdsa_paged_workspace_bytes or not 256-byte "
+                "aligned");
+  d.q = static_cast<const uint16_t*>(q->data);
+  d.q_ts = q->token_stride;
+  d.q_hs = q->head_stride;
+  d.out = static_cast<uint16_t*>(out->data);
+  d.o_ts = out->token_stride;
+  d.o_hs = out->head_stride;
+  d.lse = lse;
+  d.heads = q_heads;
+  d.group = q_heads / c->kv_heads;
+  d.scale_log2 = scale * 1.4426950408889634f;
+  d.window = 0;
+  d.idx = nullptr;
+  d.idx_stride = 0;
+  d.idx_bytes = 4;
+  d.topk = 0;
   return TDSA_OK;
 }
 
@@ -1075,6 +1168,90 @@ int tdsa_relu_index_score(const double* q, const double* keys, const double* w, 
   if (tokens == 0) return TDSA_OK;
   return launch_relu_index_score(q, keys, w, heads, dim, tokens, out,
                                  static_cast<cudaStream_t>(stream));
+}
+
+int tdsa_paged_append(const tdsa_paged_cache* cache, const tdsa_paged_batch* batch,
+                      const tdsa_token_rows* k, const tdsa_token_rows* v,
+                      const tdsa_token_rows* q, const tdsa_token_rows* q_out, int q_heads,
+                      const float* inv_freq, int rope_dim, int interleaved,
+                      const int64_t* positions, void* stream) {
+  PagedView p;
+  int rc = paged_setup(cache, batch, p);
+  if (rc) return rc;
+  if (rope_dim < 0 || rope_dim % 16 || rope_dim > cache->head_dim)
+    return fail(TDSA_ERR_INVALID, "rope_dim must be a multiple of 16 up to head_dim");
+  if (rope_dim && !inv_freq) return fail(TDSA_ERR_INVALID, "inv_freq is null");
+  if (batch->tokens == 0) return TDSA_OK;
+  rc = check_token_rows(k, cache->kv_heads, cache->head_dim, "k");
+  if (!rc) rc = check_token_rows(v, cache->kv_heads, cache->head_dim, "v");
+  if (!rc && q) {
+    if (q_heads < 1) return fail(TDSA_ERR_INVALID, "q_heads must be >= 1");
+    rc = check_token_rows(q, q_heads, cache->head_dim, "q");
+    if (!rc) rc = check_token_rows(q_out, q_heads, cache->head_dim, "q_out");
+  }
+  if (rc) return rc;
+  int* status = device_status_ptr();
+  if (!status) return fail(TDSA_ERR_CUDA, "device status word not available");
+  return launch_paged_append(p, cache->keys, cache->values, cache->dtype, cache->head_dim,
+                             k->data, k->token_stride, k->head_stride, v->data,
+                             v->token_stride, v->head_stride, q ? q->data : nullptr,
+                             q ? q->token_stride : 0, q ? q->head_stride : 0, q ? q_heads : 0,
+                             q ? q_out->data : nullptr, q ? q_out->token_stride : 0,
+                             q ? q_out->head_stride : 0, inv_freq, rope_dim, interleaved ? 1 : 0,
+                             positions, status, static_cast<cudaStream_t>(stream));
+}
+
+size_t tdsa_paged_workspace_bytes(int head_dim) {
+  if (head_dim != 64 && head_dim != 128) return 0;
+  return paged_rows_workspace_bytes(head_dim);
+}
+
+int tdsa_paged_attention(const tdsa_paged_cache* cache, const tdsa_paged_batch* batch,
+                         const tdsa_token_rows* q, int q_heads, float scale, int window,
+                         const tdsa_token_rows* out, float* lse, void* workspace,
+                         size_t workspace_bytes, void* stream) {
+  PagedView p;
+  PagedQuery d;
+  int rc = paged_setup(cache, batch, p);
+  if (rc || batch->tokens == 0) return rc;
+  rc = paged_query(cache, q, q_heads, scale, out, lse, workspace, workspace_bytes, d);
+  if (rc) return rc;
+  if (window < 0) return fail(TDSA_ERR_INVALID, "window must be >= 0");
+  d.window = window;
+  int* status = device_status_ptr();
+  if (!status) return fail(TDSA_ERR_CUDA, "device status word not available");
+  const int64_t rows = static_cast<int64_t>(batch->max_new) * d.group;
+  return launch_paged_rows(p, d, cache->dtype, cache->head_dim,
+                           static_cast<int>(std::min<int64_t>(rows, 1 << 20)), workspace, status,
+                           static_cast<cudaStream_t>(stream));
+}
+
+int tdsa_selected_attention(const tdsa_paged_cache* cache, const tdsa_paged_batch* batch,
+                            const tdsa_token_rows* q, int q_heads, float scale,
+                            const void* indices, int index_bytes, int64_t idx_stride, int k,
+                            const tdsa_token_rows* out, float* lse, void* workspace,
+                            size_t workspace_bytes, void* stream) {
+  PagedView p;
+  PagedQuery d;
+  int rc = paged_setup(cache, batch, p);
+  if (rc || batch->tokens == 0) return rc;
+  rc = paged_query(cache, q, q_heads, scale, out, lse, workspace, workspace_bytes, d);
+  if (rc) return rc;
+  if (!indices) return fail(TDSA_ERR_INVALID, "indices is null");
+  if (index_bytes != 4 && index_bytes != 8)
+    return fail(TDSA_ERR_INVALID, "index_bytes must be 4 or 8");
+  if (reinterpret_cast<uintptr_t>(indices) % index_bytes)
+    return fail(TDSA_ERR_ALIGN, "indices must be aligned to their type");
+  if (k < 1 || k > (1 << 24) || (batch->tokens > 1 && idx_stride < k))
+    return fail(TDSA_ERR_INVALID, "k must be in [1, 2^24] and idx_stride >= k");
+  d.idx = indices;
+  d.idx_bytes = index_bytes;
+  d.idx_stride = idx_stride;
+  d.topk = k;
+  int* status = device_status_ptr();
+  if (!status) return fail(TDSA_ERR_CUDA, "device status word not available");
+  return launch_paged_rows(p, d, cache->dtype, cache->head_dim, d.group, workspace, status,
+                           static_cast<cudaStream_t>(stream));
 }
 
 }  // extern "C"

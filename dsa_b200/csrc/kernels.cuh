@@ -197,6 +197,20 @@ int launch_qprep(const void* qraw, int64_t qraw_stride, const void* x, int64_t x
                  int64_t q_stride, float* w, int64_t w_stride, int dtype, int batch,
                  int rope_dim, float theta, float scale, cudaStream_t stream);
 
+// ---- paged key/value cache (paged.cuh; paged_append.cu, paged_rows.cu)
+struct PagedView;
+struct PagedQuery;
+int launch_paged_append(const PagedView& p, void* keys, void* values, int dtype, int dim,
+                        const void* k, int64_t k_ts, int64_t k_hs, const void* v, int64_t v_ts,
+                        int64_t v_hs, const void* q, int64_t q_ts, int64_t q_hs, int q_heads,
+                        void* q_out, int64_t qo_ts, int64_t qo_hs, const float* inv_freq,
+                        int rope_dim, int pairs, const int64_t* positions, int* status,
+                        cudaStream_t stream);
+size_t paged_rows_workspace_bytes(int dim);
+// rows: query rows per sequence (or token, selected attention) and key/value head, at most
+int launch_paged_rows(const PagedView& p, const PagedQuery& q, int dtype, int dim, int rows,
+                      void* ws, int* status, cudaStream_t stream);
+
 // Device status word of the current device (allocated with the module, never freed).
 int* device_status_ptr();
 

@@ -1,0 +1,735 @@
+// Attention of few query rows over a paged key/value cache: the decode step (one or a few new
+// tokens per sequence) and the attention over the positions a top-k selected.
+//
+//   out[t,h] = sum_j softmax_j(scale q[t,h].K[j]) V[j],  lse[t,h] = log sum_j exp(scale q.K[j])
+//
+// over the keys j that token t sees.  The rows of an item are the query heads that share one
+// key/value head (times the sequence's new tokens), 16 MT of them, so every key and value is
+// read from the cache once.
+//
+// Layout.  A CTA is four warps.  Each warp runs its own stream of 16-key tiles (unit u of an
+// item is 64 keys, 16 per warp) with its own ring of tiles in shared memory, filled by 16-byte
+// asynchronous copies -- a row of the cache is gathered by address, so pages and selected
+// positions cost the same -- and its own running maximum, sum and output in registers; warps
+// meet only at the end of an item's segment.  No block-wide barrier is in the key loop.  S = Q K^T
+// and O += P V are warp-level 16x8x16 matrix instructions with float32 accumulators: with 1 to
+// 32 rows the tensor work is a fifth of the time the keys take to arrive, and their operands
+// and results stay in registers, which a tile of fewer rows than the 64 to 128 of a tcgen05
+// instruction could not.  P is rounded to the cache's type for the second product (relative
+// 2^-8 in bf16 and 2^-11 in f16, the rounding that the output gets too); maxima and sums are
+// float32, the sum of the unrounded P.
+//
+// Values of keys that no row of the item sees (past the length, or of a page that is not one)
+// are zero-filled on arrival.  In a tile that some rows see and others do not, a value that is
+// not finite would turn the zero weight of the others into NaN; such a tile's product is formed
+// element by element (add_visible).
+#include <algorithm>
+
+#include "paged.cuh"
+
+namespace tdsa {
+
+namespace {
+
+constexpr int kPrWarps = 4;
+constexpr int kPrThreads = kPrWarps * 32;
+constexpr int kPrTile = 16;                     // keys per warp and tile
+constexpr int kPrUnit = kPrWarps * kPrTile;     // keys per unit of work
+
+struct RowsArgs {
+  PagedView p;
+  PagedQuery q;
+  PagedPartials part;
+  int* status;
+};
+
+template <int D, int MT>
+struct RowsCfg {
+  static constexpr int kRowBytes = D * 2;
+  static constexpr int kTileBytes = kPrTile * kRowBytes;       // K or V tile
+  static constexpr int kStageBytes = 2 * kTileBytes;
+  static constexpr int kStages = D == 128 ? 3 : 6;
+  static constexpr int kWarpBytes = kStages * kStageBytes;
+  static constexpr int kRows = 16 * MT;
+  static constexpr int kMergeO = kRows * D * 4;                // a warp's output, float32
+  static constexpr int kRing = kPrWarps * kWarpBytes;
+  static constexpr int kMl = kPrWarps * kRows * 8;
+  static constexpr int kSmem = kRing + kMl + 256 + kPrWarps * kStages * 4;
+  static_assert(kMergeO <= kWarpBytes, "a warp's output fits its ring");
+};
+
+__device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr)
+               : "memory");
+}
+__device__ __forceinline__ void ldsm4t(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr)
+               : "memory");
+}
+
+template <bool kBF16>
+__device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0,
+                                         uint32_t b1) {
+  if (kBF16)
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
+        "{%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  else
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
+        "{%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+__device__ __forceinline__ void cp_async16_fill(uint32_t dst, const void* src, bool valid) {
+  const int n = valid ? 16 : 0;  // 0 source bytes: the 16 bytes are zero-filled
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n)
+               : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() {
+  asm volatile("cp.async.commit_group;" ::: "memory");
+}
+template <int N>
+__device__ __forceinline__ void cp_async_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+
+// One item: rows [r0, r0 + rows) of the (token, head) rows of a sequence and key/value head.
+struct Item {
+  int seq, head;      // sequence, key/value head
+  int tok0;           // batch row of the sequence's (or the only) token 0
+  int r0, rows;       // row range (row r: token tok0 + r / group, head h * group + r % group)
+  int pos0;           // position of token 0
+  int k0, k1;         // keys any row sees
+  int u0, u1;         // units [u0, u1) of 64 keys covering them (at least one)
+};
+
+template <int kRows>
+__device__ __forceinline__ void range_item(const RowsArgs& a, const SeqSpan& s, int rt,
+                                           Item& it) {
+  const int g = a.q.group;
+  it.tok0 = s.q0;
+  it.r0 = rt * kRows;
+  it.rows = min(kRows, s.n * g - it.r0);
+  it.pos0 = s.len - s.n;
+  const int first = it.pos0 + it.r0 / g;
+  const int last = it.pos0 + (it.r0 + it.rows - 1) / g;
+  it.k1 = max(0, last + 1);
+  it.k0 = a.q.window > 0 ? max(0, first - (a.q.window - 1)) : 0;
+  it.k0 = min(it.k0, it.k1);
+  it.u0 = it.k0 / kPrUnit;
+  it.u1 = max(it.u0 + 1, (it.k1 + kPrUnit - 1) / kPrUnit);
+}
+
+template <bool kBF16, int D, int MT, bool kSel>
+__global__ void __launch_bounds__(kPrThreads, 2) paged_rows_kernel(const RowsArgs a) {
+  using C = RowsCfg<D, MT>;
+  constexpr int kRows = C::kRows, kStages = C::kStages;
+  constexpr int kKs = D / 16;   // 16-wide steps of the head dimension
+  constexpr int kNt = D / 8;    // 8-wide output tiles
+  constexpr int kLanesPerRow = D / 8;
+  constexpr int kRowsPerCopy = 32 / kLanesPerRow;
+  extern __shared__ __align__(128) uint8_t smem[];
+  float2* s_ml = reinterpret_cast<float2*>(smem + C::kRing);  // [warp][row]
+  int* s_meta = reinterpret_cast<int*>(smem + C::kRing + C::kMl);
+  int64_t* s_scan = reinterpret_cast<int64_t*>(s_meta + 8);   // [4] warp totals
+  // [warp][stage]: bit r is set when row r of the stage's tile holds a key of the cache
+  uint32_t* s_valid = reinterpret_cast<uint32_t*>(smem + C::kRing + C::kMl + 256) +
+                      (threadIdx.x >> 5) * kStages;
+
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int quad = lane >> 2, ql = lane & 3;
+  const int g = a.q.group, hkv = a.p.kv_heads;
+  int ctas = gridDim.x;  // CTAs that get work: no more than there are units
+  const int cta = blockIdx.x;
+  pdl_wait();
+  pdl_launch_dependents();
+
+  // ---------------------------------------------------------------- this CTA's slice
+  int64_t units;       // of the whole call
+  int64_t u_begin, u_end;
+  Item it;
+  int rt = 0;          // row tile of the current item
+  int off;             // unit of the item the slice begins at
+  SeqSpan span;
+  const int sel_units = kSel ? max(1, (a.q.topk + kPrUnit - 1) / kPrUnit) : 0;
+  const int sel_rts = kSel ? (g + kRows - 1) / kRows : 0;
+  int64_t sel_item = 0;
+  // selected attention: item i is (token, row tile, head); its sequence comes from the starts
+  auto sel_load = [&](int64_t i) {
+    const int h = static_cast<int>(i % hkv);
+    const int64_t tr = i / hkv;
+    const int t = static_cast<int>(tr / sel_rts);
+    rt = static_cast<int>(tr - static_cast<int64_t>(t) * sel_rts);
+    int c = 0;
+    for (int b = lane; b < a.p.batch; b += 32) c += __ldg(a.p.starts + b + 1) <= t;
+    c = __reduce_add_sync(0xffffffffu, c);
+    it.seq = min(c, a.p.batch - 1);
+    it.head = h;
+    span = load_span(a.p, it.seq);
+    it.tok0 = t;
+    it.r0 = rt * kRows;
+    it.rows = min(kRows, g - it.r0);
+    it.pos0 = 0;
+    it.k0 = 0;
+    it.k1 = a.q.topk;
+    it.u0 = 0;
+    it.u1 = sel_units;
+    // a row before the first sequence or past the last one: nothing is read or written
+    if (c >= a.p.batch || t < span.q0) it.k1 = it.rows = 0;
+  };
+  if (kSel) {
+    units = static_cast<int64_t>(a.p.tokens) * sel_rts * hkv * sel_units;
+    ctas = static_cast<int>(min(static_cast<int64_t>(ctas), units));
+    if (cta >= ctas) return;
+    u_begin = slice_begin(units, ctas, cta);
+    u_end = slice_begin(units, ctas, cta + 1);
+    sel_item = u_begin / sel_units;
+    off = static_cast<int>(u_begin - sel_item * sel_units);
+    sel_load(sel_item);
+  } else {
+    // units of every sequence (per key/value head), summed over the threads' chunks of the batch
+    const int chunk = (a.p.batch + kPrThreads - 1) / kPrThreads;
+    const int b0 = min(a.p.batch, tid * chunk), b1 = min(a.p.batch, b0 + chunk);
+    auto seq_units = [&](int b) {
+      const SeqSpan s = load_span(a.p, b);
+      const int tiles = (s.n * g + kRows - 1) / kRows;
+      int64_t sum = 0;
+      Item x;
+      for (int r = 0; r < tiles; ++r) {
+        range_item<kRows>(a, s, r, x);
+        sum += x.u1 - x.u0;
+      }
+      return sum;
+    };
+    int64_t mine = 0;
+    for (int b = b0; b < b1; ++b) mine += seq_units(b);
+    int64_t incl = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int64_t v = __shfl_up_sync(0xffffffffu, incl, o);
+      if (lane >= o) incl += v;
+    }
+    if (lane == 31) s_scan[warp] = incl;
+    if (tid == 0) s_meta[0] = -1;
+    __syncthreads();
+    int64_t before = 0, all = 0;
+#pragma unroll
+    for (int w = 0; w < kPrWarps; ++w) {
+      if (w < warp) before += s_scan[w];
+      all += s_scan[w];
+    }
+    units = all * hkv;
+    ctas = static_cast<int>(min(static_cast<int64_t>(ctas), units));
+    if (cta >= ctas) return;
+    u_begin = slice_begin(units, ctas, cta);
+    u_end = slice_begin(units, ctas, cta + 1);
+    int64_t at = (before + incl - mine) * hkv;
+    if (u_begin >= at && u_begin < at + mine * hkv) {
+      // the slice begins in this thread's chunk: find the sequence, row tile, head and unit
+      for (int b = b0; b < b1; ++b) {
+        const int64_t w = seq_units(b) * hkv;
+        if (u_begin < at + w) {
+          const SeqSpan s = load_span(a.p, b);
+          Item x;
+          for (int r = 0;; ++r) {
+            range_item<kRows>(a, s, r, x);
+            const int n = x.u1 - x.u0;
+            const int64_t wr = static_cast<int64_t>(n) * hkv;
+            if (u_begin < at + wr) {
+              const int rest = static_cast<int>(u_begin - at);
+              s_meta[0] = b;
+              s_meta[1] = r;
+              s_meta[2] = rest / n;
+              s_meta[3] = rest - rest / n * n;
+              break;
+            }
+            at += wr;
+          }
+          break;
+        }
+        at += w;
+      }
+    }
+    __syncthreads();
+    it.seq = s_meta[0];
+    rt = s_meta[1];
+    it.head = s_meta[2];
+    off = s_meta[3];
+    span = load_span(a.p, it.seq);
+    range_item<kRows>(a, span, rt, it);
+  }
+
+  uint8_t* ring = smem + warp * C::kWarpBytes;
+  const uint32_t ring_u = smem_u32(ring);
+  const uint32_t lm_k = ((lane >> 4) << 3) + (lane & 7);        // key row of a K ldmatrix lane
+  const uint32_t lm_kc = (lane >> 3) & 1;                       // its 16-byte chunk (0/1)
+  const uint32_t lm_v = (((lane >> 3) & 1) << 3) + (lane & 7);  // the same for V (transposed)
+  const uint32_t lm_vc = lane >> 4;
+  bool bad = false;  // a position or page outside the cache was named
+
+  for (int64_t u = u_begin; u < u_end;) {
+    const int n_units = it.u1 - it.u0;
+    const int seg = static_cast<int>(min(static_cast<int64_t>(n_units - off), u_end - u));
+    const int unit0 = it.u0 + off;  // first unit of this segment
+
+    // keys row ra / rb of m-tile m sees: [lo, hi)
+    int lo[MT][2], hi[MT][2];
+#pragma unroll
+    for (int m = 0; m < MT; ++m)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const int r = it.r0 + m * 16 + quad + 8 * e;
+        const int p = it.pos0 + r / g;
+        hi[m][e] = kSel ? it.k1 : min(p + 1, it.k1);
+        lo[m][e] = kSel ? 0 : (a.q.window > 0 ? max(0, p - (a.q.window - 1)) : 0);
+      }
+    // keys that every row sees: tiles inside need no mask
+    int all_lo = it.k0, all_hi = it.k1;
+    if (!kSel) {
+      all_hi = min(all_hi, it.pos0 + it.r0 / g + 1);
+      if (a.q.window > 0)
+        all_lo = max(all_lo, it.pos0 + (it.r0 + it.rows - 1) / g - (a.q.window - 1));
+    }
+
+    // ------------------------------------------------------------ key addresses
+    // Pair pr of the warp's tiles (tiles 2 pr and 2 pr + 1, 32 keys): lane l holds the key of
+    // row l.  raw: its position; then its page; then its offset, each loaded a pair ahead.
+    const int32_t* table = a.p.table + it.seq * a.p.table_stride;
+    const int cap = a.p.max_pages << a.p.page_shift;
+    const int64_t head_off = it.head * a.p.head_stride;
+    auto key_slot = [&](int pr) {  // index of lane l's key in the item's key list
+      return (unit0 + 2 * pr + (lane >> 4)) * kPrUnit + warp * kPrTile + (lane & 15);
+    };
+    auto load_raw = [&](int pr) -> int {
+      const int s = key_slot(pr);
+      if (2 * pr + (lane >> 4) >= seg) return -1;
+      if (!kSel) return s >= it.k0 && s < it.k1 ? s : -1;
+      if (s >= it.k1) return -1;
+      const int64_t at = static_cast<int64_t>(it.tok0) * a.q.idx_stride + s;
+      if (a.q.idx_bytes == 4) return __ldg(static_cast<const int32_t*>(a.q.idx) + at);
+      const int64_t v = __ldg(static_cast<const long long*>(a.q.idx) + at);
+      return v < 0 ? -1 : static_cast<int>(min(v, static_cast<int64_t>(0x7FFFFFFF)));
+    };
+    auto load_entry = [&](int raw) -> int {
+      if (raw < 0) return -1;
+      if (raw >= cap || (kSel && raw >= span.len)) return -2;
+      return __ldg(table + (raw >> a.p.page_shift));
+    };
+    auto to_row = [&](int raw, int entry) -> int64_t {
+      if (raw < 0) return -1;
+      const int64_t r = paged_row(a.p, entry, raw);
+      if (r < 0) bad = true;
+      return r;
+    };
+    int64_t row_now, row_next;
+    int raw2, entry2, raw3;  // of the pairs after row_next's
+    {
+      const int raw0 = load_raw(0), raw1 = load_raw(1);
+      raw2 = load_raw(2);
+      raw3 = load_raw(3);
+      const int e0 = load_entry(raw0), e1 = load_entry(raw1);
+      entry2 = load_entry(raw2);
+      row_now = to_row(raw0, e0);
+      row_next = to_row(raw1, e1);
+    }
+    int load_pair = 0;  // the pair of row_now
+    uint32_t valid_now = __ballot_sync(0xffffffffu, row_now >= 0);
+
+    // issue the copies of tile i of the segment (one group, empty past the end)
+    auto issue = [&](int i) {
+      if (i < seg) {
+        const int pr = i >> 1;
+        if (pr != load_pair) {
+          load_pair = pr;
+          row_now = row_next;
+          row_next = to_row(raw2, entry2);
+          raw2 = raw3;
+          entry2 = load_entry(raw2);
+          raw3 = load_raw(pr + 3);
+          valid_now = __ballot_sync(0xffffffffu, row_now >= 0);
+        }
+        if (lane == 0) s_valid[i % kStages] = (valid_now >> ((i & 1) * 16)) & 0xFFFFu;
+        const uint32_t st = ring_u + (i % kStages) * C::kStageBytes;
+        const int chunk = lane % kLanesPerRow;
+#pragma unroll
+        for (int c = 0; c < kPrTile / kRowsPerCopy; ++c) {
+          const int r = c * kRowsPerCopy + lane / kLanesPerRow;
+          const int64_t row = __shfl_sync(0xffffffffu, row_now, (i & 1) * 16 + r);
+          const bool ok = row >= 0;
+          const int64_t at = (ok ? row : 0) + head_off + chunk * 8;
+          const uint32_t dst = st + r * C::kRowBytes + ((chunk ^ (r & 7)) << 4);
+          cp_async16_fill(dst, a.p.keys + at, ok);
+          cp_async16_fill(dst + C::kTileBytes, a.p.values + at, ok);
+        }
+      }
+      cp_async_commit();
+    };
+
+#pragma unroll
+    for (int i = 0; i < kStages - 1; ++i) issue(i);
+
+    // ------------------------------------------------------------ query fragments
+    uint32_t qf[MT][kKs][4];
+#pragma unroll
+    for (int m = 0; m < MT; ++m) {
+      const int ra = it.r0 + m * 16 + quad, rb = ra + 8;
+      const int lim = it.r0 + it.rows;
+      const uint16_t* pa = a.q.q + static_cast<int64_t>(it.tok0 + ra / g) * a.q.q_ts +
+                           (it.head * g + ra % g) * a.q.q_hs + ql * 2;
+      const uint16_t* pb = a.q.q + static_cast<int64_t>(it.tok0 + rb / g) * a.q.q_ts +
+                           (it.head * g + rb % g) * a.q.q_hs + ql * 2;
+#pragma unroll
+      for (int k = 0; k < kKs; ++k) {
+        qf[m][k][0] = ra < lim ? *reinterpret_cast<const uint32_t*>(pa + k * 16) : 0u;
+        qf[m][k][1] = rb < lim ? *reinterpret_cast<const uint32_t*>(pb + k * 16) : 0u;
+        qf[m][k][2] = ra < lim ? *reinterpret_cast<const uint32_t*>(pa + k * 16 + 8) : 0u;
+        qf[m][k][3] = rb < lim ? *reinterpret_cast<const uint32_t*>(pb + k * 16 + 8) : 0u;
+      }
+    }
+    // ------------------------------------------------------------ the key loop
+    float o[MT][kNt][4];
+    float mx[MT][2], sum[MT][2];
+#pragma unroll
+    for (int m = 0; m < MT; ++m) {
+#pragma unroll
+      for (int n = 0; n < kNt; ++n)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[m][n][e] = 0.f;
+      mx[m][0] = mx[m][1] = -INFINITY;
+      sum[m][0] = sum[m][1] = 0.f;
+    }
+    for (int i = 0; i < seg; ++i) {
+      issue(i + kStages - 1);
+      cp_async_wait<kStages - 1>();
+      __syncwarp();
+      const uint32_t st = ring_u + (i % kStages) * C::kStageBytes;
+      const uint32_t vmask = s_valid[i % kStages];
+      const int base = (unit0 + i) * kPrUnit + warp * kPrTile;
+      float s[MT][2][4];
+#pragma unroll
+      for (int m = 0; m < MT; ++m)
+#pragma unroll
+        for (int n = 0; n < 2; ++n)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) s[m][n][e] = 0.f;
+#pragma unroll
+      for (int k = 0; k < kKs; ++k) {
+        uint32_t b[4];
+        ldsm4(b, st + lm_k * C::kRowBytes + (((2 * k + lm_kc) ^ (lm_k & 7)) << 4));
+#pragma unroll
+        for (int m = 0; m < MT; ++m) {
+          mma16816<kBF16>(s[m][0], qf[m][k], b[0], b[1]);
+          mma16816<kBF16>(s[m][1], qf[m][k], b[2], b[3]);
+        }
+      }
+      const bool whole = vmask == 0xFFFFu && base >= all_lo && base + kPrTile <= all_hi;
+      if (!whole) {
+#pragma unroll
+        for (int m = 0; m < MT; ++m)
+#pragma unroll
+          for (int n = 0; n < 2; ++n)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const int c = n * 8 + ql * 2 + (e & 1);
+              const bool see = ((vmask >> c) & 1u) && base + c >= lo[m][e >> 1] &&
+                               base + c < hi[m][e >> 1];
+              if (!see) s[m][n][e] = -INFINITY;
+            }
+      }
+      // running maximum: the reference moves only when a row's maximum has grown by more than
+      // a factor 2^8 of weight, so most tiles rescale nothing and P stays below 2^8
+      bool grow = false;
+      float top[MT][2];
+#pragma unroll
+      for (int m = 0; m < MT; ++m)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          float t = fmaxf(fmaxf(s[m][0][2 * e], s[m][0][2 * e + 1]),
+                          fmaxf(s[m][1][2 * e], s[m][1][2 * e + 1]));
+          t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 1));
+          t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 2));
+          top[m][e] = t * a.q.scale_log2;
+          grow |= top[m][e] > mx[m][e] + 8.f || (mx[m][e] == -INFINITY && top[m][e] > -INFINITY);
+        }
+      if (__any_sync(0xffffffffu, grow)) {
+#pragma unroll
+        for (int m = 0; m < MT; ++m)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const float now = fmaxf(mx[m][e], top[m][e]);
+            const float f = now == mx[m][e] ? 1.f : exp2_approx(mx[m][e] - now);
+            mx[m][e] = now;
+            sum[m][e] *= f;
+#pragma unroll
+            for (int n = 0; n < kNt; ++n) {
+              o[m][n][2 * e] *= f;
+              o[m][n][2 * e + 1] *= f;
+            }
+          }
+      }
+      uint32_t pf[MT][4];
+#pragma unroll
+      for (int m = 0; m < MT; ++m) {
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const float ref = mx[m][e] == -INFINITY ? 0.f : mx[m][e];
+#pragma unroll
+          for (int n = 0; n < 2; ++n)
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {
+              const float p = exp2_approx(fmaf(s[m][n][2 * e + x], a.q.scale_log2, -ref));
+              s[m][n][2 * e + x] = p;
+              sum[m][e] += p;
+            }
+        }
+        pf[m][0] = pack16<kBF16>(s[m][0][0], s[m][0][1]);
+        pf[m][1] = pack16<kBF16>(s[m][0][2], s[m][0][3]);
+        pf[m][2] = pack16<kBF16>(s[m][1][0], s[m][1][1]);
+        pf[m][3] = pack16<kBF16>(s[m][1][2], s[m][1][3]);
+      }
+      const uint32_t sv = st + C::kTileBytes;
+      bool slow = false;
+      if (!kSel && !whole) {
+        // does a value that only some rows see break the product with zero weights?
+        for (int c = lane; c < kPrTile * kLanesPerRow; c += 32) {
+          uint32_t x[4];
+          asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];"
+                       : "=r"(x[0]), "=r"(x[1]), "=r"(x[2]), "=r"(x[3])
+                       : "r"(sv + c * 16)
+                       : "memory");
+          slow |= nonfinite16<kBF16>(x[0]) || nonfinite16<kBF16>(x[1]) ||
+                  nonfinite16<kBF16>(x[2]) || nonfinite16<kBF16>(x[3]);
+        }
+        slow = __any_sync(0xffffffffu, slow);
+      }
+      if (!slow) {
+#pragma unroll
+        for (int c = 0; c < kKs; ++c) {
+          uint32_t b[4];
+          ldsm4t(b, sv + lm_v * C::kRowBytes + (((2 * c + lm_vc) ^ (lm_v & 7)) << 4));
+#pragma unroll
+          for (int m = 0; m < MT; ++m) {
+            mma16816<kBF16>(o[m][2 * c], pf[m], b[0], b[1]);
+            mma16816<kBF16>(o[m][2 * c + 1], pf[m], b[2], b[3]);
+          }
+        }
+      } else {
+        // element by element, only the keys a row sees
+#pragma unroll
+        for (int n2 = 0; n2 < 2; ++n2)
+#pragma unroll
+          for (int x = 0; x < 2; ++x)
+            for (int src = 0; src < 4; ++src) {
+              const int c = n2 * 8 + src * 2 + x;
+              const bool there = (vmask >> c) & 1u;
+#pragma unroll
+              for (int m = 0; m < MT; ++m) {
+                const float pa = __shfl_sync(0xffffffffu, s[m][n2][x], (lane & ~3) | src);
+                const float pb = __shfl_sync(0xffffffffu, s[m][n2][2 + x], (lane & ~3) | src);
+                const bool va = there && base + c >= lo[m][0] && base + c < hi[m][0];
+                const bool vb = there && base + c >= lo[m][1] && base + c < hi[m][1];
+#pragma unroll
+                for (int n = 0; n < kNt; ++n) {
+                  uint32_t w;
+                  asm volatile("ld.shared.u32 %0, [%1];"
+                               : "=r"(w)
+                               : "r"(sv + c * C::kRowBytes + ((n ^ (c & 7)) << 4) + ql * 4)
+                               : "memory");
+                  const float2 v = unpack16<kBF16>(w);
+                  if (va) {
+                    o[m][n][0] = fmaf(pa, v.x, o[m][n][0]);
+                    o[m][n][1] = fmaf(pa, v.y, o[m][n][1]);
+                  }
+                  if (vb) {
+                    o[m][n][2] = fmaf(pb, v.x, o[m][n][2]);
+                    o[m][n][3] = fmaf(pb, v.y, o[m][n][3]);
+                  }
+                }
+              }
+            }
+      }
+      __syncwarp();  // every lane is done with the stage before the next copies into it
+    }
+    cp_async_wait<0>();
+    __syncwarp();
+
+    // ------------------------------------------------------------ the warps' results meet
+    float* wo = reinterpret_cast<float*>(ring);
+#pragma unroll
+    for (int m = 0; m < MT; ++m)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        float t = sum[m][e];
+        t += __shfl_xor_sync(0xffffffffu, t, 1);
+        t += __shfl_xor_sync(0xffffffffu, t, 2);
+        const int r = m * 16 + quad + 8 * e;
+        if (ql == 0) s_ml[warp * kRows + r] = make_float2(mx[m][e], t);
+        if (r < it.rows) {
+#pragma unroll
+          for (int n = 0; n < kNt; ++n)
+            *reinterpret_cast<float2*>(wo + r * D + n * 8 + ql * 2) =
+                make_float2(o[m][n][2 * e], o[m][n][2 * e + 1]);
+        }
+      }
+    __syncthreads();
+    const bool entire = seg == n_units;
+    const int64_t item_u0 = u - off;  // the item's first unit in the call's list
+    const int c_first = slice_owner(units, ctas, item_u0);
+    const int c_last = slice_owner(units, ctas, item_u0 + n_units - 1);
+    const int slot = 2 * cta + (cta == c_first ? 1 : 0);
+    constexpr int kV = D / 4;            // float4 columns
+    constexpr int kG = kPrThreads / kV;  // row groups
+    const int col = tid % kV, rg = tid / kV;
+    auto store_row = [&](int r, float m, float l, float4 v) {
+      const int row = it.r0 + r;
+      const int64_t t = it.tok0 + row / g;
+      const int h = it.head * g + row % g;
+      const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);  // NaN stays NaN
+      uint2 w;
+      w.x = pack16<kBF16>(v.x * inv, v.y * inv);
+      w.y = pack16<kBF16>(v.z * inv, v.w * inv);
+      if (l == 0.f) w = make_uint2(0u, 0u);
+      *reinterpret_cast<uint2*>(a.q.out + t * a.q.o_ts + h * a.q.o_hs + col * 4) = w;
+      if (a.q.lse && col == 0)
+        a.q.lse[t * a.q.heads + h] = l == 0.f ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f;
+    };
+    for (int r = rg; r < it.rows; r += kG) {
+      float m = -INFINITY;
+#pragma unroll
+      for (int w = 0; w < kPrWarps; ++w) m = fmaxf(m, s_ml[w * kRows + r].x);
+      const float ref = m == -INFINITY ? 0.f : m;
+      float l = 0.f;
+      float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+      for (int w = 0; w < kPrWarps; ++w) {
+        const float2 ml = s_ml[w * kRows + r];
+        const float f = exp2_approx(ml.x - ref);
+        const float4 x = *reinterpret_cast<const float4*>(
+            reinterpret_cast<const float*>(smem + w * C::kWarpBytes) + r * D + col * 4);
+        if (ml.x != -INFINITY) {
+          l += ml.y * f;
+          v.x += x.x * f, v.y += x.y * f, v.z += x.z * f, v.w += x.w * f;
+        } else {
+          l += ml.y;  // zero, or NaN when a score was NaN
+        }
+      }
+      if (entire) {
+        store_row(r, m, l, v);
+      } else {
+        if (col == 0) a.part.ml[static_cast<int64_t>(slot) * kRows + r] = make_float2(m, l);
+        *reinterpret_cast<float4*>(a.part.o + (static_cast<int64_t>(slot) * kRows + r) * D +
+                                   col * 4) = v;
+      }
+    }
+    if (!entire) {
+      __syncthreads();
+      if (tid == 0) {
+        __threadfence();
+        const uint32_t n = static_cast<uint32_t>(c_last - c_first + 1);
+        const uint32_t old = atomicAdd(a.part.counters + c_first, 1u);
+        s_meta[4] = old == n - 1;
+        if (old == n - 1) a.part.counters[c_first] = 0u;
+        __threadfence();
+      }
+      __syncthreads();
+      if (s_meta[4]) {
+        // the last to arrive: partials of CTAs c_first .. c_last, in that order
+        for (int r = rg; r < it.rows; r += kG) {
+          float m = -INFINITY;
+          for (int c = c_first; c <= c_last; ++c) {
+            const int64_t sl = 2 * static_cast<int64_t>(c) + (c == c_first ? 1 : 0);
+            m = fmaxf(m, __ldcg(&a.part.ml[sl * kRows + r]).x);
+          }
+          const float ref = m == -INFINITY ? 0.f : m;
+          float l = 0.f;
+          float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+          for (int c = c_first; c <= c_last; ++c) {
+            const int64_t sl = 2 * static_cast<int64_t>(c) + (c == c_first ? 1 : 0);
+            const float2 ml = __ldcg(&a.part.ml[sl * kRows + r]);
+            const float4 x =
+                __ldcg(reinterpret_cast<const float4*>(a.part.o + (sl * kRows + r) * D) + col);
+            const float f = exp2_approx(ml.x - ref);
+            l += ml.y * f;
+            v.x += x.x * f, v.y += x.y * f, v.z += x.z * f, v.w += x.w * f;
+          }
+          store_row(r, m, l, v);
+        }
+      }
+    }
+
+    // ------------------------------------------------------------ the next item
+    u += seg;
+    if (u >= u_end) break;
+    __syncthreads();  // the ring and s_ml are free again
+    off = 0;
+    if (kSel) {
+      sel_load(++sel_item);
+    } else {
+      if (++it.head == hkv) {
+        it.head = 0;
+        if ((++rt) * kRows >= span.n * g) {
+          rt = 0;
+          do {
+            span = load_span(a.p, ++it.seq);
+          } while (span.n == 0 && it.seq + 1 < a.p.batch);
+        }
+        range_item<kRows>(a, span, rt, it);
+      }
+    }
+  }
+  if (__any_sync(0xffffffffu, bad) && lane == 0) atomicOr(a.status, TDSA_STATUS_RANGE);
+}
+
+template <bool kBF16, int D, int MT, bool kSel>
+int launch_rows_t(RowsArgs a, int ctas, void* ws, cudaStream_t stream) {
+  using C = RowsCfg<D, MT>;
+  a.part = paged_partials(ws, ctas, C::kRows);
+  auto kern = paged_rows_kernel<kBF16, D, MT, kSel>;
+  TDSA_CUDA_CHECK(ensure_dynamic_smem(reinterpret_cast<const void*>(kern), C::kSmem));
+  TDSA_CUDA_CHECK(launch_pdl(kern, dim3(static_cast<unsigned>(ctas)), dim3(kPrThreads), C::kSmem,
+                             stream, a));
+  TDSA_CUDA_CHECK(cudaGetLastError());
+  return TDSA_OK;
+}
+
+template <bool kBF16, int D>
+int launch_rows_d(const RowsArgs& a, int mt, bool sel, int ctas, void* ws, cudaStream_t stream) {
+  if (sel)
+    return mt == 1 ? launch_rows_t<kBF16, D, 1, true>(a, ctas, ws, stream)
+                   : launch_rows_t<kBF16, D, 2, true>(a, ctas, ws, stream);
+  return mt == 1 ? launch_rows_t<kBF16, D, 1, false>(a, ctas, ws, stream)
+                 : launch_rows_t<kBF16, D, 2, false>(a, ctas, ws, stream);
+}
+
+int rows_ctas() { return 2 * device_sm_count(current_device()); }
+
+}  // namespace
+
+size_t paged_rows_workspace_bytes(int dim) { return paged_partial_bytes(rows_ctas(), 32, dim); }
+
+int launch_paged_rows(const PagedView& p, const PagedQuery& q, int dtype, int dim, int rows,
+                      void* ws, int* status, cudaStream_t stream) {
+  RowsArgs a;
+  a.p = p;
+  a.q = q;
+  a.status = status;
+  const int mt = rows <= 16 ? 1 : 2;
+  const bool sel = q.idx != nullptr;
+  const int ctas = rows_ctas();
+  if (dtype == TDSA_BF16)
+    return dim == 128 ? launch_rows_d<true, 128>(a, mt, sel, ctas, ws, stream)
+                      : launch_rows_d<true, 64>(a, mt, sel, ctas, ws, stream);
+  return dim == 128 ? launch_rows_d<false, 128>(a, mt, sel, ctas, ws, stream)
+                    : launch_rows_d<false, 64>(a, mt, sel, ctas, ws, stream);
+}
+
+}  // namespace tdsa

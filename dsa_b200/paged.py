@@ -1,0 +1,259 @@
+"""Paged key/value cache next to the indexer: append, attention of new tokens over the cache,
+and attention over the positions that a top-k selected.
+
+The reference project temporal_dsa stops at the selection of the keys; a decode step goes on
+with these: ``PagedAppender.append`` writes the new tokens' keys (rotated) and values into
+their pages, ``paged_attention`` lets a chunk of new tokens attend to the cache (a prompt's
+chunk, drafted tokens, or one token per sequence), and ``selected_attention`` lets each token
+attend to the positions of its indexer's top-k only.
+
+A cache is two page arrays ``[pages, page_size, kv_heads, head_dim]``; a batch names the
+sequences of one call by a page table, the row ranges of their new tokens and their lengths.
+The new tokens of all sequences are packed: ``[tokens, heads, head_dim]``, sequence ``b`` in
+rows ``query_starts[b]`` to ``query_starts[b + 1] - 1``.  All kernels run on the current torch
+stream; the batch's tensors live on the device, and nothing here waits for it.
+"""
+
+from __future__ import annotations
+
+import ctypes as C
+import math
+
+import torch
+
+from . import _capi as capi
+from .indexer import require_cuda, stream_ptr
+
+_DTYPES = {torch.float16: capi.TDSA_F16, torch.bfloat16: capi.TDSA_BF16}
+
+
+class PagedKV:
+    """The pages of a cache: ``keys`` and ``values`` ``[pages, page_size, kv_heads, head_dim]``,
+    bfloat16 or float16, with the same strides (views of one interleaved buffer have them)."""
+
+    def __init__(self, keys: torch.Tensor, values: torch.Tensor):
+        require_cuda(keys, values)
+        if keys.dim() != 4 or keys.shape != values.shape:
+            raise ValueError("keys and values must be [pages, page_size, kv_heads, head_dim]")
+        if keys.dtype not in _DTYPES or values.dtype != keys.dtype:
+            raise ValueError("keys and values must share a dtype, bfloat16 or float16")
+        if keys.device != values.device:
+            raise ValueError("keys and values must be on one device")
+        if keys.stride() != values.stride() or keys.stride(-1) != 1:
+            raise ValueError("keys and values must have the same strides, 1 on the last axis")
+        self.keys, self.values = keys, values
+        self.pages, self.page_size, self.kv_heads, self.head_dim = keys.shape
+        self.dtype, self.device = keys.dtype, keys.device
+        self._c = capi.TdsaPagedCache(keys.data_ptr(), values.data_ptr(), *keys.stride()[:3],
+                                      *keys.shape, _DTYPES[keys.dtype])
+        self._ref = C.byref(self._c)
+
+    @classmethod
+    def empty(cls, pages: int, page_size: int, kv_heads: int, head_dim: int, *,
+              dtype: torch.dtype = torch.bfloat16, device="cuda") -> "PagedKV":
+        shape = (pages, page_size, kv_heads, head_dim)
+        return cls(torch.empty(shape, dtype=dtype, device=device),
+                   torch.empty(shape, dtype=dtype, device=device))
+
+
+class PagedBatch:
+    """The sequences of a call.  ``page_table`` int32 ``[batch, max_pages]``: position ``p`` of
+    sequence ``b`` is row ``p % page_size`` of page ``page_table[b, p // page_size]``.
+    ``query_starts`` int32 ``[batch + 1]`` and ``lengths`` int32 ``[batch]`` (positions with the
+    new tokens, which are the last ones).  The tensors may be rewritten in place between calls.
+    ``max_new``: the most new tokens a sequence has (default: no bound is known); it chooses
+    the kernel, results do not depend on it."""
+
+    def __init__(self, page_table: torch.Tensor, query_starts: torch.Tensor,
+                 lengths: torch.Tensor, *, max_new: int | None = None):
+        require_cuda(page_table, query_starts, lengths)
+        if page_table.dim() != 2 or page_table.shape[0] < 1 or page_table.shape[1] < 1:
+            raise ValueError("page_table must be [batch, max_pages]")
+        batch = page_table.shape[0]
+        if query_starts.shape != (batch + 1,) or lengths.shape != (batch,):
+            raise ValueError("query_starts must be [batch + 1] and lengths [batch]")
+        for t in (page_table, query_starts, lengths):
+            if t.dtype != torch.int32:
+                raise ValueError("page_table, query_starts and lengths must be int32")
+            if t.stride(-1) != 1:
+                raise ValueError("page_table, query_starts and lengths need unit last stride")
+            if t.device != page_table.device:
+                raise ValueError("page_table, query_starts and lengths must be on one device")
+        if max_new is not None and max_new < 0:
+            raise ValueError("max_new must be >= 0")
+        self.page_table, self.query_starts, self.lengths = page_table, query_starts, lengths
+        self.batch, self.max_new, self.device = batch, max_new, page_table.device
+        self._c = capi.TdsaPagedBatch(page_table.data_ptr(), page_table.stride(0),
+                                      query_starts.data_ptr(), lengths.data_ptr(), batch,
+                                      page_table.shape[1], 0, 0)
+        self._ref = C.byref(self._c)
+
+    def _for(self, tokens: int):
+        self._c.tokens = tokens
+        self._c.max_new = tokens if self.max_new is None else min(self.max_new, tokens)
+        return self._ref
+
+
+def _rows(t: torch.Tensor, cache: PagedKV, heads: int | None, tokens: int | None,
+          name: str) -> capi.TdsaTokenRows:
+    """``t`` [tokens, heads, head_dim] as C rows; strides and alignment are the library's check."""
+    shape = t.shape
+    if len(shape) != 3 or shape[2] != cache.head_dim or (
+            heads is not None and shape[1] != heads) or (
+            tokens is not None and shape[0] != tokens):
+        raise ValueError(f"{name} must be [tokens, {heads or 'heads'}, {cache.head_dim}], "
+                         f"got {list(shape)}")
+    if t.dtype != cache.dtype:
+        raise ValueError(f"{name} must have the cache's dtype")
+    if t.device != cache.device:
+        raise ValueError(f"{name} must be on the cache's device")
+    ts, hs, ds = t.stride()
+    if ds != 1:
+        raise ValueError(f"{name} needs unit stride on the last axis")
+    return capi.TdsaTokenRows(t.data_ptr(), ts, hs)
+
+
+def _check_batch(batch: PagedBatch, cache: PagedKV) -> None:
+    if batch.device != cache.device:
+        raise ValueError("batch and cache must be on one device")
+
+
+_WORKSPACES: dict[tuple[int, int, int], torch.Tensor] = {}
+
+
+def paged_workspace(device: torch.device, head_dim: int) -> torch.Tensor:
+    """Zeroed scratch of the attention calls.  Outside CUDA-graph capture one buffer per
+    (device, stream, head_dim) is kept: calls on one stream run in order and each leaves it
+    ready for the next.  During a capture a fresh one is returned, which the graph keeps."""
+    key = (device.index, stream_ptr(device), head_dim)
+    ws = _WORKSPACES.get(key)
+    capturing = torch.cuda.is_current_stream_capturing()
+    if ws is None or capturing:
+        with torch.cuda.device(device):
+            nbytes = capi.lib().tdsa_paged_workspace_bytes(head_dim)
+        ws = torch.zeros(max(nbytes, 1), device=device, dtype=torch.uint8)
+        if not capturing:
+            _WORKSPACES[key] = ws
+    return ws
+
+
+class PagedAppender:
+    """Appends new tokens to a paged cache, one launch (tdsa_paged_append): keys are rotated by
+    their positions, keys and values go to their pages, and queries are rotated on the way.
+
+    The rotation turns the pairs of the leading ``rope_dim`` features (a multiple of 16; 0 turns
+    nothing) by ``position * inv_freq[j]``: features ``j`` and ``j + rope_dim / 2`` (the layout
+    of ``apply_noninterleaved_rope``), or ``2 j`` and ``2 j + 1`` when ``interleaved``.
+    ``inv_freq`` float32 ``[rope_dim / 2]`` defaults to ``rope_theta ** (-2 j / rope_dim)``.
+    """
+
+    def __init__(self, cache: PagedKV, *, rope_dim: int = 64, rope_theta: float = 10_000.0,
+                 inv_freq: torch.Tensor | None = None, interleaved: bool = False):
+        if rope_dim < 0 or rope_dim % 16 or rope_dim > cache.head_dim:
+            raise ValueError("rope_dim must be a multiple of 16 up to the head dimension")
+        half = rope_dim // 2
+        if inv_freq is None:
+            j = torch.arange(half, device=cache.device, dtype=torch.float64)
+            inv_freq = (rope_theta ** (-j / max(half, 1))).float()
+        require_cuda(inv_freq)
+        if (inv_freq.shape != (half,) or inv_freq.dtype != torch.float32
+                or inv_freq.device != cache.device):
+            raise ValueError("inv_freq must be float32 [rope_dim / 2] on the cache's device")
+        self.cache, self.rope_dim, self.interleaved = cache, int(rope_dim), bool(interleaved)
+        self.inv_freq = inv_freq.contiguous()
+        self._fn = capi.lib().tdsa_paged_append
+
+    def append(self, batch: PagedBatch, k: torch.Tensor, v: torch.Tensor,
+               q: torch.Tensor | None = None, *, positions: torch.Tensor | None = None,
+               q_out: torch.Tensor | None = None) -> torch.Tensor | None:
+        """k, v ``[tokens, kv_heads, head_dim]`` -> cache; returns the rotated ``q`` (in
+        ``q_out``, a new tensor by default, ``q`` itself allowed) or None without ``q``.
+        ``positions`` int64 ``[tokens]`` replaces the tokens' positions in the angles."""
+        cache = self.cache
+        _check_batch(batch, cache)
+        tokens = k.shape[0]
+        kr = _rows(k, cache, cache.kv_heads, None, "k")
+        vr = _rows(v, cache, cache.kv_heads, tokens, "v")
+        qr = qo = None
+        q_heads = 0
+        if q is not None:
+            qr = _rows(q, cache, None, tokens, "q")
+            q_heads = q.shape[1]
+            if q_out is None:
+                q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+            qo = _rows(q_out, cache, q_heads, tokens, "q_out")
+        elif q_out is not None:
+            raise ValueError("q_out needs q")
+        pos = None
+        if positions is not None:
+            if (positions.dtype != torch.int64 or positions.shape != (tokens,)
+                    or positions.device != cache.device or not positions.is_contiguous()):
+                raise ValueError("positions must be contiguous int64 [tokens] on the cache's "
+                                 "device")
+            pos = positions.data_ptr()
+        capi.check(self._fn(cache._ref, batch._for(tokens), C.byref(kr), C.byref(vr),
+                            None if qr is None else C.byref(qr),
+                            None if qo is None else C.byref(qo), q_heads,
+                            self.inv_freq.data_ptr(), self.rope_dim, int(self.interleaved), pos,
+                            stream_ptr(cache.device)))
+        return q_out
+
+
+def _attention_args(q, cache, batch, scale, out, return_lse):
+    _check_batch(batch, cache)
+    qr = _rows(q, cache, None, None, "q")
+    tokens, heads = q.shape[0], q.shape[1]
+    if out is None:
+        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    orr = _rows(out, cache, heads, tokens, "out")
+    lse = (torch.empty(tokens, heads, dtype=torch.float32, device=q.device) if return_lse
+           else None)
+    if scale is None:
+        scale = 1.0 / math.sqrt(cache.head_dim)
+    return qr, orr, out, lse, tokens, heads, scale, paged_workspace(cache.device, cache.head_dim)
+
+
+def paged_attention(q: torch.Tensor, cache: PagedKV, batch: PagedBatch, *,
+                    scale: float | None = None, window: int | None = None,
+                    out: torch.Tensor | None = None, return_lse: bool = False):
+    """Attention of the new tokens over their sequences' cached positions up to their own.
+
+    q ``[tokens, heads, head_dim]`` (heads a multiple of the cache's kv_heads; head ``h`` reads
+    key/value head ``h // (heads // kv_heads)``) -> out of the same shape, and with
+    ``return_lse`` the float32 log-sum-exp ``[tokens, heads]``.  ``window``: a token sees only
+    the last ``window`` positions up to its own.  ``scale`` defaults to ``head_dim ** -0.5``.
+    A token that sees nothing gets zeros and ``-inf``.  The tokens must be in the cache already
+    (``PagedAppender.append``).
+    """
+    if window is not None and window < 1:
+        raise ValueError("window must be >= 1")
+    qr, orr, out, lse, tokens, heads, scale, ws = _attention_args(q, cache, batch, scale, out,
+                                                                  return_lse)
+    capi.check(capi.lib().tdsa_paged_attention(
+        cache._ref, batch._for(tokens), C.byref(qr), heads, scale, window or 0, C.byref(orr),
+        None if lse is None else lse.data_ptr(), ws.data_ptr(), ws.numel(),
+        stream_ptr(cache.device)))
+    return (out, lse) if return_lse else out
+
+
+def selected_attention(q: torch.Tensor, cache: PagedKV, batch: PagedBatch,
+                       indices: torch.Tensor, *, scale: float | None = None,
+                       out: torch.Tensor | None = None, return_lse: bool = False):
+    """Attention of every new token over the positions it lists: ``indices`` int32 or int64
+    ``[tokens, k]``, positions of the token's own sequence in any order, negative entries
+    skipped -- what ``topk`` and ``ScoreTopkPlan`` return.  The rest as ``paged_attention``."""
+    require_cuda(indices)
+    qr, orr, out, lse, tokens, heads, scale, ws = _attention_args(q, cache, batch, scale, out,
+                                                                  return_lse)
+    if indices.dim() != 2 or indices.shape[0] != tokens or indices.shape[1] < 1:
+        raise ValueError("indices must be [tokens, k]")
+    if indices.dtype not in (torch.int32, torch.int64):
+        raise ValueError("indices must be int32 or int64")
+    if indices.stride(-1) != 1 or indices.device != cache.device:
+        raise ValueError("indices need unit last stride, on the cache's device")
+    capi.check(capi.lib().tdsa_selected_attention(
+        cache._ref, batch._for(tokens), C.byref(qr), heads, scale, indices.data_ptr(),
+        indices.element_size(), indices.stride(0), indices.shape[1], C.byref(orr),
+        None if lse is None else lse.data_ptr(), ws.data_ptr(), ws.numel(),
+        stream_ptr(cache.device)))
+    return (out, lse) if return_lse else out

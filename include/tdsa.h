@@ -586,6 +586,108 @@ int tdsa_query_prep(const void* qraw, int64_t qraw_stride, const void* hidden,
                     int64_t w_stride, int dtype, int batch, int rope_dim, float rope_theta,
                     float weight_scale, void* stream);
 
+/*
+ * Paged key/value cache: append of new tokens, attention of new tokens over the cache, and
+ * attention over selected positions.  No counterpart in the reference project, which stops at
+ * the selection: these are the steps that follow it in a decode loop.
+ *
+ * A cache is two arrays of pages, keys and values, [pages][page_size][kv_heads][head_dim] of
+ * `dtype` (TDSA_BF16 or TDSA_F16) with the same strides (elements, multiples of 8; unit stride
+ * on the last axis) and 16-byte aligned bases.  head_dim 64 or 128; page_size a power of two,
+ * 16 to 1024.
+ * A batch names the sequences of one call: page_table [batch][max_pages] device int32, row
+ * stride table_stride (position p of sequence b is row p % page_size of page
+ * page_table[b][p / page_size]); query_starts [batch + 1] device int32, the sequences' new
+ * tokens are rows query_starts[b] .. query_starts[b + 1] - 1 of the packed [tokens] arrays
+ * (ascending; rows outside every sequence are neither read nor written); lengths [batch]
+ * device int32, positions of each sequence with its new tokens, which are its last ones.
+ * max_new is the host's bound on a sequence's new tokens: it chooses a kernel, and results do
+ * not depend on it.  max_pages * page_size <= 2^30.  Table entries are read only where a
+ * position is needed; a page outside [0, pages) raises TDSA_STATUS_RANGE and its positions
+ * count as absent.
+ */
+typedef struct tdsa_paged_cache {
+  void* keys;
+  void* values;
+  int64_t page_stride;
+  int64_t row_stride;
+  int64_t head_stride;
+  int32_t pages;
+  int32_t page_size;
+  int32_t kv_heads;
+  int32_t head_dim;
+  int32_t dtype;
+} tdsa_paged_cache;
+
+typedef struct tdsa_paged_batch {
+  const int32_t* page_table;
+  int64_t table_stride;
+  const int32_t* query_starts;
+  const int32_t* lengths;
+  int32_t batch;
+  int32_t max_pages;
+  int32_t tokens;
+  int32_t max_new;
+} tdsa_paged_batch;
+
+/* Packed rows [tokens][heads][head_dim] of the cache's dtype: token and head strides in
+ * elements (multiples of 8), unit stride on the last axis, 16-byte aligned base. */
+typedef struct tdsa_token_rows {
+  void* data;
+  int64_t token_stride;
+  int64_t head_stride;
+} tdsa_token_rows;
+
+/*
+ * Writes the keys (rotated) and values of every new token into its slot of the cache and, when
+ * q is not NULL, its rotated queries into q_out (which may be q).  The rotation turns the
+ * pairs of the leading rope_dim features (0, or a multiple of 16 up to head_dim), the halves'
+ * j and j + rope_dim / 2 or, with interleaved != 0, neighbours 2 j and 2 j + 1, by the angle
+ * position * inv_freq[j] (device float32 [rope_dim / 2]); positions (device int64 [tokens])
+ * replaces the tokens' positions in the angle, NULL keeps them.  The angle is reduced in
+ * float64, products are float32, rounded once.  A token whose slot is not in the cache
+ * (more new tokens than positions, or a page outside the cache) raises TDSA_STATUS_RANGE and
+ * its key and value are not stored.  One launch on `stream`.
+ */
+int tdsa_paged_append(const tdsa_paged_cache* cache, const tdsa_paged_batch* batch,
+                      const tdsa_token_rows* k, const tdsa_token_rows* v,
+                      const tdsa_token_rows* q, const tdsa_token_rows* q_out, int q_heads,
+                      const float* inv_freq, int rope_dim, int interleaved,
+                      const int64_t* positions, void* stream);
+
+/*
+ * Attention of every new token over its sequence's positions up to its own (the last `window`
+ * of them when window > 0):
+ *   out[t][h] = sum_j softmax_j(scale * q[t][h] . K[j][h / g]) V[j][h / g],  g = q_heads /
+ *   kv_heads;  lse[t][h] = log sum_j exp(scale * q . K[j]) (float32, [tokens][q_heads], NULL:
+ *   not wanted).
+ * A token that sees no key gets out 0 and lse -inf.  float32 scores, maxima and sums; the
+ * softmax weights are rounded to the cache's type for the product with V.  scale > 0.
+ * workspace: tdsa_paged_workspace_bytes bytes, 256-byte aligned, zero before its first use;
+ * every call leaves it ready for the next one on the same stream.
+ */
+int tdsa_paged_attention(const tdsa_paged_cache* cache, const tdsa_paged_batch* batch,
+                         const tdsa_token_rows* q, int q_heads, float scale, int window,
+                         const tdsa_token_rows* out, float* lse, void* workspace,
+                         size_t workspace_bytes, void* stream);
+
+/*
+ * Attention of every new token over the positions it lists: indices [tokens][k] of index_bytes
+ * (4 = int32, 8 = int64), row stride idx_stride, in any order, negative entries skipped (what
+ * tdsa_topk writes, for the sequence's positions).  Every listed position is used as often as
+ * it is listed, whether it comes before the token or not; one at or past its sequence's length
+ * raises TDSA_STATUS_RANGE and is skipped.  Otherwise as tdsa_paged_attention, the workspace
+ * included.
+ */
+int tdsa_selected_attention(const tdsa_paged_cache* cache, const tdsa_paged_batch* batch,
+                            const tdsa_token_rows* q, int q_heads, float scale,
+                            const void* indices, int index_bytes, int64_t idx_stride, int k,
+                            const tdsa_token_rows* out, float* lse, void* workspace,
+                            size_t workspace_bytes, void* stream);
+
+/* Bytes of workspace of the two attention calls on the current device. */
+size_t tdsa_paged_workspace_bytes(int head_dim);
+
 #ifdef __cplusplus
 }
 #endif

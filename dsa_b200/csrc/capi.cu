@@ -229,7 +229,8 @@ int paged_setup(const tdsa_paged_cache* c, const tdsa_paged_batch* b, PagedView&
       c->head_stride % 8)
     return fail(TDSA_ERR_ALIGN,
                 "cache bases must be 16-byte aligned, strides multiples of 8 elements");
-  if (c->page_stride < 0 || c->row_stride < c->head_dim ||
+  if (c->page_stride < 0 || (c->pages > 1 && c->page_stride < c->head_dim) ||
+      c->row_stride < c->head_dim ||
       (c->kv_heads > 1 && c->head_stride < c->head_dim))
     return fail(TDSA_ERR_INVALID, "cache strides overlap the rows");
   if (b->batch < 1 || b->batch > 65535)
@@ -271,11 +272,14 @@ int check_token_rows(const tdsa_token_rows* r, int heads, int dim, const char* n
   return TDSA_OK;
 }
 
-int paged_query(const tdsa_paged_cache* c, const tdsa_token_rows* q, int q_heads, float scale,
+int paged_query(const tdsa_paged_cache* c, int tokens, const tdsa_token_rows* q, int q_heads,
+                float scale,
                 const tdsa_token_rows* out, float* lse, void* ws, size_t ws_bytes,
                 PagedQuery& d) {
   if (q_heads < 1 || q_heads % c->kv_heads)
     return fail(TDSA_ERR_INVALID, "q_heads must be a multiple of kv_heads");
+  if (static_cast<int64_t>(tokens) * q_heads > (int64_t(1) << 30))
+    return fail(TDSA_ERR_UNSUPPORTED, "tokens * q_heads must be at most 2^30");
   int rc = check_token_rows(q, q_heads, c->head_dim, "q");
   if (!rc) rc = check_token_rows(out, q_heads, c->head_dim, "out");
   if (rc) return rc;
@@ -1203,7 +1207,7 @@ int tdsa_paged_append(const tdsa_paged_cache* cache, const tdsa_paged_batch* bat
 
 size_t tdsa_paged_workspace_bytes(int head_dim) {
   if (head_dim != 64 && head_dim != 128) return 0;
-  return paged_rows_workspace_bytes(head_dim);
+  return std::max(paged_rows_workspace_bytes(head_dim), paged_chunk_workspace_bytes(head_dim));
 }
 
 int tdsa_paged_attention(const tdsa_paged_cache* cache, const tdsa_paged_batch* batch,
@@ -1214,13 +1218,16 @@ int tdsa_paged_attention(const tdsa_paged_cache* cache, const tdsa_paged_batch* 
   PagedQuery d;
   int rc = paged_setup(cache, batch, p);
   if (rc || batch->tokens == 0) return rc;
-  rc = paged_query(cache, q, q_heads, scale, out, lse, workspace, workspace_bytes, d);
+  rc = paged_query(cache, batch->tokens, q, q_heads, scale, out, lse, workspace, workspace_bytes, d);
   if (rc) return rc;
   if (window < 0) return fail(TDSA_ERR_INVALID, "window must be >= 0");
   d.window = window;
   int* status = device_status_ptr();
   if (!status) return fail(TDSA_ERR_CUDA, "device status word not available");
   const int64_t rows = static_cast<int64_t>(batch->max_new) * d.group;
+  if (rows > 32)
+    return launch_paged_chunk(p, d, cache->dtype, cache->head_dim, workspace, status,
+                              static_cast<cudaStream_t>(stream));
   return launch_paged_rows(p, d, cache->dtype, cache->head_dim,
                            static_cast<int>(std::min<int64_t>(rows, 1 << 20)), workspace, status,
                            static_cast<cudaStream_t>(stream));
@@ -1235,7 +1242,7 @@ int tdsa_selected_attention(const tdsa_paged_cache* cache, const tdsa_paged_batc
   PagedQuery d;
   int rc = paged_setup(cache, batch, p);
   if (rc || batch->tokens == 0) return rc;
-  rc = paged_query(cache, q, q_heads, scale, out, lse, workspace, workspace_bytes, d);
+  rc = paged_query(cache, batch->tokens, q, q_heads, scale, out, lse, workspace, workspace_bytes, d);
   if (rc) return rc;
   if (!indices) return fail(TDSA_ERR_INVALID, "indices is null");
   if (index_bytes != 4 && index_bytes != 8)

@@ -197,7 +197,7 @@ int launch_qprep(const void* qraw, int64_t qraw_stride, const void* x, int64_t x
                  int64_t q_stride, float* w, int64_t w_stride, int dtype, int batch,
                  int rope_dim, float theta, float scale, cudaStream_t stream);
 
-// ---- paged key/value cache (paged.cuh; paged_append.cu, paged_rows.cu)
+// ---- paged key/value cache (paged.cuh; paged_append.cu, paged_rows.cu, paged_chunk.cu)
 struct PagedView;
 struct PagedQuery;
 int launch_paged_append(const PagedView& p, void* keys, void* values, int dtype, int dim,
@@ -210,6 +210,11 @@ size_t paged_rows_workspace_bytes(int dim);
 // rows: query rows per sequence (or token, selected attention) and key/value head, at most
 int launch_paged_rows(const PagedView& p, const PagedQuery& q, int dtype, int dim, int rows,
                       void* ws, int* status, cudaStream_t stream);
+
+// any number of query rows, on the tensor cores
+size_t paged_chunk_workspace_bytes(int dim);
+int launch_paged_chunk(const PagedView& p, const PagedQuery& q, int dtype, int dim, void* ws,
+                       int* status, cudaStream_t stream);
 
 // Device status word of the current device (allocated with the module, never freed).
 int* device_status_ptr();

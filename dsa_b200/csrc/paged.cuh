@@ -128,4 +128,132 @@ struct PagedQuery {
   int idx_bytes, topk;
 };
 
+// One item: rows [r0, r0 + rows) of the (token, head) rows of a sequence and key/value head.
+struct PagedItem {
+  int seq, head;      // sequence, key/value head
+  int tok0;           // batch row of the sequence's (or the only) token 0
+  int r0, rows;       // row range (row r: token tok0 + r / group, head h * group + r % group)
+  int pos0;           // position of token 0
+  int k0, k1;         // keys any row sees
+  int u0, u1;         // units [u0, u1) of kUnit keys covering them (at least one)
+};
+
+template <int kRows, int kUnit>
+__device__ __forceinline__ void paged_range_item(const PagedQuery& q, const SeqSpan& s, int rt,
+                                                 PagedItem& it) {
+  const int g = q.group;
+  it.tok0 = s.q0;
+  it.r0 = rt * kRows;
+  it.rows = min(kRows, s.n * g - it.r0);
+  it.pos0 = s.len - s.n;
+  const int first = it.pos0 + it.r0 / g;
+  const int last = it.pos0 + (it.r0 + it.rows - 1) / g;
+  it.k1 = max(0, last + 1);
+  it.k0 = q.window > 0 ? max(0, first - (q.window - 1)) : 0;
+  it.k0 = min(it.k0, it.k1);
+  it.u0 = it.k0 / kUnit;
+  it.u1 = max(it.u0 + 1, (it.k1 + kUnit - 1) / kUnit);
+}
+
+// Where CTA `cta` of at most `ctas` begins in the call's list of units (sequence, row tile,
+// head, unit), found by all kThreads threads of the block from the sequences' unit counts.
+struct PagedSlice {
+  int64_t units, begin, end;
+  int ctas;  // CTAs that have work: no more than there are units
+  int seq, row_tile, head, off;
+};
+
+template <int kThreads, int kRows, int kUnit>
+__device__ __forceinline__ PagedSlice paged_find_slice(const PagedView& p, const PagedQuery& q,
+                                                       int ctas, int cta, int64_t* s_scan,
+                                                       int* s_found) {
+  constexpr int kWarps = kThreads / 32;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int chunk = (p.batch + kThreads - 1) / kThreads;
+  const int b0 = min(p.batch, tid * chunk), b1 = min(p.batch, b0 + chunk);
+  auto seq_units = [&](int b) {
+    const SeqSpan s = load_span(p, b);
+    const int tiles = static_cast<int>((static_cast<int64_t>(s.n) * q.group + kRows - 1) / kRows);
+    int64_t sum = 0;
+    PagedItem x;
+    for (int r = 0; r < tiles; ++r) {
+      paged_range_item<kRows, kUnit>(q, s, r, x);
+      sum += x.u1 - x.u0;
+    }
+    return sum;
+  };
+  int64_t mine = 0;
+  for (int b = b0; b < b1; ++b) mine += seq_units(b);
+  int64_t incl = mine;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int64_t v = __shfl_up_sync(0xffffffffu, incl, o);
+    if (lane >= o) incl += v;
+  }
+  if (lane == 31) s_scan[warp] = incl;
+  __syncthreads();
+  int64_t before = 0, all = 0;
+#pragma unroll
+  for (int w = 0; w < kWarps; ++w) {
+    if (w < warp) before += s_scan[w];
+    all += s_scan[w];
+  }
+  PagedSlice r;
+  r.units = all * p.kv_heads;
+  r.ctas = static_cast<int>(min(static_cast<int64_t>(ctas), r.units));
+  r.begin = r.end = 0;
+  if (cta >= r.ctas) return r;
+  r.begin = slice_begin(r.units, r.ctas, cta);
+  r.end = slice_begin(r.units, r.ctas, cta + 1);
+  int64_t at = (before + incl - mine) * p.kv_heads;
+  if (r.begin >= at && r.begin < at + mine * p.kv_heads) {
+    // the slice begins in this thread's chunk of the batch
+    for (int b = b0; b < b1; ++b) {
+      const int64_t w = seq_units(b) * p.kv_heads;
+      if (r.begin >= at + w) {
+        at += w;
+        continue;
+      }
+      const SeqSpan s = load_span(p, b);
+      PagedItem x;
+      for (int t = 0;; ++t) {
+        paged_range_item<kRows, kUnit>(q, s, t, x);
+        const int n = x.u1 - x.u0;
+        const int64_t wr = static_cast<int64_t>(n) * p.kv_heads;
+        if (r.begin < at + wr) {
+          const int64_t rest = r.begin - at;
+          s_found[0] = b;
+          s_found[1] = t;
+          s_found[2] = static_cast<int>(rest / n);
+          s_found[3] = static_cast<int>(rest % n);
+          break;
+        }
+        at += wr;
+      }
+      break;
+    }
+  }
+  __syncthreads();
+  r.seq = s_found[0];
+  r.row_tile = s_found[1];
+  r.head = s_found[2];
+  r.off = s_found[3];
+  return r;
+}
+
+// The item after `it` in the list (there is one).
+template <int kRows, int kUnit>
+__device__ __forceinline__ void paged_next_item(const PagedView& p, const PagedQuery& q,
+                                                SeqSpan& span, int& row_tile, PagedItem& it) {
+  if (++it.head < p.kv_heads) return;
+  it.head = 0;
+  if (static_cast<int64_t>(++row_tile) * kRows >= static_cast<int64_t>(span.n) * q.group) {
+    row_tile = 0;
+    do {
+      span = load_span(p, ++it.seq);
+    } while (span.n == 0 && it.seq + 1 < p.batch);
+  }
+  paged_range_item<kRows, kUnit>(q, span, row_tile, it);
+}
+
 }  // namespace tdsa

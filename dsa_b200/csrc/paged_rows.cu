@@ -101,33 +101,6 @@ __device__ __forceinline__ void cp_async_wait() {
   asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
 }
 
-// One item: rows [r0, r0 + rows) of the (token, head) rows of a sequence and key/value head.
-struct Item {
-  int seq, head;      // sequence, key/value head
-  int tok0;           // batch row of the sequence's (or the only) token 0
-  int r0, rows;       // row range (row r: token tok0 + r / group, head h * group + r % group)
-  int pos0;           // position of token 0
-  int k0, k1;         // keys any row sees
-  int u0, u1;         // units [u0, u1) of 64 keys covering them (at least one)
-};
-
-template <int kRows>
-__device__ __forceinline__ void range_item(const RowsArgs& a, const SeqSpan& s, int rt,
-                                           Item& it) {
-  const int g = a.q.group;
-  it.tok0 = s.q0;
-  it.r0 = rt * kRows;
-  it.rows = min(kRows, s.n * g - it.r0);
-  it.pos0 = s.len - s.n;
-  const int first = it.pos0 + it.r0 / g;
-  const int last = it.pos0 + (it.r0 + it.rows - 1) / g;
-  it.k1 = max(0, last + 1);
-  it.k0 = a.q.window > 0 ? max(0, first - (a.q.window - 1)) : 0;
-  it.k0 = min(it.k0, it.k1);
-  it.u0 = it.k0 / kPrUnit;
-  it.u1 = max(it.u0 + 1, (it.k1 + kPrUnit - 1) / kPrUnit);
-}
-
 template <bool kBF16, int D, int MT, bool kSel>
 __global__ void __launch_bounds__(kPrThreads, 2) paged_rows_kernel(const RowsArgs a) {
   using C = RowsCfg<D, MT>;
@@ -155,7 +128,7 @@ __global__ void __launch_bounds__(kPrThreads, 2) paged_rows_kernel(const RowsArg
   // ---------------------------------------------------------------- this CTA's slice
   int64_t units;       // of the whole call
   int64_t u_begin, u_end;
-  Item it;
+  PagedItem it;
   int rt = 0;          // row tile of the current item
   int off;             // unit of the item the slice begins at
   SeqSpan span;
@@ -195,76 +168,19 @@ __global__ void __launch_bounds__(kPrThreads, 2) paged_rows_kernel(const RowsArg
     off = static_cast<int>(u_begin - sel_item * sel_units);
     sel_load(sel_item);
   } else {
-    // units of every sequence (per key/value head), summed over the threads' chunks of the batch
-    const int chunk = (a.p.batch + kPrThreads - 1) / kPrThreads;
-    const int b0 = min(a.p.batch, tid * chunk), b1 = min(a.p.batch, b0 + chunk);
-    auto seq_units = [&](int b) {
-      const SeqSpan s = load_span(a.p, b);
-      const int tiles = (s.n * g + kRows - 1) / kRows;
-      int64_t sum = 0;
-      Item x;
-      for (int r = 0; r < tiles; ++r) {
-        range_item<kRows>(a, s, r, x);
-        sum += x.u1 - x.u0;
-      }
-      return sum;
-    };
-    int64_t mine = 0;
-    for (int b = b0; b < b1; ++b) mine += seq_units(b);
-    int64_t incl = mine;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int64_t v = __shfl_up_sync(0xffffffffu, incl, o);
-      if (lane >= o) incl += v;
-    }
-    if (lane == 31) s_scan[warp] = incl;
-    if (tid == 0) s_meta[0] = -1;
-    __syncthreads();
-    int64_t before = 0, all = 0;
-#pragma unroll
-    for (int w = 0; w < kPrWarps; ++w) {
-      if (w < warp) before += s_scan[w];
-      all += s_scan[w];
-    }
-    units = all * hkv;
-    ctas = static_cast<int>(min(static_cast<int64_t>(ctas), units));
+    const PagedSlice sl = paged_find_slice<kPrThreads, kRows, kPrUnit>(a.p, a.q, ctas, cta,
+                                                                      s_scan, s_meta);
+    units = sl.units;
+    ctas = sl.ctas;
     if (cta >= ctas) return;
-    u_begin = slice_begin(units, ctas, cta);
-    u_end = slice_begin(units, ctas, cta + 1);
-    int64_t at = (before + incl - mine) * hkv;
-    if (u_begin >= at && u_begin < at + mine * hkv) {
-      // the slice begins in this thread's chunk: find the sequence, row tile, head and unit
-      for (int b = b0; b < b1; ++b) {
-        const int64_t w = seq_units(b) * hkv;
-        if (u_begin < at + w) {
-          const SeqSpan s = load_span(a.p, b);
-          Item x;
-          for (int r = 0;; ++r) {
-            range_item<kRows>(a, s, r, x);
-            const int n = x.u1 - x.u0;
-            const int64_t wr = static_cast<int64_t>(n) * hkv;
-            if (u_begin < at + wr) {
-              const int rest = static_cast<int>(u_begin - at);
-              s_meta[0] = b;
-              s_meta[1] = r;
-              s_meta[2] = rest / n;
-              s_meta[3] = rest - rest / n * n;
-              break;
-            }
-            at += wr;
-          }
-          break;
-        }
-        at += w;
-      }
-    }
-    __syncthreads();
-    it.seq = s_meta[0];
-    rt = s_meta[1];
-    it.head = s_meta[2];
-    off = s_meta[3];
+    u_begin = sl.begin;
+    u_end = sl.end;
+    it.seq = sl.seq;
+    it.head = sl.head;
+    rt = sl.row_tile;
+    off = sl.off;
     span = load_span(a.p, it.seq);
-    range_item<kRows>(a, span, rt, it);
+    paged_range_item<kRows, kPrUnit>(a.q, span, rt, it);
   }
 
   uint8_t* ring = smem + warp * C::kWarpBytes;
@@ -674,16 +590,7 @@ __global__ void __launch_bounds__(kPrThreads, 2) paged_rows_kernel(const RowsArg
     if (kSel) {
       sel_load(++sel_item);
     } else {
-      if (++it.head == hkv) {
-        it.head = 0;
-        if ((++rt) * kRows >= span.n * g) {
-          rt = 0;
-          do {
-            span = load_span(a.p, ++it.seq);
-          } while (span.n == 0 && it.seq + 1 < a.p.batch);
-        }
-        range_item<kRows>(a, span, rt, it);
-      }
+      paged_next_item<kRows, kPrUnit>(a.p, a.q, span, rt, it);
     }
   }
   if (__any_sync(0xffffffffu, bad) && lane == 0) atomicOr(a.status, TDSA_STATUS_RANGE);

@@ -28,7 +28,11 @@ namespace tdsa {
 
 namespace {
 
-constexpr int kPcThreads = 320;
+constexpr int kPcThreads = 384;        // warps 10 and 11 only fill the third warpgroup
+// Registers per thread: 168 at launch (65536 / 384); the third warpgroup gives 96 of its own to
+// the two that hold rows.  2 * 216 + 72 = 3 * 168.
+constexpr int kPcRegsRows = 216, kPcRegsRest = 72;
+static_assert(2 * kPcRegsRows + kPcRegsRest <= 3 * 168, "registers of the launch");
 constexpr int kPcTile = 128;           // rows of a tile
 constexpr int kPcRows = 2 * kPcTile;   // rows of an item
 constexpr int kPcUnit = 128;           // keys of a unit
@@ -67,8 +71,27 @@ __device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t* r) {
       "r"(r[29]), "r"(r[30]), "r"(r[31])
       : "memory");
 }
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t* r) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], "
+      "{%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(taddr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]),
+      "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]),
+      "r"(r[15])
+      : "memory");
+}
 __device__ __forceinline__ void tmem_wait_st() {
   asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+      "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]),
+        "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]),
+        "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(taddr)
+      : "memory");
 }
 __device__ __forceinline__ uint32_t tmem_ld1(uint32_t taddr) {
   uint32_t r;
@@ -123,6 +146,89 @@ __device__ __forceinline__ bool tile_any(int t, bool v) {
   return r != 0;
 }
 
+template <int N>
+__device__ __forceinline__ void regs_inc() {
+  asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
+}
+template <int N>
+__device__ __forceinline__ void regs_dec() {
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
+}
+
+// Two float32 at once (one issue slot): a * b + c, a + b.
+__device__ __forceinline__ uint64_t pair(float lo, float hi) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+  return r;
+}
+__device__ __forceinline__ float2 unpair(uint64_t v) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+  return r;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+
+// O += P V of one unit for one row, element by element over the keys [j0, j1) that the row
+// sees: P from TMEM (s_addr), V from its swizzled unit in shared memory.  first: O starts at 0.
+template <bool kBF16, int D>
+__device__ __noinline__ void add_visible(uint32_t s_addr, uint32_t o_addr, const uint8_t* sv,
+                                         int j0, int j1, bool first) {
+  for (int c = 0; c < D / 32; ++c) {
+    uint32_t o[32];
+    __syncwarp();
+    if (!first) {
+      tmem_ld32(o_addr + c * 32, o);
+      tmem_wait_ld();
+    } else {
+#pragma unroll
+      for (int x = 0; x < 32; ++x) o[x] = 0u;
+    }
+    for (int jp = 0; jp < kPcUnit / 2; ++jp) {
+      __syncwarp();
+      const uint32_t w = tmem_ld1(s_addr + jp);
+      tmem_wait_ld();
+      const float2 pw = unpack16<kBF16>(w);
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const int j = 2 * jp + e;
+        if (j < j0 || j >= j1) continue;
+        const float pj = e ? pw.y : pw.x;
+        const uint8_t* vr = sv + (c >> 1) * kPcHalf + j * 128;
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+          const uint4 v =
+              *reinterpret_cast<const uint4*>(vr + ((((c & 1) * 4 + x) ^ (j & 7)) << 4));
+          const uint32_t vv[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+          for (int y = 0; y < 4; ++y) {
+            const float2 f = unpack16<kBF16>(vv[y]);
+            const int at = x * 8 + y * 2;
+            o[at] = __float_as_uint(fmaf(pj, f.x, __uint_as_float(o[at])));
+            o[at + 1] = __float_as_uint(fmaf(pj, f.y, __uint_as_float(o[at + 1])));
+          }
+        }
+      }
+    }
+    __syncwarp();
+    tmem_st32(o_addr + c * 32, o);
+    tmem_wait_st();
+  }
+}
+
 // A warp's wait: every lane gets the same answer, so a wait that runs out ends the whole warp.
 __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity,
                                           volatile int* abort_flag) {
@@ -150,8 +256,8 @@ __global__ void __launch_bounds__(kPcThreads, 1)
   volatile int* skip = abort_flag + 1;   // [tile] this unit's product was formed by the threads
   int* s_last = const_cast<int*>(abort_flag) + 3;  // [tile]
   int* s_found = s_last + 2;             // [4]
-  // [unit mod 16]: bit b is set when box b of the unit names no page of the cache (the ring
-  // holds fewer than 16 units)
+  // [unit mod 16]: bit b is set when keys 16 b .. 16 b + 15 of the unit lie in a page that is
+  // not the cache's (the ring holds fewer than 16 units)
   volatile uint32_t* absent = reinterpret_cast<volatile uint32_t*>(s_found + 4);
   int64_t* s_scan = reinterpret_cast<int64_t*>(
       (reinterpret_cast<uintptr_t>(s_found + 20) + 7) & ~uintptr_t(7));  // [10]
@@ -215,6 +321,7 @@ __global__ void __launch_bounds__(kPcThreads, 1)
     }
   };
 
+  if (warp >= 8) regs_dec<kPcRegsRest>();
   if (warp == 8) {
     // ------------------------------------------------------------ copies of K and V
     const int box = a.page_box, boxes = kPcUnit / box;
@@ -234,8 +341,9 @@ __global__ void __launch_bounds__(kPcThreads, 1)
         const int pos = (unit0 + i) * kPcUnit + lane * box;
         int page = entry;
         if (page < 0 || page > a.p.pages) page = a.p.pages;
+        const bool none = page == a.p.pages && lane < boxes && pos < it.k1 && pos + box > it.k0;
         const uint32_t gone = __ballot_sync(
-            0xffffffffu, page == a.p.pages && lane < boxes && pos < it.k1 && pos + box > it.k0);
+            0xffffffffu, __shfl_sync(0xffffffffu, none, (lane * 16 / box) & 31) && lane < 8);
         bad |= gone != 0u;
         if (lane == 0) absent[(n_loads >> 1) & 15] = gone;
         entry = entry_of(i + 1);
@@ -352,8 +460,9 @@ __global__ void __launch_bounds__(kPcThreads, 1)
     __syncwarp();
     volatile int no_abort = 0;
     mbar_wait(done, 0, &no_abort);
-  } else {
+  } else if (warp < 8) {
     // ------------------------------------------------------------ rows: softmax and output
+    regs_inc<kPcRegsRows>();
     const int t = warp >> 2;                      // tile
     const int row = (warp & 3) * 32 + lane;       // of the tile; also the TMEM lane
     const uint32_t lane_base = static_cast<uint32_t>(warp & 3) << 21;
@@ -398,28 +507,32 @@ __global__ void __launch_bounds__(kPcThreads, 1)
         const int base = (unit0 + i) * kPcUnit;
         if (!warp_wait(&sfull[t], s_n++ & 1u, abort_flag)) return false;
         tc_fence_after();
-        uint32_t s[128];
+        uint32_t s[4][32];
 #pragma unroll
-        for (int c = 0; c < 4; ++c)
-          tmem_ld32(s_addr + c * 32, *reinterpret_cast<uint32_t(*)[32]>(s + c * 32));
+        for (int c = 0; c < 4; ++c) tmem_ld32(s_addr + c * 32, s[c]);
         tmem_wait_ld();
         const bool masked = base < all_lo || base + kPcUnit > all_hi;
         if (masked) {
 #pragma unroll
           for (int j = 0; j < 128; ++j)
-            if (base + j < lo || base + j >= hi) s[j] = 0xFF800000u;  // -infinity
+            if (base + j < lo || base + j >= hi) s[j >> 5][j & 31] = 0xFF800000u;  // -infinity
         }
         const uint32_t gone = absent[((v0 >> 1) + i) & 15];
         if (gone) {
-          const int per = 31 - __clz(a.page_box);
 #pragma unroll
           for (int j = 0; j < 128; ++j)
-            if ((gone >> (j >> per)) & 1u) s[j] = 0xFF800000u;
+            if ((gone >> (j >> 4)) & 1u) s[j >> 5][j & 31] = 0xFF800000u;
         }
-        float top = __uint_as_float(s[0]);
+        float tops[4];
 #pragma unroll
-        for (int j = 1; j < 128; ++j) top = fmaxf(top, __uint_as_float(s[j]));
-        top *= a.q.scale_log2;
+        for (int c = 0; c < 4; ++c) {
+          tops[c] = __uint_as_float(s[c][0]);
+#pragma unroll
+          for (int j = 1; j < 31; j += 2)
+            tops[c] = max3(tops[c], __uint_as_float(s[c][j]), __uint_as_float(s[c][j + 1]));
+          tops[c] = fmaxf(tops[c], __uint_as_float(s[c][31]));
+        }
+        const float top = fmaxf(max3(tops[0], tops[1], tops[2]), tops[3]) * a.q.scale_log2;
         const bool grow = top > ref + 8.f;
         if (__any_sync(0xffffffffu, grow)) {
           const float now = fmaxf(ref, top);
@@ -428,33 +541,36 @@ __global__ void __launch_bounds__(kPcThreads, 1)
           sum *= f;
           if (i > 0) {
 #pragma unroll
-            for (int c = 0; c < D / 32; ++c) {
-              uint32_t o[32];
-              tmem_ld32(o_addr + c * 32, o);
+            for (int c = 0; c < D / 16; ++c) {
+              uint32_t o[16];
+              tmem_ld16(o_addr + c * 16, o);
               tmem_wait_ld();
 #pragma unroll
-              for (int j = 0; j < 32; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * f);
-              tmem_st32(o_addr + c * 32, o);
+              for (int j = 0; j < 16; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * f);
+              tmem_st16(o_addr + c * 16, o);
             }
           }
         }
         const float neg = ref == -INFINITY ? 0.f : -ref;
-        float part[4] = {0.f, 0.f, 0.f, 0.f};
+        const uint64_t scale2 = pair(a.q.scale_log2, a.q.scale_log2), neg2 = pair(neg, neg);
+        uint64_t part[2] = {0ull, 0ull};
 #pragma unroll
-        for (int c = 0; c < 2; ++c) {
-          uint32_t p[32];
+        for (int c = 0; c < 4; ++c) {
+          uint32_t p[16];
 #pragma unroll
-          for (int j = 0; j < 32; ++j) {
-            const float x = exp2_approx(
-                fmaf(__uint_as_float(s[c * 64 + 2 * j]), a.q.scale_log2, neg));
-            const float y = exp2_approx(
-                fmaf(__uint_as_float(s[c * 64 + 2 * j + 1]), a.q.scale_log2, neg));
-            part[j & 3] += x + y;
-            p[j] = pack16<kBF16>(x, y);
+          for (int j = 0; j < 16; ++j) {
+            const float2 x = unpair(fma2(
+                pair(__uint_as_float(s[c][2 * j]), __uint_as_float(s[c][2 * j + 1])), scale2, neg2));
+            const float e0 = exp2_approx(x.x), e1 = exp2_approx(x.y);
+            part[j & 1] = add2(part[j & 1], pair(e0, e1));
+            p[j] = pack16<kBF16>(e0, e1);
           }
-          tmem_st32(s_addr + c * 32, p);
+          tmem_st16(s_addr + c * 16, p);
         }
-        sum += (part[0] + part[1]) + (part[2] + part[3]);
+        {
+          const float2 x = unpair(add2(part[0], part[1]));
+          sum += x.x + x.y;
+        }
         tmem_wait_st();
         bool alone = false;
         if (masked) {
@@ -475,48 +591,9 @@ __global__ void __launch_bounds__(kPcThreads, 1)
             }
           }
           alone = tile_any(t, odd);
-          if (alone) {
-            const int j0 = max(0, lo - base), j1 = min(kPcUnit, hi - base);
-            for (int c = 0; c < D / 32; ++c) {
-              uint32_t o[32];
-              if (i > 0) {
-                tmem_ld32(o_addr + c * 32, o);
-                tmem_wait_ld();
-              } else {
-#pragma unroll
-                for (int x = 0; x < 32; ++x) o[x] = 0u;
-              }
-              for (int jp = 0; jp < kPcUnit / 2; ++jp) {
-                __syncwarp();
-                const uint32_t w = tmem_ld1(s_addr + jp);
-                tmem_wait_ld();
-                const float2 pw = unpack16<kBF16>(w);
-#pragma unroll
-                for (int e = 0; e < 2; ++e) {
-                  const int j = 2 * jp + e;
-                  if (j < j0 || j >= j1) continue;
-                  const float pj = e ? pw.y : pw.x;
-                  const uint8_t* vr = sv + (c >> 1) * kPcHalf + j * 128;
-#pragma unroll
-                  for (int x = 0; x < 4; ++x) {
-                    const uint4 v = *reinterpret_cast<const uint4*>(
-                        vr + ((((c & 1) * 4 + x) ^ (j & 7)) << 4));
-                    const uint32_t vv[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-                    for (int y = 0; y < 4; ++y) {
-                      const float2 f = unpack16<kBF16>(vv[y]);
-                      const int at = x * 8 + y * 2;
-                      o[at] = __float_as_uint(fmaf(pj, f.x, __uint_as_float(o[at])));
-                      o[at + 1] = __float_as_uint(fmaf(pj, f.y, __uint_as_float(o[at + 1])));
-                    }
-                  }
-                }
-              }
-              __syncwarp();
-              tmem_st32(o_addr + c * 32, o);
-              tmem_wait_st();
-            }
-          }
+          if (alone)
+            add_visible<kBF16, D>(s_addr, o_addr, sv, max(0, lo - base), min(kPcUnit, hi - base),
+                                  i == 0);
         }
         if (row == 0) skip[t] = alone ? 1 : 0;
         tc_fence_before();

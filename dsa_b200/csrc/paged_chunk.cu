@@ -3,24 +3,30 @@
 //   out[t,h] = sum_j softmax_j(scale q[t,h].K[j]) V[j] over the keys j that token t sees.
 //
 // An item is 256 query rows -- the (token, head) rows that share one key/value head -- in two
-// tiles of 128, and walks its keys in units of 128.  One CTA per SM; roles:
+// tiles of 128, and walks its keys in units of 128, each in two parts of 64.  One CTA per SM;
+// roles:
 //   warps 0-3, 4-7: one tile each, one row per thread (softmax, output);
-//   warp 8: page lookups and TMA copies of K and V units into a ring in shared memory;
-//   warp 9: tcgen05 products, S = Q K^T (both from shared memory) and O += P V (P from TMEM).
-// TMEM holds S (128 columns) and O (D columns) of both tiles; P, 16-bit, takes the place of S
-// once its thread has read the row.  The two tiles alternate: while one tile's rows take their
-// exponentials, the tensor core runs the other tile's products, and a unit of K and V is
-// fetched once for both.
+//   warp 8: the CTA's list of items, page lookups and TMA copies of K and V units into a ring
+//     in shared memory (a unit is fetched once for both tiles);
+//   warps 9, 10: one tile's tcgen05 products each, S = Q K^T (both from shared memory) and
+//     O += P V (P from TMEM).
+// TMEM holds two S buffers (64 columns) and O (D columns) per tile; P, 16-bit, takes the place
+// of S once its thread has read the row.  S of part n + 2 is issued behind O += P V of part n,
+// so a row finds the scores of its next part ready when it is done with one, and the time from
+// P to the next S (products, and 500 cycles of their start and completion) is hidden behind a
+// part's exponentials.  With one 128-wide S buffer per tile that time was not hidden: 3980
+// cycles a unit against 2048 of products.
 //
-// S is only issued for unit i + 1 after O += P V of unit i, and tensor products of one CTA
-// complete in the order of their issue, so the completion of S(i + 1) also says that O is at
-// rest: the thread that owns a row then rescales it in place when the row's maximum has grown
-// by a factor of more than 2^8 (rare after the first units), with no extra hand-shake.
+// The products that one thread issues complete in order, so the completion of S(n + 1) also
+// says that O += P V of part n - 1 is done: the thread that owns a row waits for it before it
+// rescales its row of O in place, which it does only when the row's maximum has grown by a
+// factor of more than 2^8 of weight (rare after the first units).
 //
 // Scores, maxima, sums and O are float32.  P is rounded to the cache's type for the second
 // product (2^-8 relative in bf16, 2^-11 in f16, the rounding that the output gets too); the sum
 // adds the unrounded P.
 #include <algorithm>
+#include <type_traits>
 
 #include "paged.cuh"
 
@@ -28,14 +34,12 @@ namespace tdsa {
 
 namespace {
 
-constexpr int kPcThreads = 384;        // warps 10 and 11 only fill the third warpgroup
-// Registers per thread: 168 at launch (65536 / 384); the third warpgroup gives 96 of its own to
-// the two that hold rows.  2 * 216 + 72 = 3 * 168.
-constexpr int kPcRegsRows = 216, kPcRegsRest = 72;
-static_assert(2 * kPcRegsRows + kPcRegsRest <= 3 * 168, "registers of the launch");
+constexpr int kPcThreads = 352;
 constexpr int kPcTile = 128;           // rows of a tile
 constexpr int kPcRows = 2 * kPcTile;   // rows of an item
 constexpr int kPcUnit = 128;           // keys of a unit
+constexpr int kPcPart = 64;            // keys of a part of a unit
+constexpr int kPcPolyOf8 = 3;          // of 8 pairs of exponentials, on the fma pipe
 constexpr int kPcHalf = kPcUnit * 128; // bytes of a 64-wide half of a unit (or of a Q tile)
 
 struct ChunkArgs {
@@ -100,14 +104,49 @@ __device__ __forceinline__ uint32_t tmem_ld1(uint32_t taddr) {
   return r;
 }
 
-// D[tmem] (+)= A[tmem] * B[smem desc], kind::f16, A's 16-bit values packed two to a column.
-__device__ __forceinline__ void umma_f16_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t bdesc,
-                                            uint32_t idesc, uint32_t accumulate) {
+// One lane of a converged warp.
+__device__ __forceinline__ uint32_t elect_one() {
+  uint32_t r;
   asm volatile(
       "{\n\t.reg .pred p;\n\t"
+      "elect.sync _|p, 0xffffffff;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}\n"
+      : "=r"(r));
+  return r;
+}
+
+// The products are issued by the whole warp under the predicate of one lane: their operands
+// stay in uniform registers, where a branch on the lane would move each of them there first
+// (a group of eight took 720 to 910 cycles to issue that way, longer than it takes to run).
+// D[tmem] (+)= A[smem desc] * B[smem desc]^T, kind::f16.
+__device__ __forceinline__ void umma_ss(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc,
+                                        uint32_t idesc, uint32_t accumulate, uint32_t on) {
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t"
       "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}\n" ::"r"(d_tmem),
-      "r"(a_tmem), "l"(bdesc), "r"(idesc), "r"(accumulate)
+      "setp.ne.b32 q, %5, 0;\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}\n" ::"r"(d_tmem),
+      "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate), "r"(on)
+      : "memory");
+}
+// D[tmem] (+)= A[tmem] * B[smem desc], A's 16-bit values packed two to a column.
+__device__ __forceinline__ void umma_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t bdesc,
+                                        uint32_t idesc, uint32_t accumulate, uint32_t on) {
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "setp.ne.b32 q, %5, 0;\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}\n" ::"r"(d_tmem),
+      "r"(a_tmem), "l"(bdesc), "r"(idesc), "r"(accumulate), "r"(on)
+      : "memory");
+}
+__device__ __forceinline__ void umma_commit_on(uint64_t* bar, uint32_t on) {
+  asm volatile(
+      "{\n\t.reg .pred q;\n\t"
+      "setp.ne.b32 q, %1, 0;\n\t"
+      "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}\n" ::
+          "r"(smem_u32(bar)),
+      "r"(on)
       : "memory");
 }
 
@@ -127,32 +166,6 @@ __device__ __forceinline__ void tma_load_4d(void* dst, const CUtensorMap* map, u
       "l"(reinterpret_cast<uint64_t>(map)), "r"(smem_u32(bar)), "r"(c0), "r"(c1), "r"(c2),
       "r"(c3)
       : "memory");
-}
-
-// Barrier of the 128 threads of tile t (named barrier 1 + t).
-__device__ __forceinline__ void tile_sync(int t) {
-  asm volatile("bar.sync %0, 128;" ::"r"(1 + t) : "memory");
-}
-__device__ __forceinline__ bool tile_any(int t, bool v) {
-  int r;
-  asm volatile(
-      "{\n\t.reg .pred p, q;\n\t"
-      "setp.ne.b32 p, %2, 0;\n\t"
-      "bar.red.or.pred q, %1, 128, p;\n\t"
-      "selp.b32 %0, 1, 0, q;\n\t}\n"
-      : "=r"(r)
-      : "r"(1 + t), "r"(static_cast<int>(v))
-      : "memory");
-  return r != 0;
-}
-
-template <int N>
-__device__ __forceinline__ void regs_inc() {
-  asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
-}
-template <int N>
-__device__ __forceinline__ void regs_dec() {
-  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
 }
 
 // Two float32 at once (one issue slot): a * b + c, a + b.
@@ -182,8 +195,8 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
   return r;
 }
 
-// O += P V of one unit for one row, element by element over the keys [j0, j1) that the row
-// sees: P from TMEM (s_addr), V from its swizzled unit in shared memory.  first: O starts at 0.
+// O += P V of one part for one row, element by element over its keys [j0, j1) that the row
+// sees: P from TMEM (s_addr), V from its swizzled rows in shared memory.  first: O starts at 0.
 template <bool kBF16, int D>
 __device__ __noinline__ void add_visible(uint32_t s_addr, uint32_t o_addr, const uint8_t* sv,
                                          int j0, int j1, bool first) {
@@ -197,7 +210,7 @@ __device__ __noinline__ void add_visible(uint32_t s_addr, uint32_t o_addr, const
 #pragma unroll
       for (int x = 0; x < 32; ++x) o[x] = 0u;
     }
-    for (int jp = 0; jp < kPcUnit / 2; ++jp) {
+    for (int jp = 0; jp < kPcPart / 2; ++jp) {
       __syncwarp();
       const uint32_t w = tmem_ld1(s_addr + jp);
       tmem_wait_ld();
@@ -235,6 +248,34 @@ __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity,
   return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag));
 }
 
+// 2^x of two values on the fma pipe, for -126 <= x (smaller ones are taken as -126) and x well
+// below 2^22: x = n + f with n the nearest integer (read off the low bits of x + 1.5 2^23) and
+// |f| <= 1/2, 2^f by the degree-4 polynomial of least largest relative error (2.6e-6, found by
+// Remez exchange), n added to the exponent.
+__device__ __forceinline__ float2 exp2_poly2(uint64_t x2) {
+  const float2 v = unpair(x2);
+  const uint64_t x = pair(fmaxf(v.x, -126.f), fmaxf(v.y, -126.f));
+  const uint64_t magic = pair(12582912.f, 12582912.f);
+  const uint64_t r = add2(x, magic);
+  const uint64_t n = add2(r, pair(-12582912.f, -12582912.f));
+  const uint64_t f = fma2(n, pair(-1.f, -1.f), x);
+  uint64_t p = fma2(pair(0x1.3997d6p-7f, 0x1.3997d6p-7f), f, pair(0x1.ca1440p-5f, 0x1.ca1440p-5f));
+  p = fma2(p, f, pair(0x1.ec06dap-3f, 0x1.ec06dap-3f));
+  p = fma2(p, f, pair(0x1.62e0dcp-1f, 0x1.62e0dcp-1f));
+  p = fma2(p, f, pair(0x1.ffffe8p-1f, 0x1.ffffe8p-1f));
+  const float2 pv = unpair(p), rv = unpair(r);
+  return make_float2(__uint_as_float(__float_as_uint(pv.x) + (__float_as_uint(rv.x) << 23)),
+                     __uint_as_float(__float_as_uint(pv.y) + (__float_as_uint(rv.y) << 23)));
+}
+
+// A segment of an item, published by the copy warp to the others.
+struct ChunkSegment {
+  int unit0, units;    // first unit and number of units (0: the CTA's list ends)
+  int item_units, pad;
+  int64_t item_u0;     // the item's first unit in the call's list
+  int head, tok0, r0, rows, pos0, k0, k1, pad2;
+};
+
 template <bool kBF16, int D>
 __global__ void __launch_bounds__(kPcThreads, 1)
     paged_chunk_kernel(const __grid_constant__ CUtensorMap kmap,
@@ -247,35 +288,44 @@ __global__ void __launch_bounds__(kPcThreads, 1)
   uint64_t* full = reinterpret_cast<uint64_t*>(s_q + C::kQ);
   uint64_t* empty = full + C::kStages;
   uint64_t* qfull = empty + C::kStages;  // [tile]
-  uint64_t* sfull = qfull + 2;           // [tile] S is complete (and O at rest)
-  uint64_t* pfull = sfull + 2;           // [tile] P is in TMEM, O rescaled or read out
-  uint64_t* ofull = pfull + 2;           // [tile] the segment's last product is complete
-  uint64_t* done = ofull + 2;
-  uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(done + 1);
+  uint64_t* sfull = qfull + 2;           // [tile][buffer] S(n) and O += P V (n - 2) are complete
+  uint64_t* pfull = sfull + 4;           // [tile][buffer] P(n) is in TMEM, O rescaled or read out
+  uint64_t* met = pfull + 4;             // [tile] the tile's four warps meet
+  uint64_t* gfull = met + 2;             // [2] a segment is published
+  uint64_t* gempty = gfull + 2;          // [2] everyone is done with it
+  uint64_t* done = gempty + 2;           // [tile]
+  uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(done + 2);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_holder + 1);
-  volatile int* skip = abort_flag + 1;   // [tile] this unit's product was formed by the threads
-  int* s_last = const_cast<int*>(abort_flag) + 3;  // [tile]
+  // [tile][buffer]: the threads formed this part's O += P V themselves
+  volatile int* skip = abort_flag + 1;
+  volatile int* s_odd = abort_flag + 5;            // [tile][turn] a warp's vote
+  int* s_last = const_cast<int*>(abort_flag) + 9;  // [tile]
   int* s_found = s_last + 2;             // [4]
   // [unit mod 16]: bit b is set when keys 16 b .. 16 b + 15 of the unit lie in a page that is
   // not the cache's (the ring holds fewer than 16 units)
   volatile uint32_t* absent = reinterpret_cast<volatile uint32_t*>(s_found + 4);
   int64_t* s_scan = reinterpret_cast<int64_t*>(
-      (reinterpret_cast<uintptr_t>(s_found + 20) + 7) & ~uintptr_t(7));  // [10]
+      (reinterpret_cast<uintptr_t>(s_found + 20) + 15) & ~uintptr_t(15));  // [12]
+  ChunkSegment* s_seg = reinterpret_cast<ChunkSegment*>(s_scan + 12);      // [2]
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
     for (int s = 0; s < C::kStages; ++s) {
       mbar_init(&full[s], 1);
-      mbar_init(&empty[s], 1);
+      mbar_init(&empty[s], 2);
     }
     for (int t = 0; t < 2; ++t) {
       mbar_init(&qfull[t], 4);
-      mbar_init(&sfull[t], 1);
-      mbar_init(&pfull[t], 4);
-      mbar_init(&ofull[t], 1);
-      skip[t] = 0;
+      for (int b = 0; b < 2; ++b) {
+        mbar_init(&sfull[2 * t + b], 1);
+        mbar_init(&pfull[2 * t + b], 4);
+        skip[2 * t + b] = s_odd[2 * t + b] = 0;
+      }
+      mbar_init(&gfull[t], 1);
+      mbar_init(&gempty[t], 10);
+      mbar_init(&done[t], 1);
+      mbar_init(&met[t], 4);
     }
-    mbar_init(done, 1);
     *abort_flag = 0;
     fence_mbar_init();
   }
@@ -296,38 +346,44 @@ __global__ void __launch_bounds__(kPcThreads, 1)
 
   const PagedSlice sl = paged_find_slice<kPcThreads, kPcRows, kPcUnit>(
       a.p, a.q, gridDim.x, blockIdx.x, s_scan, s_found);
-  const int cta = blockIdx.x;
-  PagedItem it;
-  SeqSpan span;
-  int rt = sl.row_tile, off = sl.off;
-  if (sl.begin < sl.end) {
-    it.seq = sl.seq;
-    it.head = sl.head;
-    span = load_span(a.p, it.seq);
-    paged_range_item<kPcRows, kPcUnit>(a.q, span, rt, it);
-  }
-  // every role walks the same segments: calls f(unit0, units in the segment, units in the
-  // item, the item's first unit in the list) for each until it returns false
-  auto walk = [&](auto&& f) {
-    int64_t u = sl.begin;
-    while (u < sl.end) {
-      const int n = it.u1 - it.u0;
-      const int seg = static_cast<int>(min(static_cast<int64_t>(n - off), sl.end - u));
-      if (!f(it.u0 + off, seg, n, u - off)) return;
-      u += seg;
-      if (u >= sl.end) return;
-      off = 0;
-      paged_next_item<kPcRows, kPcUnit>(a.p, a.q, span, rt, it);
-    }
-  };
 
-  if (warp >= 8) regs_dec<kPcRegsRest>();
   if (warp == 8) {
-    // ------------------------------------------------------------ copies of K and V
+    // ------------------------------------------------------------ the list, copies of K and V
     const int box = a.page_box, boxes = kPcUnit / box;
-    uint32_t n_loads = 0;
-    bool bad = false;
-    walk([&](int unit0, int seg, int, int64_t) {
+    uint32_t n_loads = 0, n_seg = 0;
+    bool bad = false, ok = true;
+    PagedItem it = {};
+    SeqSpan span = {};
+    int rt = sl.row_tile, off = sl.off;
+    int64_t u = sl.begin;
+    if (u < sl.end) {
+      it.seq = sl.seq;
+      it.head = sl.head;
+      span = load_span(a.p, it.seq);
+      paged_range_item<kPcRows, kPcUnit>(a.q, span, rt, it);
+    }
+    while (ok) {
+      const bool end = u >= sl.end;
+      const int n = end ? 0 : it.u1 - it.u0;
+      const int seg = end ? 0 : static_cast<int>(min(static_cast<int64_t>(n - off), sl.end - u));
+      const uint32_t gs = n_seg & 1u;
+      if (!warp_wait(&gempty[gs], ((n_seg >> 1) & 1u) ^ 1u, abort_flag)) break;
+      if (lane == 0) {
+        ChunkSegment g;
+        g.unit0 = it.u0 + off;
+        g.units = seg;
+        g.item_units = n;
+        g.item_u0 = u - off;
+        g.head = it.head, g.tok0 = it.tok0, g.r0 = it.r0, g.rows = it.rows, g.pos0 = it.pos0;
+        g.k0 = it.k0, g.k1 = it.k1;
+        g.pad = g.pad2 = 0;
+        s_seg[gs] = g;
+        mbar_arrive(&gfull[gs]);
+      }
+      __syncwarp();
+      ++n_seg;
+      if (end) break;
+      const int unit0 = it.u0 + off;
       const int32_t* table = a.p.table + it.seq * a.p.table_stride;
       // lane l looks up the page of the unit's l-th box; positions no row sees are not looked
       // up, and like pages that are not the cache's they are read past its end, as zeros
@@ -337,7 +393,7 @@ __global__ void __launch_bounds__(kPcThreads, 1)
         return __ldg(table + (pos >> a.p.page_shift));
       };
       int entry = entry_of(0);
-      for (int i = 0; i < seg; ++i) {
+      for (int i = 0; i < seg && ok; ++i) {
         const int pos = (unit0 + i) * kPcUnit + lane * box;
         int page = entry;
         if (page < 0 || page > a.p.pages) page = a.p.pages;
@@ -351,7 +407,10 @@ __global__ void __launch_bounds__(kPcThreads, 1)
 #pragma unroll
         for (int kv = 0; kv < 2; ++kv) {
           const uint32_t s = n_loads % C::kStages, ph = (n_loads / C::kStages) & 1u;
-          if (!warp_wait(&empty[s], ph ^ 1u, abort_flag)) return false;
+          if (!warp_wait(&empty[s], ph ^ 1u, abort_flag)) {
+            ok = false;
+            break;
+          }
           if (lane == 0) mbar_arrive_expect_tx(&full[s], C::kTileBytes);
           __syncwarp();
           uint8_t* dst = smem + s * C::kTileBytes;
@@ -363,8 +422,12 @@ __global__ void __launch_bounds__(kPcThreads, 1)
           ++n_loads;
         }
       }
-      return true;
-    });
+      u += seg;
+      if (u < sl.end) {
+        off = 0;
+        paged_next_item<kPcRows, kPcUnit>(a.p, a.q, span, rt, it);
+      }
+    }
     __syncwarp();
     if (bad && lane == 0) atomicOr(a.status, TDSA_STATUS_RANGE);
     // every issued copy lands before the CTA can exit
@@ -373,115 +436,43 @@ __global__ void __launch_bounds__(kPcThreads, 1)
       const uint32_t n = (n_loads - s + C::kStages - 1) / C::kStages;
       mbar_wait(&full[s], (n - 1) & 1u, &no_abort);
     }
-  } else if (warp == 9) {
-    // ------------------------------------------------------------ tensor products
-    constexpr uint32_t idesc_s = umma_idesc_f16(kBF16, kPcTile, kPcUnit);
-    constexpr uint32_t idesc_o = umma_idesc_f16(kBF16, kPcTile, D) | (1u << 16);
-    uint32_t n_take = 0, q_n[2] = {0, 0}, p_n[2] = {0, 0};
-    auto take = [&]() -> int {  // the ring's next stage, -1 when the CTA aborts
-      const uint32_t s = n_take % C::kStages, ph = (n_take / C::kStages) & 1u;
-      if (!warp_wait(&full[s], ph, abort_flag)) return -1;
-      ++n_take;
-      return static_cast<int>(s);
-    };
-    auto issue_s = [&](int t, int stage) {
-      if (lane == 0) {
-        const uint32_t qa = smem_u32(s_q + t * C::kTileBytes);
-        const uint32_t ka = smem_u32(smem + stage * C::kTileBytes);
-#pragma unroll
-        for (int k = 0; k < D / 16; ++k)
-          umma_f16(tmem + t * 128, sw128_kmajor_desc(qa + (k >> 2) * kPcHalf + (k & 3) * 32),
-                   sw128_kmajor_desc(ka + (k >> 2) * kPcHalf + (k & 3) * 32), idesc_s,
-                   k > 0 ? 1u : 0u);
-        umma_commit(&sfull[t]);
-      }
-      __syncwarp();
-    };
-    walk([&](int unit0, int seg, int, int64_t) {
-      const int tiles = it.rows > kPcTile ? 2 : 1;
-      int ks = take();
-      if (ks < 0) return false;
-      for (int t = 0; t < tiles; ++t) {
-        if (!warp_wait(&qfull[t], q_n[t]++ & 1u, abort_flag)) return false;
-        tc_fence_after();
-        issue_s(t, ks);
-      }
-      if (lane == 0) umma_commit(&empty[ks]);
-      __syncwarp();
-      for (int i = 0; i < seg; ++i) {
-        const int vs = take();
-        if (vs < 0) return false;
-        // rows of V that no row of the item sees may hold anything: zero weights times
-        // infinities or NaN would be NaN, so they become zeros
-        const int base = (unit0 + i) * kPcUnit;
-        if (base < it.k0 || base + kPcUnit > it.k1) {
-          for (int x = lane; x < C::kHalves * kPcUnit * 8; x += 32) {
-            const int r = (x >> 3) & (kPcUnit - 1);
-            if (base + r < it.k0 || base + r >= it.k1)
-              *reinterpret_cast<uint4*>(smem + vs * C::kTileBytes + x * 16) =
-                  make_uint4(0u, 0u, 0u, 0u);
-          }
-          fence_proxy_async_smem();
-          __syncwarp();
-        }
-        const bool more = i + 1 < seg;
-        if (more) {
-          ks = take();
-          if (ks < 0) return false;
-        }
-        for (int t = 0; t < tiles; ++t) {
-          if (!warp_wait(&pfull[t], p_n[t]++ & 1u, abort_flag)) return false;
-          tc_fence_after();
-          if (lane == 0 && !skip[t]) {
-            const uint32_t va = smem_u32(smem + vs * C::kTileBytes);
-#pragma unroll
-            for (int k = 0; k < kPcUnit / 16; ++k)
-              umma_f16_ts(tmem + C::kOCol + t * D, tmem + t * 128 + k * 8,
-                          sw128_mnmajor_desc(va + k * 2048), idesc_o, (i > 0 || k > 0) ? 1u : 0u);
-          }
-          __syncwarp();
-          if (more) {
-            issue_s(t, ks);
-          } else {
-            if (lane == 0) umma_commit(&ofull[t]);
-            __syncwarp();
-          }
-        }
-        if (lane == 0) {
-          umma_commit(&empty[vs]);
-          if (more) umma_commit(&empty[ks]);
-        }
-        __syncwarp();
-      }
-      return true;
-    });
-    __syncwarp();
-    if (lane == 0) umma_commit(done);
-    __syncwarp();
-    volatile int no_abort = 0;
-    mbar_wait(done, 0, &no_abort);
   } else if (warp < 8) {
     // ------------------------------------------------------------ rows: softmax and output
-    regs_inc<kPcRegsRows>();
     const int t = warp >> 2;                      // tile
     const int row = (warp & 3) * 32 + lane;       // of the tile; also the TMEM lane
     const uint32_t lane_base = static_cast<uint32_t>(warp & 3) << 21;
     const uint32_t s_addr = tmem + lane_base + t * 128;
     const uint32_t o_addr = tmem + lane_base + C::kOCol + t * D;
-    const int g = a.q.group;
-    uint32_t s_n = 0, o_n = 0;
-    uint32_t n_v = 1;  // ring index of the current unit's V (K, V, K, V, ...)
-    walk([&](int unit0, int seg, int n_units, int64_t item_u0) {
-      const uint32_t v0 = n_v;
-      n_v += 2 * seg;
-      if (t == 1 && it.rows <= kPcTile) return true;
-      const int r_item = t * kPcTile + row;  // row of the item
-      const bool valid = r_item < it.rows;
-      const int r = it.r0 + r_item;
-      const int tok = it.tok0 + r / g, qh = it.head * g + r % g;
+    const float scale = a.q.scale_log2;
+    uint32_t s_ph[2] = {0, 0};
+    uint32_t n_unit = 0;  // units of the CTA's list before the segment
+    bool was_alone[2] = {false, false};
+    // the tile's warps meet (a bounded wait); false when the CTA aborts
+    uint32_t met_n = 0;
+    auto meet = [&]() -> bool {
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&met[t]);
+      return warp_wait(&met[t], met_n++ & 1u, abort_flag);
+    };
+    for (uint32_t n_seg = 0;; ++n_seg) {
+      const ChunkSegment* sg = &s_seg[n_seg & 1u];
+      if (!warp_wait(&gfull[n_seg & 1u], (n_seg >> 1) & 1u, abort_flag)) break;
+      const int units = sg->units;
+      if (units == 0) break;
+      if (t == 1 && sg->rows <= kPcTile) {
+        n_unit += units;
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&gempty[n_seg & 1u]);
+        continue;
+      }
+      const bool valid = t * kPcTile + row < sg->rows;
+      int lo, hi, all_lo, all_hi;  // keys this row sees; keys every row of the tile sees
       {
+        const int g = a.q.group, r = sg->r0 + t * kPcTile + row;
         const uint4* src = reinterpret_cast<const uint4*>(
-            a.q.q + static_cast<int64_t>(valid ? tok : 0) * a.q.q_ts + (valid ? qh : 0) * a.q.q_hs);
+            a.q.q + (valid ? static_cast<int64_t>(sg->tok0 + r / g) * a.q.q_ts +
+                                 (sg->head * g + r % g) * a.q.q_hs
+                           : 0));
         uint8_t* dst = s_q + t * C::kTileBytes + row * 128;
 #pragma unroll
         for (int c = 0; c < D / 8; ++c) {
@@ -491,124 +482,174 @@ __global__ void __launch_bounds__(kPcThreads, 1)
         fence_proxy_async_smem();
         __syncwarp();
         if (lane == 0) mbar_arrive(&qfull[t]);
+        const int pos = sg->pos0 + r / g, w = a.q.window;
+        const int last = min(sg->rows, (t + 1) * kPcTile) - 1;
+        hi = valid ? min(pos + 1, sg->k1) : sg->k1;
+        lo = valid && w > 0 ? max(0, pos - (w - 1)) : 0;
+        all_hi = min(sg->k1, sg->pos0 + (sg->r0 + t * kPcTile) / g + 1);
+        all_lo = w > 0 ? max(sg->k0, sg->pos0 + (sg->r0 + last) / g - (w - 1)) : sg->k0;
       }
-      // keys this row sees, and keys every row of the tile sees
-      const int pos = it.pos0 + r / g;
-      const int hi = valid ? min(pos + 1, it.k1) : it.k1;
-      const int lo = valid && a.q.window > 0 ? max(0, pos - (a.q.window - 1)) : 0;
-      const int last_row = min(it.rows, (t + 1) * kPcTile) - 1;
-      const int all_hi = min(it.k1, it.pos0 + (it.r0 + t * kPcTile) / g + 1);
-      const int all_lo =
-          a.q.window > 0
-              ? max(it.k0, it.pos0 + (it.r0 + last_row) / g - (a.q.window - 1))
-              : it.k0;
       float ref = -INFINITY, sum = 0.f;
-      for (int i = 0; i < seg; ++i) {
-        const int base = (unit0 + i) * kPcUnit;
-        if (!warp_wait(&sfull[t], s_n++ & 1u, abort_flag)) return false;
-        tc_fence_after();
-        uint32_t s[4][32];
+      int base = sg->unit0 * kPcUnit;
+      bool ok = true;
+      for (int i = 0; i < units && ok; ++i) {
 #pragma unroll
-        for (int c = 0; c < 4; ++c) tmem_ld32(s_addr + c * 32, s[c]);
-        tmem_wait_ld();
-        const bool masked = base < all_lo || base + kPcUnit > all_hi;
-        if (masked) {
+        for (int b = 0; b < 2; ++b, base += kPcPart) {
+          if (ok) ok = warp_wait(&sfull[2 * t + b], s_ph[b], abort_flag);
+          if (!ok) break;
+          s_ph[b] ^= 1u;
+          tc_fence_after();
+          const uint32_t sb = s_addr + b * kPcPart;
+          uint32_t s[2][32];
+          tmem_ld32(sb, s[0]);
+          tmem_ld32(sb + 32, s[1]);
+          // written before the unit's copies were, so it is there when S is
+          const uint32_t gone = (absent[(n_unit + i) & 15] >> (4 * b)) & 15u;
+          const bool masked = base < all_lo || base + kPcPart > all_hi || gone;
+          if (was_alone[b] && !masked) {  // this buffer's products are the tensor core's again
+            if (row == 0) skip[2 * t + b] = 0;
+            was_alone[b] = false;
+          }
+          tmem_wait_ld();
+          if (masked) {
 #pragma unroll
-          for (int j = 0; j < 128; ++j)
-            if (base + j < lo || base + j >= hi) s[j >> 5][j & 31] = 0xFF800000u;  // -infinity
-        }
-        const uint32_t gone = absent[((v0 >> 1) + i) & 15];
-        if (gone) {
+            for (int c = 0; c < 2; ++c)
 #pragma unroll
-          for (int j = 0; j < 128; ++j)
-            if ((gone >> (j >> 4)) & 1u) s[j >> 5][j & 31] = 0xFF800000u;
-        }
-        float tops[4];
+              for (int j = 0; j < 32; ++j) {
+                const int k = base + c * 32 + j;
+                if (k < lo || k >= hi || ((gone >> (2 * c + (j >> 4))) & 1u))
+                  s[c][j] = 0xFF800000u;  // -infinity
+              }
+          }
+          float tops[4];
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          tops[c] = __uint_as_float(s[c][0]);
+          for (int c = 0; c < 4; ++c) {
+            const uint32_t* x = s[c >> 1] + (c & 1) * 16;
+            tops[c] = max3(__uint_as_float(x[0]), __uint_as_float(x[1]), __uint_as_float(x[2]));
 #pragma unroll
-          for (int j = 1; j < 31; j += 2)
-            tops[c] = max3(tops[c], __uint_as_float(s[c][j]), __uint_as_float(s[c][j + 1]));
-          tops[c] = fmaxf(tops[c], __uint_as_float(s[c][31]));
-        }
-        const float top = fmaxf(max3(tops[0], tops[1], tops[2]), tops[3]) * a.q.scale_log2;
-        const bool grow = top > ref + 8.f;
-        if (__any_sync(0xffffffffu, grow)) {
-          const float now = fmaxf(ref, top);
-          const float f = now == ref ? 1.f : exp2_approx(ref - now);
-          ref = now;
-          sum *= f;
-          if (i > 0) {
+            for (int j = 3; j < 15; j += 2)
+              tops[c] = max3(tops[c], __uint_as_float(x[j]), __uint_as_float(x[j + 1]));
+            tops[c] = fmaxf(tops[c], __uint_as_float(x[15]));
+          }
+          const float top = fmaxf(max3(tops[0], tops[1], tops[2]), tops[3]) * scale;
+          if (__any_sync(0xffffffffu, top > ref + 8.f)) {
+            const float now = fmaxf(ref, top);
+            const float f = now == ref ? 1.f : exp2_approx(ref - now);
+            ref = now;
+            sum *= f;
+            if (i > 0 || b > 0) {
+              // O += P V of the part before is complete with the S after this one
+              ok = warp_wait(&sfull[2 * t + (b ^ 1)], s_ph[b ^ 1], abort_flag);
+              if (!ok) break;
+              tc_fence_after();
 #pragma unroll
-            for (int c = 0; c < D / 16; ++c) {
-              uint32_t o[16];
-              tmem_ld16(o_addr + c * 16, o);
-              tmem_wait_ld();
+              for (int c = 0; c < D / 16; ++c) {
+                uint32_t o[16];
+                tmem_ld16(o_addr + c * 16, o);
+                tmem_wait_ld();
 #pragma unroll
-              for (int j = 0; j < 16; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * f);
-              tmem_st16(o_addr + c * 16, o);
+                for (int j = 0; j < 16; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * f);
+                tmem_st16(o_addr + c * 16, o);
+              }
             }
           }
-        }
-        const float neg = ref == -INFINITY ? 0.f : -ref;
-        const uint64_t scale2 = pair(a.q.scale_log2, a.q.scale_log2), neg2 = pair(neg, neg);
-        uint64_t part[2] = {0ull, 0ull};
+          const float neg = ref == -INFINITY ? 0.f : -ref;
+          const uint64_t scale2 = pair(scale, scale), neg2 = pair(neg, neg);
+          uint64_t part[2] = {0ull, 0ull};
+          // P of columns 32 c .. 32 c + 31; poly of 8 pairs take the polynomial, which does not
+          // take the -infinity of a masked score
+          auto weights = [&](int c, auto poly) {
+            uint32_t p[16];
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          uint32_t p[16];
-#pragma unroll
-          for (int j = 0; j < 16; ++j) {
-            const float2 x = unpair(fma2(
-                pair(__uint_as_float(s[c][2 * j]), __uint_as_float(s[c][2 * j + 1])), scale2, neg2));
-            const float e0 = exp2_approx(x.x), e1 = exp2_approx(x.y);
-            part[j & 1] = add2(part[j & 1], pair(e0, e1));
-            p[j] = pack16<kBF16>(e0, e1);
-          }
-          tmem_st16(s_addr + c * 16, p);
-        }
-        {
-          const float2 x = unpair(add2(part[0], part[1]));
-          sum += x.x + x.y;
-        }
-        tmem_wait_st();
-        bool alone = false;
-        if (masked) {
-          // a value that only some rows see and that is not finite: zero weights times it
-          // would be NaN for the others, so the threads form this unit's product themselves
-          const uint32_t vi = v0 + 2 * i;
-          const uint32_t st = vi % C::kStages;
-          if (!warp_wait(&full[st], (vi / C::kStages) & 1u, abort_flag)) return false;
-          const uint8_t* sv = smem + st * C::kTileBytes;
-          bool odd = false;
-          if (base + row >= it.k0 && base + row < it.k1) {
-#pragma unroll
-            for (int c = 0; c < D / 8; ++c) {
-              const uint4 x = *reinterpret_cast<const uint4*>(sv + (c >> 3) * kPcHalf + row * 128 +
-                                                              (c & 7) * 16);
-              odd |= nonfinite16<kBF16>(x.x) || nonfinite16<kBF16>(x.y) ||
-                     nonfinite16<kBF16>(x.z) || nonfinite16<kBF16>(x.w);
+            for (int j = 0; j < 16; ++j) {
+              const uint64_t x2 =
+                  fma2(pair(__uint_as_float(s[c][2 * j]), __uint_as_float(s[c][2 * j + 1])), scale2,
+                       neg2);
+              float2 e;
+              if (j % 8 < decltype(poly)::value) {
+                e = exp2_poly2(x2);
+              } else {
+                const float2 x = unpair(x2);
+                e = make_float2(exp2_approx(x.x), exp2_approx(x.y));
+              }
+              part[j & 1] = add2(part[j & 1], pair(e.x, e.y));
+              p[j] = pack16<kBF16>(e.x, e.y);
             }
+            tmem_st16(sb + c * 16, p);
+          };
+          if (masked) {
+            weights(0, std::integral_constant<int, 0>{});
+            weights(1, std::integral_constant<int, 0>{});
+          } else {
+            weights(0, std::integral_constant<int, kPcPolyOf8>{});
+            weights(1, std::integral_constant<int, kPcPolyOf8>{});
           }
-          alone = tile_any(t, odd);
-          if (alone)
-            add_visible<kBF16, D>(s_addr, o_addr, sv, max(0, lo - base), min(kPcUnit, hi - base),
-                                  i == 0);
+          {
+            const float2 x = unpair(add2(part[0], part[1]));
+            sum += x.x + x.y;
+          }
+          tmem_wait_st();
+          if (masked) {
+            // a value that only some rows see and that is not finite: zero weights times it
+            // would be NaN for the others, so the threads form this part's product themselves
+            const uint32_t vi = 2 * (n_unit + i) + 1;  // K, V, K, V, ... fill the ring
+            const uint32_t st = vi % C::kStages;
+            ok = warp_wait(&full[st], (vi / C::kStages) & 1u, abort_flag);
+            if (!ok) break;
+            const uint8_t* sv = smem + st * C::kTileBytes + b * kPcPart * 128;
+            const int key = row & (kPcPart - 1);
+            bool odd = false;
+            if (base + key >= sg->k0 && base + key < sg->k1) {
+#pragma unroll
+              for (int x = 0; x < D / 16; ++x) {  // half a row of V per thread
+                const int c = (row / kPcPart) * (D / 16) + x;
+                const uint4 w = *reinterpret_cast<const uint4*>(sv + (c >> 3) * kPcHalf +
+                                                                key * 128 + (c & 7) * 16);
+                odd |= nonfinite16<kBF16>(w.x) || nonfinite16<kBF16>(w.y) ||
+                       nonfinite16<kBF16>(w.z) || nonfinite16<kBF16>(w.w);
+              }
+            }
+            const uint32_t turn = met_n & 1u;
+            if (__any_sync(0xffffffffu, odd) && lane == 0) s_odd[2 * t + turn] = 1;
+            ok = meet();
+            if (!ok) break;
+            const bool alone = s_odd[2 * t + turn] != 0;
+            ok = meet();  // every warp has read the vote
+            if (!ok) break;
+            if (row == 0) s_odd[2 * t + turn] = 0;
+            if (alone) {
+              ok = warp_wait(&sfull[2 * t + (b ^ 1)], s_ph[b ^ 1], abort_flag);
+              if (!ok) break;
+              tc_fence_after();
+              add_visible<kBF16, D>(sb, o_addr, sv, max(0, lo - base), min(kPcPart, hi - base),
+                                    i == 0 && b == 0);
+            }
+            if (alone != was_alone[b] && row == 0) skip[2 * t + b] = alone ? 1 : 0;
+            was_alone[b] = alone;
+          }
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&pfull[2 * t + b]);
         }
-        if (row == 0) skip[t] = alone ? 1 : 0;
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&pfull[t]);
       }
+      n_unit += units;
 
       // ---------------------------------------------------------- output
-      if (!warp_wait(&ofull[t], o_n++ & 1u, abort_flag)) return false;
+#pragma unroll
+      for (int b = 0; b < 2; ++b) {
+        if (ok) ok = warp_wait(&sfull[2 * t + b], s_ph[b], abort_flag);
+        s_ph[b] ^= 1u;
+      }
+      if (!ok) break;
       tc_fence_after();
-      const bool entire = seg == n_units;
-      if (entire) {
+      const int g = a.q.group;
+      const int r_item = t * kPcTile + row;  // row of the item
+      if (units == sg->item_units) {
         const float inv = sum > 0.f ? 1.f / sum : (sum == 0.f ? 0.f : sum);  // NaN stays NaN
-        uint4* dst = reinterpret_cast<uint4*>(a.q.out + static_cast<int64_t>(tok) * a.q.o_ts +
-                                              qh * a.q.o_hs);
+        const int r = sg->r0 + r_item;
+        const int64_t tok = sg->tok0 + r / g;
+        const int qh = sg->head * g + r % g;
+        uint4* dst = reinterpret_cast<uint4*>(a.q.out + tok * a.q.o_ts + qh * a.q.o_hs);
 #pragma unroll
         for (int c = 0; c < D / 32; ++c) {
           uint32_t o[32];
@@ -629,84 +670,185 @@ __global__ void __launch_bounds__(kPcThreads, 1)
         }
         tc_fence_before();
         if (valid && a.q.lse)
-          a.q.lse[static_cast<int64_t>(tok) * a.q.heads + qh] =
+          a.q.lse[tok * a.q.heads + qh] =
               sum == 0.f ? -INFINITY : (ref + log2f(sum)) * 0.6931471805599453f;
-        return true;
-      }
-      const int c_first = slice_owner(sl.units, sl.ctas, item_u0);
-      const int c_last = slice_owner(sl.units, sl.ctas, item_u0 + n_units - 1);
-      {
-        const int64_t slot = 2 * cta + (cta == c_first ? 1 : 0);
-        const int64_t at = slot * kPcRows + r_item;
-        a.part.ml[at] = make_float2(ref, sum);
-        float4* dst = reinterpret_cast<float4*>(a.part.o + at * D);
+      } else {
+        const int c_first = slice_owner(sl.units, sl.ctas, sg->item_u0);
+        const int c_last = slice_owner(sl.units, sl.ctas, sg->item_u0 + sg->item_units - 1);
+        {
+          const int cta = blockIdx.x;
+          const int64_t slot = 2 * cta + (cta == c_first ? 1 : 0);
+          const int64_t at = slot * kPcRows + r_item;
+          a.part.ml[at] = make_float2(ref, sum);
+          float4* dst = reinterpret_cast<float4*>(a.part.o + at * D);
 #pragma unroll
-        for (int c = 0; c < D / 32; ++c) {
-          uint32_t o[32];
-          tmem_ld32(o_addr + c * 32, o);
-          tmem_wait_ld();
+          for (int c = 0; c < D / 32; ++c) {
+            uint32_t o[32];
+            tmem_ld32(o_addr + c * 32, o);
+            tmem_wait_ld();
 #pragma unroll
-          for (int x = 0; x < 8; ++x)
-            dst[c * 8 + x] =
-                make_float4(__uint_as_float(o[4 * x]), __uint_as_float(o[4 * x + 1]),
-                            __uint_as_float(o[4 * x + 2]), __uint_as_float(o[4 * x + 3]));
-        }
-        tc_fence_before();
-      }
-      tile_sync(t);
-      if (row == 0) {
-        __threadfence();
-        uint32_t* counter = a.part.counters + 2 * c_first + t;
-        const uint32_t n = static_cast<uint32_t>(c_last - c_first + 1);
-        const uint32_t old = atomicAdd(counter, 1u);
-        if (old == n - 1) *counter = 0u;
-        s_last[t] = old == n - 1;
-        __threadfence();
-      }
-      tile_sync(t);
-      if (s_last[t]) {
-        // the last to arrive: partials of CTAs c_first .. c_last in that order, a warp per row
-        constexpr int kV = D / 32;  // floats of a row per lane
-        const int rows = min(it.rows - t * kPcTile, kPcTile);
-        for (int x = warp & 3; x < rows; x += 4) {
-          const int ri = t * kPcTile + x;
-          float m = -INFINITY;
-          for (int c = c_first; c <= c_last; ++c)
-            m = fmaxf(m, __ldcg(&a.part.ml[(2 * static_cast<int64_t>(c) + (c == c_first)) *
-                                               kPcRows + ri]).x);
-          const float mr = m == -INFINITY ? 0.f : m;
-          float l = 0.f, v[kV];
-#pragma unroll
-          for (int y = 0; y < kV; ++y) v[y] = 0.f;
-#pragma unroll 2
-          for (int c = c_first; c <= c_last; ++c) {
-            const int64_t at = (2 * static_cast<int64_t>(c) + (c == c_first)) * kPcRows + ri;
-            const float2 ml = __ldcg(&a.part.ml[at]);
-            const float f = exp2_approx(ml.x - mr);
-            l += ml.y * f;
-#pragma unroll
-            for (int y = 0; y < kV / 2; ++y) {
-              const float2 w = __ldcg(
-                  reinterpret_cast<const float2*>(a.part.o + at * D) + y * 32 + lane);
-              v[2 * y] += w.x * f;
-              v[2 * y + 1] += w.y * f;
-            }
+            for (int x = 0; x < 8; ++x)
+              dst[c * 8 + x] =
+                  make_float4(__uint_as_float(o[4 * x]), __uint_as_float(o[4 * x + 1]),
+                              __uint_as_float(o[4 * x + 2]), __uint_as_float(o[4 * x + 3]));
           }
-          const int rg = it.r0 + ri;
-          const int64_t to = it.tok0 + rg / g;
-          const int h = it.head * g + rg % g;
-          const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
+          tc_fence_before();
+        }
+        if (!meet()) break;
+        if (row == 0) {
+          __threadfence();
+          uint32_t* counter = a.part.counters + 2 * c_first + t;
+          const uint32_t n = static_cast<uint32_t>(c_last - c_first + 1);
+          const uint32_t old = atomicAdd(counter, 1u);
+          if (old == n - 1) *counter = 0u;
+          s_last[t] = old == n - 1;
+          __threadfence();
+        }
+        if (!meet()) break;
+        if (s_last[t]) {
+          // the last to arrive: partials of CTAs c_first .. c_last in that order, a warp per row
+          constexpr int kV = D / 32;  // floats of a row per lane
+          const int rows = min(sg->rows - t * kPcTile, kPcTile);
+          for (int x = warp & 3; x < rows; x += 4) {
+            const int ri = t * kPcTile + x;
+            float m = -INFINITY;
+            for (int c = c_first; c <= c_last; ++c)
+              m = fmaxf(m, __ldcg(&a.part.ml[(2 * static_cast<int64_t>(c) + (c == c_first)) *
+                                                 kPcRows + ri]).x);
+            const float mr = m == -INFINITY ? 0.f : m;
+            float l = 0.f, v[kV];
 #pragma unroll
-          for (int y = 0; y < kV / 2; ++y)
-            *(reinterpret_cast<uint32_t*>(a.q.out + to * a.q.o_ts + h * a.q.o_hs) + y * 32 + lane) =
-                l == 0.f ? 0u : pack16<kBF16>(v[2 * y] * inv, v[2 * y + 1] * inv);
-          if (a.q.lse && lane == 0)
-            a.q.lse[to * a.q.heads + h] =
-                l == 0.f ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f;
+            for (int y = 0; y < kV; ++y) v[y] = 0.f;
+#pragma unroll 2
+            for (int c = c_first; c <= c_last; ++c) {
+              const int64_t at = (2 * static_cast<int64_t>(c) + (c == c_first)) * kPcRows + ri;
+              const float2 ml = __ldcg(&a.part.ml[at]);
+              const float f = exp2_approx(ml.x - mr);
+              l += ml.y * f;
+#pragma unroll
+              for (int y = 0; y < kV / 2; ++y) {
+                const float2 w =
+                    __ldcg(reinterpret_cast<const float2*>(a.part.o + at * D) + y * 32 + lane);
+                v[2 * y] += w.x * f;
+                v[2 * y + 1] += w.y * f;
+              }
+            }
+            const int rg = sg->r0 + ri;
+            const int64_t to = sg->tok0 + rg / g;
+            const int h = sg->head * g + rg % g;
+            const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
+#pragma unroll
+            for (int y = 0; y < kV / 2; ++y)
+              *(reinterpret_cast<uint32_t*>(a.q.out + to * a.q.o_ts + h * a.q.o_hs) + y * 32 +
+                lane) = l == 0.f ? 0u : pack16<kBF16>(v[2 * y] * inv, v[2 * y + 1] * inv);
+            if (a.q.lse && lane == 0)
+              a.q.lse[to * a.q.heads + h] =
+                  l == 0.f ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f;
+          }
         }
       }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&gempty[n_seg & 1u]);
+    }
+  } else {
+    // ------------------------------------------------------------ tensor products of a tile
+    const int t = warp - 9;
+    constexpr uint32_t idesc_s = umma_idesc_f16(kBF16, kPcTile, kPcPart);
+    constexpr uint32_t idesc_o = umma_idesc_f16(kBF16, kPcTile, D) | (1u << 16);
+    const uint32_t one = elect_one();
+    const uint32_t qa = smem_u32(s_q) + t * C::kTileBytes, ring_base = smem_u32(smem);
+    uint32_t stage = 0, stage_ph = 0;  // the ring's next stage
+    uint32_t q_ph = 0, p_ph = 0;
+    auto take = [&](uint32_t& s) -> bool {
+      s = stage;
+      if (!warp_wait(&full[s], stage_ph, abort_flag)) return false;
+      if (++stage == C::kStages) stage = 0, stage_ph ^= 1u;
       return true;
-    });
+    };
+    auto issue_s = [&](uint32_t s, int b) {  // keys 64 b .. of the unit, into buffer b
+      const uint32_t ka = ring_base + s * C::kTileBytes + b * kPcPart * 128;
+#pragma unroll
+      for (int k = 0; k < D / 16; ++k)
+        umma_ss(tmem + t * 128 + b * kPcPart,
+                sw128_kmajor_desc(qa + (k >> 2) * kPcHalf + (k & 3) * 32),
+                sw128_kmajor_desc(ka + (k >> 2) * kPcHalf + (k & 3) * 32), idesc_s,
+                k > 0 ? 1u : 0u, one);
+    };
+    bool ok = true;
+    for (uint32_t n_seg = 0; ok; ++n_seg) {
+      const uint32_t gs = n_seg & 1u;
+      if (!warp_wait(&gfull[gs], (n_seg >> 1) & 1u, abort_flag)) break;
+      const int units = s_seg[gs].units;
+      const int base0 = s_seg[gs].unit0 * kPcUnit;
+      const int k0 = s_seg[gs].k0, k1 = s_seg[gs].k1;
+      const bool mine = t == 0 || s_seg[gs].rows > kPcTile;
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&gempty[gs]);
+      if (units == 0) break;
+      uint32_t ks = 0, vs = 0;
+      if (!mine) {  // the item has one tile: only hand the stages on
+        for (int i = 0; i < 2 * units && ok; ++i) {
+          ok = take(ks);
+          if (ok && lane == 0) mbar_arrive(&empty[ks]);
+          __syncwarp();
+        }
+        continue;
+      }
+      ok = take(ks) && warp_wait(&qfull[t], q_ph, abort_flag);
+      q_ph ^= 1u;
+      if (!ok) break;
+      tc_fence_after();
+#pragma unroll
+      for (int b = 0; b < 2; ++b) {
+        issue_s(ks, b);
+        umma_commit_on(&sfull[2 * t + b], one);
+      }
+      umma_commit_on(&empty[ks], one);
+      for (int i = 0; i < units; ++i) {
+        ok = take(vs);
+        if (!ok) break;
+        // rows of V that no row of the item sees may hold anything: zero weights times
+        // infinities or NaN would be NaN, so they become zeros (both tiles' warps write them)
+        const int base = base0 + i * kPcUnit;
+        if (base < k0 || base + kPcUnit > k1) {
+          for (int x = lane; x < C::kHalves * kPcUnit * 8; x += 32) {
+            const int r = (x >> 3) & (kPcUnit - 1);
+            if (base + r < k0 || base + r >= k1)
+              *reinterpret_cast<uint4*>(smem + vs * C::kTileBytes + x * 16) =
+                  make_uint4(0u, 0u, 0u, 0u);
+          }
+          fence_proxy_async_smem();
+          __syncwarp();
+        }
+        const bool more = i + 1 < units;
+        if (more) ok = take(ks);
+        if (!ok) break;
+        const uint32_t va = ring_base + vs * C::kTileBytes;
+#pragma unroll
+        for (int b = 0; b < 2; ++b) {
+          if (ok) ok = warp_wait(&pfull[2 * t + b], p_ph, abort_flag);
+          if (!ok) break;
+          tc_fence_after();
+          const uint32_t on = skip[2 * t + b] ? 0u : one;
+#pragma unroll
+          for (int k = 0; k < kPcPart / 16; ++k)
+            umma_ts(tmem + C::kOCol + t * D, tmem + t * 128 + b * kPcPart + k * 8,
+                    sw128_mnmajor_desc(va + (4 * b + k) * 2048), idesc_o,
+                    (i > 0 || b > 0 || k > 0) ? 1u : 0u, on);
+          if (more) issue_s(ks, b);
+          // past the last part too: its second commit says that O is complete
+          umma_commit_on(&sfull[2 * t + b], one);
+        }
+        if (!ok) break;
+        p_ph ^= 1u;
+        umma_commit_on(&empty[vs], one);
+        if (more) umma_commit_on(&empty[ks], one);
+      }
+    }
+    __syncwarp();
+    umma_commit_on(&done[t], one);
+    volatile int no_abort = 0;
+    mbar_wait(&done[t], 0, &no_abort);
   }
 
   __syncthreads();

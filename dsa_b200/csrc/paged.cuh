@@ -163,27 +163,11 @@ struct PagedSlice {
   int seq, row_tile, head, off;
 };
 
-template <int kThreads, int kRows, int kUnit>
-__device__ __forceinline__ PagedSlice paged_find_slice(const PagedView& p, const PagedQuery& q,
-                                                       int ctas, int cta, int64_t* s_scan,
-                                                       int* s_found) {
+// Sum over the block's threads before this one, and over all of them.
+template <int kThreads>
+__device__ __forceinline__ int64_t block_scan(int64_t mine, int64_t* s_scan, int64_t& all) {
   constexpr int kWarps = kThreads / 32;
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const int chunk = (p.batch + kThreads - 1) / kThreads;
-  const int b0 = min(p.batch, tid * chunk), b1 = min(p.batch, b0 + chunk);
-  auto seq_units = [&](int b) {
-    const SeqSpan s = load_span(p, b);
-    const int tiles = static_cast<int>((static_cast<int64_t>(s.n) * q.group + kRows - 1) / kRows);
-    int64_t sum = 0;
-    PagedItem x;
-    for (int r = 0; r < tiles; ++r) {
-      paged_range_item<kRows, kUnit>(q, s, r, x);
-      sum += x.u1 - x.u0;
-    }
-    return sum;
-  };
-  int64_t mine = 0;
-  for (int b = b0; b < b1; ++b) mine += seq_units(b);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   int64_t incl = mine;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
@@ -192,46 +176,104 @@ __device__ __forceinline__ PagedSlice paged_find_slice(const PagedView& p, const
   }
   if (lane == 31) s_scan[warp] = incl;
   __syncthreads();
-  int64_t before = 0, all = 0;
+  int64_t before = incl - mine;
+  all = 0;
 #pragma unroll
   for (int w = 0; w < kWarps; ++w) {
     if (w < warp) before += s_scan[w];
     all += s_scan[w];
   }
+  __syncthreads();
+  return before;
+}
+
+// Row tiles are numbered over the whole batch and shared out evenly, so that one long sequence
+// costs no more than many short ones.  s_scan: kThreads / 32 values; s_first: kThreads values.
+template <int kThreads, int kRows, int kUnit>
+__device__ __forceinline__ PagedSlice paged_find_slice(const PagedView& p, const PagedQuery& q,
+                                                       int ctas, int cta, int64_t* s_scan,
+                                                       int* s_first, int* s_found) {
+  const int tid = threadIdx.x;
+  const int chunk = (p.batch + kThreads - 1) / kThreads;
+  auto tiles_of = [&](const SeqSpan& s) { return (s.n * q.group + kRows - 1) / kRows; };
+  int64_t mine = 0, all_tiles;
+  for (int b = tid * chunk; b < min(p.batch, (tid + 1) * chunk); ++b)
+    mine += tiles_of(load_span(p, b));
+  const int64_t first = block_scan<kThreads>(mine, s_scan, all_tiles);
+  s_first[tid] = static_cast<int>(first);  // tiles: fewer than the call's rows, 2^30
+  __syncthreads();
+
+  // this thread's tiles [t0, t1): the sequence and the row tile of the first
+  const int tiles = static_cast<int>(all_tiles);
+  const int per = (tiles + kThreads - 1) / kThreads;
+  const int t0 = min(tiles, tid * per), t1 = min(tiles, t0 + per);
+  int b = 0, rt = 0;
+  SeqSpan s = {};
+  auto seek = [&]() {
+    int lo = 0, hi = kThreads - 1;  // the last chunk that begins at or before t0
+    while (lo < hi) {
+      const int mid = (lo + hi + 1) >> 1;
+      if (s_first[mid] <= t0) lo = mid;
+      else hi = mid - 1;
+    }
+    b = lo * chunk;
+    rt = t0 - s_first[lo];
+    for (;; ++b) {
+      s = load_span(p, b);
+      const int n = tiles_of(s);
+      if (rt < n) return;
+      rt -= n;
+    }
+  };
+  // calls f(units of the tile) for this thread's tiles until it returns false
+  auto each = [&](auto&& f) {
+    for (int t = t0; t < t1; ++t) {
+      PagedItem x;
+      paged_range_item<kRows, kUnit>(q, s, rt, x);
+      if (!f(x.u1 - x.u0)) return;
+      if (++rt == tiles_of(s) && t + 1 < t1) {
+        rt = 0;
+        do {
+          s = load_span(p, ++b);
+        } while (s.n == 0);
+      }
+    }
+  };
+  if (t0 < t1) seek();
+  const int b_first = b, rt_first = rt;
+  const SeqSpan s_first_span = s;
+  int64_t sum = 0, all;
+  each([&](int n) {
+    sum += n;
+    return true;
+  });
+  const int64_t before = block_scan<kThreads>(sum, s_scan, all);
   PagedSlice r;
   r.units = all * p.kv_heads;
   r.ctas = static_cast<int>(min(static_cast<int64_t>(ctas), r.units));
   r.begin = r.end = 0;
+  r.seq = r.row_tile = r.head = r.off = 0;
   if (cta >= r.ctas) return r;
   r.begin = slice_begin(r.units, r.ctas, cta);
   r.end = slice_begin(r.units, r.ctas, cta + 1);
-  int64_t at = (before + incl - mine) * p.kv_heads;
-  if (r.begin >= at && r.begin < at + mine * p.kv_heads) {
-    // the slice begins in this thread's chunk of the batch
-    for (int b = b0; b < b1; ++b) {
-      const int64_t w = seq_units(b) * p.kv_heads;
+  int64_t at = before * p.kv_heads;
+  if (r.begin >= at && r.begin < at + sum * p.kv_heads) {
+    b = b_first;  // the slice begins in this thread's tiles
+    rt = rt_first;
+    s = s_first_span;
+    each([&](int n) {
+      const int64_t w = static_cast<int64_t>(n) * p.kv_heads;
       if (r.begin >= at + w) {
         at += w;
-        continue;
+        return true;
       }
-      const SeqSpan s = load_span(p, b);
-      PagedItem x;
-      for (int t = 0;; ++t) {
-        paged_range_item<kRows, kUnit>(q, s, t, x);
-        const int n = x.u1 - x.u0;
-        const int64_t wr = static_cast<int64_t>(n) * p.kv_heads;
-        if (r.begin < at + wr) {
-          const int64_t rest = r.begin - at;
-          s_found[0] = b;
-          s_found[1] = t;
-          s_found[2] = static_cast<int>(rest / n);
-          s_found[3] = static_cast<int>(rest % n);
-          break;
-        }
-        at += wr;
-      }
-      break;
-    }
+      const int64_t rest = r.begin - at;
+      s_found[0] = b;
+      s_found[1] = rt;
+      s_found[2] = static_cast<int>(rest / n);
+      s_found[3] = static_cast<int>(rest % n);
+      return false;
+    });
   }
   __syncthreads();
   r.seq = s_found[0];

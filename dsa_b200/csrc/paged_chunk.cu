@@ -39,7 +39,6 @@ constexpr int kPcTile = 128;           // rows of a tile
 constexpr int kPcRows = 2 * kPcTile;   // rows of an item
 constexpr int kPcUnit = 128;           // keys of a unit
 constexpr int kPcPart = 64;            // keys of a part of a unit
-constexpr int kPcPolyOf8 = 3;          // of 8 pairs of exponentials, on the fma pipe
 constexpr int kPcHalf = kPcUnit * 128; // bytes of a 64-wide half of a unit (or of a Q tile)
 
 struct ChunkArgs {
@@ -298,8 +297,8 @@ __global__ void __launch_bounds__(kPcThreads, 1)
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_holder + 1);
   // [tile][buffer]: the threads formed this part's O += P V themselves
   volatile int* skip = abort_flag + 1;
-  volatile int* s_odd = abort_flag + 5;            // [tile][turn] a warp's vote
-  int* s_last = const_cast<int*>(abort_flag) + 9;  // [tile]
+  volatile int* s_odd = abort_flag + 5;             // [tile][3] votes of the tile's warps
+  int* s_last = const_cast<int*>(abort_flag) + 11;  // [tile]
   int* s_found = s_last + 2;             // [4]
   // [unit mod 16]: bit b is set when keys 16 b .. 16 b + 15 of the unit lie in a page that is
   // not the cache's (the ring holds fewer than 16 units)
@@ -319,8 +318,9 @@ __global__ void __launch_bounds__(kPcThreads, 1)
       for (int b = 0; b < 2; ++b) {
         mbar_init(&sfull[2 * t + b], 1);
         mbar_init(&pfull[2 * t + b], 4);
-        skip[2 * t + b] = s_odd[2 * t + b] = 0;
+        skip[2 * t + b] = 0;
       }
+      for (int v = 0; v < 3; ++v) s_odd[3 * t + v] = 0;
       mbar_init(&gfull[t], 1);
       mbar_init(&gempty[t], 10);
       mbar_init(&done[t], 1);
@@ -345,7 +345,9 @@ __global__ void __launch_bounds__(kPcThreads, 1)
   pdl_launch_dependents();
 
   const PagedSlice sl = paged_find_slice<kPcThreads, kPcRows, kPcUnit>(
-      a.p, a.q, gridDim.x, blockIdx.x, s_scan, s_found);
+      a.p, a.q, gridDim.x, blockIdx.x, s_scan, reinterpret_cast<int*>(smem), s_found);
+  fence_proxy_async_smem();  // the ring was its scratch: copies may write there after this
+  __syncthreads();
 
   if (warp == 8) {
     // ------------------------------------------------------------ the list, copies of K and V
@@ -449,6 +451,7 @@ __global__ void __launch_bounds__(kPcThreads, 1)
     bool was_alone[2] = {false, false};
     // the tile's warps meet (a bounded wait); false when the CTA aborts
     uint32_t met_n = 0;
+    int vote = 0;
     auto meet = [&]() -> bool {
       __syncwarp();
       if (lane == 0) mbar_arrive(&met[t]);
@@ -556,8 +559,8 @@ __global__ void __launch_bounds__(kPcThreads, 1)
           const float neg = ref == -INFINITY ? 0.f : -ref;
           const uint64_t scale2 = pair(scale, scale), neg2 = pair(neg, neg);
           uint64_t part[2] = {0ull, 0ull};
-          // P of columns 32 c .. 32 c + 31; poly of 8 pairs take the polynomial, which does not
-          // take the -infinity of a masked score
+          // P of columns 32 c .. 32 c + 31; a third of the pairs take the polynomial, which does
+          // not take the -infinity of a masked score
           auto weights = [&](int c, auto poly) {
             uint32_t p[16];
 #pragma unroll
@@ -566,7 +569,7 @@ __global__ void __launch_bounds__(kPcThreads, 1)
                   fma2(pair(__uint_as_float(s[c][2 * j]), __uint_as_float(s[c][2 * j + 1])), scale2,
                        neg2);
               float2 e;
-              if (j % 8 < decltype(poly)::value) {
+              if (decltype(poly)::value && j % 3 == 1) {
                 e = exp2_poly2(x2);
               } else {
                 const float2 x = unpair(x2);
@@ -578,11 +581,11 @@ __global__ void __launch_bounds__(kPcThreads, 1)
             tmem_st16(sb + c * 16, p);
           };
           if (masked) {
-            weights(0, std::integral_constant<int, 0>{});
-            weights(1, std::integral_constant<int, 0>{});
+            weights(0, std::false_type{});
+            weights(1, std::false_type{});
           } else {
-            weights(0, std::integral_constant<int, kPcPolyOf8>{});
-            weights(1, std::integral_constant<int, kPcPolyOf8>{});
+            weights(0, std::true_type{});
+            weights(1, std::true_type{});
           }
           {
             const float2 x = unpair(add2(part[0], part[1]));
@@ -609,14 +612,14 @@ __global__ void __launch_bounds__(kPcThreads, 1)
                        nonfinite16<kBF16>(w.z) || nonfinite16<kBF16>(w.w);
               }
             }
-            const uint32_t turn = met_n & 1u;
-            if (__any_sync(0xffffffffu, odd) && lane == 0) s_odd[2 * t + turn] = 1;
+            // three ballots in turn: the next one was last read before the meeting before this
+            if (__any_sync(0xffffffffu, odd) && lane == 0) s_odd[3 * t + vote] = 1;
+            const int next_vote = vote == 2 ? 0 : vote + 1;
+            if (row == 0) s_odd[3 * t + next_vote] = 0;
             ok = meet();
             if (!ok) break;
-            const bool alone = s_odd[2 * t + turn] != 0;
-            ok = meet();  // every warp has read the vote
-            if (!ok) break;
-            if (row == 0) s_odd[2 * t + turn] = 0;
+            const bool alone = s_odd[3 * t + vote] != 0;
+            vote = next_vote;
             if (alone) {
               ok = warp_wait(&sfull[2 * t + (b ^ 1)], s_ph[b ^ 1], abort_flag);
               if (!ok) break;
@@ -644,55 +647,25 @@ __global__ void __launch_bounds__(kPcThreads, 1)
       tc_fence_after();
       const int g = a.q.group;
       const int r_item = t * kPcTile + row;  // row of the item
-      if (units == sg->item_units) {
-        const float inv = sum > 0.f ? 1.f / sum : (sum == 0.f ? 0.f : sum);  // NaN stays NaN
-        const int r = sg->r0 + r_item;
-        const int64_t tok = sg->tok0 + r / g;
-        const int qh = sg->head * g + r % g;
-        uint4* dst = reinterpret_cast<uint4*>(a.q.out + tok * a.q.o_ts + qh * a.q.o_hs);
+      const int c_first = slice_owner(sl.units, sl.ctas, sg->item_u0);
+      const int c_last = slice_owner(sl.units, sl.ctas, sg->item_u0 + sg->item_units - 1);
+      bool write = true;
+      if (units != sg->item_units) {
+        // a part of the item: float32, the rows of a column quad side by side
+        const int cta = blockIdx.x;
+        const int64_t slot = 2 * cta + (cta == c_first ? 1 : 0);
+        a.part.ml[slot * kPcRows + r_item] = make_float2(ref, sum);
+        float4* dst = reinterpret_cast<float4*>(a.part.o + slot * kPcRows * D) + r_item;
 #pragma unroll
         for (int c = 0; c < D / 32; ++c) {
           uint32_t o[32];
           tmem_ld32(o_addr + c * 32, o);
           tmem_wait_ld();
-          if (valid) {
 #pragma unroll
-            for (int x = 0; x < 4; ++x) {
-              uint32_t w[4];
-#pragma unroll
-              for (int y = 0; y < 4; ++y)
-                w[y] = sum == 0.f ? 0u
-                                  : pack16<kBF16>(__uint_as_float(o[x * 8 + 2 * y]) * inv,
-                                                  __uint_as_float(o[x * 8 + 2 * y + 1]) * inv);
-              dst[c * 4 + x] = make_uint4(w[0], w[1], w[2], w[3]);
-            }
-          }
-        }
-        tc_fence_before();
-        if (valid && a.q.lse)
-          a.q.lse[tok * a.q.heads + qh] =
-              sum == 0.f ? -INFINITY : (ref + log2f(sum)) * 0.6931471805599453f;
-      } else {
-        const int c_first = slice_owner(sl.units, sl.ctas, sg->item_u0);
-        const int c_last = slice_owner(sl.units, sl.ctas, sg->item_u0 + sg->item_units - 1);
-        {
-          const int cta = blockIdx.x;
-          const int64_t slot = 2 * cta + (cta == c_first ? 1 : 0);
-          const int64_t at = slot * kPcRows + r_item;
-          a.part.ml[at] = make_float2(ref, sum);
-          float4* dst = reinterpret_cast<float4*>(a.part.o + at * D);
-#pragma unroll
-          for (int c = 0; c < D / 32; ++c) {
-            uint32_t o[32];
-            tmem_ld32(o_addr + c * 32, o);
-            tmem_wait_ld();
-#pragma unroll
-            for (int x = 0; x < 8; ++x)
-              dst[c * 8 + x] =
-                  make_float4(__uint_as_float(o[4 * x]), __uint_as_float(o[4 * x + 1]),
-                              __uint_as_float(o[4 * x + 2]), __uint_as_float(o[4 * x + 3]));
-          }
-          tc_fence_before();
+          for (int x = 0; x < 8; ++x)
+            dst[(c * 8 + x) * kPcRows] =
+                make_float4(__uint_as_float(o[4 * x]), __uint_as_float(o[4 * x + 1]),
+                            __uint_as_float(o[4 * x + 2]), __uint_as_float(o[4 * x + 3]));
         }
         if (!meet()) break;
         if (row == 0) {
@@ -705,48 +678,87 @@ __global__ void __launch_bounds__(kPcThreads, 1)
           __threadfence();
         }
         if (!meet()) break;
-        if (s_last[t]) {
-          // the last to arrive: partials of CTAs c_first .. c_last in that order, a warp per row
-          constexpr int kV = D / 32;  // floats of a row per lane
-          const int rows = min(sg->rows - t * kPcTile, kPcTile);
-          for (int x = warp & 3; x < rows; x += 4) {
-            const int ri = t * kPcTile + x;
-            float m = -INFINITY;
-            for (int c = c_first; c <= c_last; ++c)
-              m = fmaxf(m, __ldcg(&a.part.ml[(2 * static_cast<int64_t>(c) + (c == c_first)) *
-                                                 kPcRows + ri]).x);
-            const float mr = m == -INFINITY ? 0.f : m;
-            float l = 0.f, v[kV];
-#pragma unroll
-            for (int y = 0; y < kV; ++y) v[y] = 0.f;
-#pragma unroll 2
-            for (int c = c_first; c <= c_last; ++c) {
-              const int64_t at = (2 * static_cast<int64_t>(c) + (c == c_first)) * kPcRows + ri;
-              const float2 ml = __ldcg(&a.part.ml[at]);
-              const float f = exp2_approx(ml.x - mr);
-              l += ml.y * f;
-#pragma unroll
-              for (int y = 0; y < kV / 2; ++y) {
-                const float2 w =
-                    __ldcg(reinterpret_cast<const float2*>(a.part.o + at * D) + y * 32 + lane);
-                v[2 * y] += w.x * f;
-                v[2 * y + 1] += w.y * f;
-              }
-            }
-            const int rg = sg->r0 + ri;
-            const int64_t to = sg->tok0 + rg / g;
-            const int h = sg->head * g + rg % g;
-            const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
-#pragma unroll
-            for (int y = 0; y < kV / 2; ++y)
-              *(reinterpret_cast<uint32_t*>(a.q.out + to * a.q.o_ts + h * a.q.o_hs) + y * 32 +
-                lane) = l == 0.f ? 0u : pack16<kBF16>(v[2 * y] * inv, v[2 * y + 1] * inv);
-            if (a.q.lse && lane == 0)
-              a.q.lse[to * a.q.heads + h] =
-                  l == 0.f ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f;
+        write = s_last[t] != 0;
+      }
+      if (write) {
+        float m = ref, l = sum;
+        const bool split = units != sg->item_units;
+        auto slot_of = [&](int c) { return (2 * static_cast<int64_t>(c) + (c == c_first)) * kPcRows; };
+        if (split) {  // the last to arrive adds the parts up, in the CTAs' order
+          m = -INFINITY;
+          l = 0.f;
+#pragma unroll 4
+          for (int c = c_first; c <= c_last; ++c)
+            m = fmaxf(m, __ldcg(&a.part.ml[slot_of(c) + r_item]).x);
+        }
+        const float mr = m == -INFINITY ? 0.f : m;
+        if (split) {
+#pragma unroll 4
+          for (int c = c_first; c <= c_last; ++c) {
+            const float2 ml = __ldcg(&a.part.ml[slot_of(c) + r_item]);
+            l += ml.y * exp2_approx(ml.x - mr);
           }
         }
+        const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);  // NaN stays NaN
+        // 16-bit rows by way of the warp's own rows of the queries, which nothing reads any
+        // more, then whole rows side by side to memory
+        uint8_t* stage = s_q + t * C::kTileBytes + (warp & 3) * 32 * 128;
+        auto staged = [&](int r, int c) {  // 16 bytes: chunk c of the warp's row r
+          return reinterpret_cast<uint4*>(stage + (c >> 3) * kPcHalf + r * 128 +
+                                          (((c & 7) ^ (r & 7)) << 4));
+        };
+#pragma unroll
+        for (int c = 0; c < D / 32; ++c) {
+          float v[32];
+          if (split) {
+#pragma unroll
+            for (int x = 0; x < 32; ++x) v[x] = 0.f;
+            for (int k = c_first; k <= c_last; ++k) {
+              const int64_t sl_k = slot_of(k);
+              const float f = exp2_approx(__ldcg(&a.part.ml[sl_k + r_item]).x - mr);
+              const float4* o = reinterpret_cast<const float4*>(a.part.o + sl_k * D) + r_item;
+#pragma unroll
+              for (int x = 0; x < 8; ++x) {
+                const float4 w = __ldcg(o + (c * 8 + x) * kPcRows);
+                v[4 * x] += w.x * f, v[4 * x + 1] += w.y * f;
+                v[4 * x + 2] += w.z * f, v[4 * x + 3] += w.w * f;
+              }
+            }
+          } else {
+            uint32_t o[32];
+            tmem_ld32(o_addr + c * 32, o);
+            tmem_wait_ld();
+#pragma unroll
+            for (int x = 0; x < 32; ++x) v[x] = __uint_as_float(o[x]);
+          }
+#pragma unroll
+          for (int x = 0; x < 4; ++x) {
+            uint32_t w[4];
+#pragma unroll
+            for (int y = 0; y < 4; ++y)
+              w[y] = l == 0.f ? 0u : pack16<kBF16>(v[x * 8 + 2 * y] * inv, v[x * 8 + 2 * y + 1] * inv);
+            *staged(lane, c * 4 + x) = make_uint4(w[0], w[1], w[2], w[3]);
+          }
+        }
+        __syncwarp();
+        constexpr int kLanes = D / 8;  // lanes per row
+        const int part_of = lane % kLanes;
+        const int rows = min(32, sg->rows - t * kPcTile - (warp & 3) * 32);
+#pragma unroll 4
+        for (int x = lane / kLanes; x < rows; x += 32 / kLanes) {
+          const int r = sg->r0 + t * kPcTile + (warp & 3) * 32 + x;
+          *(reinterpret_cast<uint4*>(a.q.out + static_cast<int64_t>(sg->tok0 + r / g) * a.q.o_ts +
+                                     (sg->head * g + r % g) * a.q.o_hs) +
+            part_of) = *staged(x, part_of);
+        }
+        __syncwarp();
+        if (valid && a.q.lse) {
+          const int r = sg->r0 + r_item;
+          a.q.lse[static_cast<int64_t>(sg->tok0 + r / g) * a.q.heads + sg->head * g + r % g] =
+              l == 0.f ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f;
+        }
       }
+      tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(&gempty[n_seg & 1u]);
     }

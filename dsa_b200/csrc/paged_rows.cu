@@ -168,8 +168,8 @@ __global__ void __launch_bounds__(kPrThreads, 2) paged_rows_kernel(const RowsArg
     off = static_cast<int>(u_begin - sel_item * sel_units);
     sel_load(sel_item);
   } else {
-    const PagedSlice sl = paged_find_slice<kPrThreads, kRows, kPrUnit>(a.p, a.q, ctas, cta,
-                                                                      s_scan, s_meta);
+    const PagedSlice sl = paged_find_slice<kPrThreads, kRows, kPrUnit>(
+        a.p, a.q, ctas, cta, s_scan, reinterpret_cast<int*>(smem), s_meta);
     units = sl.units;
     ctas = sl.ctas;
     if (cta >= ctas) return;
@@ -557,27 +557,41 @@ __global__ void __launch_bounds__(kPrThreads, 2) paged_rows_kernel(const RowsArg
       }
       __syncthreads();
       if (s_meta[4]) {
-        // the last to arrive: partials of CTAs c_first .. c_last, in that order
-        for (int r = rg; r < it.rows; r += kG) {
-          float m = -INFINITY;
-          for (int c = c_first; c <= c_last; ++c) {
-            const int64_t sl = 2 * static_cast<int64_t>(c) + (c == c_first ? 1 : 0);
-            m = fmaxf(m, __ldcg(&a.part.ml[sl * kRows + r]).x);
-          }
+        // the last to arrive: partials of CTAs c_first .. c_last, in that order.  First every
+        // row's maximum, sum and the partials' factors (a warp per row, a lane per partial),
+        // then the rows themselves.
+        const int parts = c_last - c_first + 1;
+        float* fac = reinterpret_cast<float*>(smem);  // [row][parts]; the ring is idle
+        auto slot_of = [&](int p) { return 2 * static_cast<int64_t>(c_first + p) + (p == 0); };
+        for (int r = warp; r < it.rows; r += kPrWarps) {
+          float m = -INFINITY, l = 0.f;
+          for (int p = lane; p < parts; p += 32)
+            m = fmaxf(m, __ldcg(&a.part.ml[slot_of(p) * kRows + r]).x);
+#pragma unroll
+          for (int o2 = 16; o2 > 0; o2 >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o2));
           const float ref = m == -INFINITY ? 0.f : m;
-          float l = 0.f;
-          float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
-          for (int c = c_first; c <= c_last; ++c) {
-            const int64_t sl = 2 * static_cast<int64_t>(c) + (c == c_first ? 1 : 0);
-            const float2 ml = __ldcg(&a.part.ml[sl * kRows + r]);
-            const float4 x =
-                __ldcg(reinterpret_cast<const float4*>(a.part.o + (sl * kRows + r) * D) + col);
+          for (int p = lane; p < parts; p += 32) {
+            const float2 ml = __ldcg(&a.part.ml[slot_of(p) * kRows + r]);
             const float f = exp2_approx(ml.x - ref);
+            fac[r * parts + p] = f;
             l += ml.y * f;
+          }
+#pragma unroll
+          for (int o2 = 16; o2 > 0; o2 >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o2);
+          if (lane == 0) s_ml[r] = make_float2(m, l);
+        }
+        __syncthreads();
+        for (int r = rg; r < it.rows; r += kG) {
+          const float2 ml = s_ml[r];
+          float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 8
+          for (int p = 0; p < parts; ++p) {
+            const float4 x = __ldcg(
+                reinterpret_cast<const float4*>(a.part.o + (slot_of(p) * kRows + r) * D) + col);
+            const float f = fac[r * parts + p];
             v.x += x.x * f, v.y += x.y * f, v.z += x.z * f, v.w += x.w * f;
           }
-          store_row(r, m, l, v);
+          store_row(r, ml.x, ml.y, v);
         }
       }
     }

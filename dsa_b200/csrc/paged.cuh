@@ -83,12 +83,20 @@ __device__ __forceinline__ float exp2_approx(float x) {
   return y;
 }
 
-// Slice of CTA c of `ctas` (at most `units`) over `units`, and the CTA whose slice holds unit u.
+// Slice of CTA c of `ctas` (at most `units`) over `units`, and the CTA whose slice holds unit u:
+// the first units % ctas slices have one unit more.  32-bit divisions where they do.
+__device__ __forceinline__ int64_t quotient(int64_t a, int64_t b) {
+  if ((a | b) >> 31) return a / b;
+  return static_cast<uint32_t>(a) / static_cast<uint32_t>(b);
+}
 __device__ __forceinline__ int64_t slice_begin(int64_t units, int ctas, int c) {
-  return units * c / ctas;
+  const int64_t base = quotient(units, ctas);
+  return base * c + min(static_cast<int64_t>(c), units - base * ctas);
 }
 __device__ __forceinline__ int slice_owner(int64_t units, int ctas, int64_t u) {
-  return static_cast<int>(((u + 1) * ctas - 1) / units);
+  const int64_t base = quotient(units, ctas), more = units - base * ctas;
+  if (u < more * (base + 1)) return static_cast<int>(quotient(u, base + 1));
+  return static_cast<int>(more + quotient(u - more * (base + 1), base));
 }
 
 // Workspace of a split call: one arrival counter per CTA (an item that is split is known by
@@ -270,8 +278,9 @@ __device__ __forceinline__ PagedSlice paged_find_slice(const PagedView& p, const
       const int64_t rest = r.begin - at;
       s_found[0] = b;
       s_found[1] = rt;
-      s_found[2] = static_cast<int>(rest / n);
-      s_found[3] = static_cast<int>(rest % n);
+      const int64_t head = quotient(rest, n);
+      s_found[2] = static_cast<int>(head);
+      s_found[3] = static_cast<int>(rest - head * n);
       return false;
     });
   }

@@ -26,7 +26,6 @@
 // product (2^-8 relative in bf16, 2^-11 in f16, the rounding that the output gets too); the sum
 // adds the unrounded P.
 #include <algorithm>
-#include <type_traits>
 
 #include "paged.cuh"
 
@@ -247,8 +246,9 @@ __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity,
   return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag));
 }
 
-// 2^x of two values on the fma pipe, for -126 <= x (smaller ones are taken as -126) and x well
-// below 2^22: x = n + f with n the nearest integer (read off the low bits of x + 1.5 2^23) and
+// 2^x of two values on the fma pipe, for x well below 2^22; x below -126 is taken as -126, so a
+// key that a row does not see weighs 2^-126 instead of nothing (rows that see no key at all are
+// told by their maximum). x = n + f with n the nearest integer (read off the low bits of x + 1.5 2^23) and
 // |f| <= 1/2, 2^f by the degree-4 polynomial of least largest relative error (2.6e-6, found by
 // Remez exchange), n added to the exponent.
 __device__ __forceinline__ float2 exp2_poly2(uint64_t x2) {
@@ -446,9 +446,9 @@ __global__ void __launch_bounds__(kPcThreads, 1)
     const uint32_t s_addr = tmem + lane_base + t * 128;
     const uint32_t o_addr = tmem + lane_base + C::kOCol + t * D;
     const float scale = a.q.scale_log2;
-    uint32_t s_ph[2] = {0, 0};
+    // one bit per buffer: the parity of its next S, and whether its last product was the threads'
+    uint32_t s_ph = 0, was_alone = 0;
     uint32_t n_unit = 0;  // units of the CTA's list before the segment
-    bool was_alone[2] = {false, false};
     // the tile's warps meet (a bounded wait); false when the CTA aborts
     uint32_t met_n = 0;
     int vote = 0;
@@ -496,11 +496,11 @@ __global__ void __launch_bounds__(kPcThreads, 1)
       int base = sg->unit0 * kPcUnit;
       bool ok = true;
       for (int i = 0; i < units && ok; ++i) {
-#pragma unroll
+#pragma unroll 1
         for (int b = 0; b < 2; ++b, base += kPcPart) {
-          if (ok) ok = warp_wait(&sfull[2 * t + b], s_ph[b], abort_flag);
+          ok = warp_wait(&sfull[2 * t + b], (s_ph >> b) & 1u, abort_flag);
           if (!ok) break;
-          s_ph[b] ^= 1u;
+          s_ph ^= 1u << b;
           tc_fence_after();
           const uint32_t sb = s_addr + b * kPcPart;
           uint32_t s[2][32];
@@ -509,9 +509,9 @@ __global__ void __launch_bounds__(kPcThreads, 1)
           // written before the unit's copies were, so it is there when S is
           const uint32_t gone = (absent[(n_unit + i) & 15] >> (4 * b)) & 15u;
           const bool masked = base < all_lo || base + kPcPart > all_hi || gone;
-          if (was_alone[b] && !masked) {  // this buffer's products are the tensor core's again
+          if (((was_alone >> b) & 1u) && !masked) {  // the tensor core's again
             if (row == 0) skip[2 * t + b] = 0;
-            was_alone[b] = false;
+            was_alone &= ~(1u << b);
           }
           tmem_wait_ld();
           if (masked) {
@@ -542,10 +542,10 @@ __global__ void __launch_bounds__(kPcThreads, 1)
             sum *= f;
             if (i > 0 || b > 0) {
               // O += P V of the part before is complete with the S after this one
-              ok = warp_wait(&sfull[2 * t + (b ^ 1)], s_ph[b ^ 1], abort_flag);
+              ok = warp_wait(&sfull[2 * t + (b ^ 1)], (s_ph >> (b ^ 1)) & 1u, abort_flag);
               if (!ok) break;
               tc_fence_after();
-#pragma unroll
+#pragma unroll 1
               for (int c = 0; c < D / 16; ++c) {
                 uint32_t o[16];
                 tmem_ld16(o_addr + c * 16, o);
@@ -559,9 +559,9 @@ __global__ void __launch_bounds__(kPcThreads, 1)
           const float neg = ref == -INFINITY ? 0.f : -ref;
           const uint64_t scale2 = pair(scale, scale), neg2 = pair(neg, neg);
           uint64_t part[2] = {0ull, 0ull};
-          // P of columns 32 c .. 32 c + 31; a third of the pairs take the polynomial, which does
-          // not take the -infinity of a masked score
-          auto weights = [&](int c, auto poly) {
+          // a third of the pairs take the polynomial
+#pragma unroll
+          for (int c = 0; c < 2; ++c) {
             uint32_t p[16];
 #pragma unroll
             for (int j = 0; j < 16; ++j) {
@@ -569,7 +569,7 @@ __global__ void __launch_bounds__(kPcThreads, 1)
                   fma2(pair(__uint_as_float(s[c][2 * j]), __uint_as_float(s[c][2 * j + 1])), scale2,
                        neg2);
               float2 e;
-              if (decltype(poly)::value && j % 3 == 1) {
+              if (j % 3 == 1) {
                 e = exp2_poly2(x2);
               } else {
                 const float2 x = unpair(x2);
@@ -579,13 +579,6 @@ __global__ void __launch_bounds__(kPcThreads, 1)
               p[j] = pack16<kBF16>(e.x, e.y);
             }
             tmem_st16(sb + c * 16, p);
-          };
-          if (masked) {
-            weights(0, std::false_type{});
-            weights(1, std::false_type{});
-          } else {
-            weights(0, std::true_type{});
-            weights(1, std::true_type{});
           }
           {
             const float2 x = unpair(add2(part[0], part[1]));
@@ -621,14 +614,14 @@ __global__ void __launch_bounds__(kPcThreads, 1)
             const bool alone = s_odd[3 * t + vote] != 0;
             vote = next_vote;
             if (alone) {
-              ok = warp_wait(&sfull[2 * t + (b ^ 1)], s_ph[b ^ 1], abort_flag);
+              ok = warp_wait(&sfull[2 * t + (b ^ 1)], (s_ph >> (b ^ 1)) & 1u, abort_flag);
               if (!ok) break;
               tc_fence_after();
               add_visible<kBF16, D>(sb, o_addr, sv, max(0, lo - base), min(kPcPart, hi - base),
                                     i == 0 && b == 0);
             }
-            if (alone != was_alone[b] && row == 0) skip[2 * t + b] = alone ? 1 : 0;
-            was_alone[b] = alone;
+            if (row == 0) skip[2 * t + b] = alone ? 1 : 0;
+            was_alone = (was_alone & ~(1u << b)) | (static_cast<uint32_t>(alone) << b);
           }
           tc_fence_before();
           __syncwarp();
@@ -638,11 +631,9 @@ __global__ void __launch_bounds__(kPcThreads, 1)
       n_unit += units;
 
       // ---------------------------------------------------------- output
-#pragma unroll
-      for (int b = 0; b < 2; ++b) {
-        if (ok) ok = warp_wait(&sfull[2 * t + b], s_ph[b], abort_flag);
-        s_ph[b] ^= 1u;
-      }
+      for (int b = 0; b < 2; ++b)
+        if (ok) ok = warp_wait(&sfull[2 * t + b], (s_ph >> b) & 1u, abort_flag);
+      s_ph ^= 3u;
       if (!ok) break;
       tc_fence_after();
       const int g = a.q.group;
@@ -656,7 +647,7 @@ __global__ void __launch_bounds__(kPcThreads, 1)
         const int64_t slot = 2 * cta + (cta == c_first ? 1 : 0);
         a.part.ml[slot * kPcRows + r_item] = make_float2(ref, sum);
         float4* dst = reinterpret_cast<float4*>(a.part.o + slot * kPcRows * D) + r_item;
-#pragma unroll
+#pragma unroll 1
         for (int c = 0; c < D / 32; ++c) {
           uint32_t o[32];
           tmem_ld32(o_addr + c * 32, o);
@@ -699,7 +690,9 @@ __global__ void __launch_bounds__(kPcThreads, 1)
             l += ml.y * exp2_approx(ml.x - mr);
           }
         }
-        const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);  // NaN stays NaN
+        // a row that sees no key has no maximum; one whose scores are all NaN has a NaN sum
+        const bool none = m == -INFINITY && l == l;
+        const float inv = 1.f / l;
         // 16-bit rows by way of the warp's own rows of the queries, which nothing reads any
         // more, then whole rows side by side to memory
         uint8_t* stage = s_q + t * C::kTileBytes + (warp & 3) * 32 * 128;
@@ -707,7 +700,7 @@ __global__ void __launch_bounds__(kPcThreads, 1)
           return reinterpret_cast<uint4*>(stage + (c >> 3) * kPcHalf + r * 128 +
                                           (((c & 7) ^ (r & 7)) << 4));
         };
-#pragma unroll
+#pragma unroll 1
         for (int c = 0; c < D / 32; ++c) {
           float v[32];
           if (split) {
@@ -736,7 +729,7 @@ __global__ void __launch_bounds__(kPcThreads, 1)
             uint32_t w[4];
 #pragma unroll
             for (int y = 0; y < 4; ++y)
-              w[y] = l == 0.f ? 0u : pack16<kBF16>(v[x * 8 + 2 * y] * inv, v[x * 8 + 2 * y + 1] * inv);
+              w[y] = none ? 0u : pack16<kBF16>(v[x * 8 + 2 * y] * inv, v[x * 8 + 2 * y + 1] * inv);
             *staged(lane, c * 4 + x) = make_uint4(w[0], w[1], w[2], w[3]);
           }
         }
@@ -755,7 +748,7 @@ __global__ void __launch_bounds__(kPcThreads, 1)
         if (valid && a.q.lse) {
           const int r = sg->r0 + r_item;
           a.q.lse[static_cast<int64_t>(sg->tok0 + r / g) * a.q.heads + sg->head * g + r % g] =
-              l == 0.f ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f;
+              none ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f;
         }
       }
       tc_fence_before();

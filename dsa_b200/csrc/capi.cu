@@ -299,6 +299,9 @@ int paged_query(const tdsa_paged_cache* c, int tokens, const tdsa_token_rows* q,
   d.lse = lse;
   d.heads = q_heads;
   d.group = q_heads / c->kv_heads;
+  if (d.group > 1024)
+    return fail(TDSA_ERR_UNSUPPORTED, "at most 1024 query heads per key/value head");
+  d.group_magic = d.group > 1 ? static_cast<uint32_t>((uint64_t(1) << 32) / d.group + 1) : 0u;
   d.scale_log2 = scale * 1.4426950408889634f;
   d.window = 0;
   d.idx = nullptr;

@@ -128,6 +128,7 @@ struct PagedQuery {
   int64_t o_ts, o_hs;
   float* lse;        // [tokens][heads] or null
   int heads, group;  // query heads, query heads per key/value head
+  uint32_t group_magic;  // floor(2^32 / group) + 1 (0 for a group of 1): see row_token
   float scale_log2;  // scale * log2(e)
   int window;        // keys a token sees up to its own position; 0: all
   // selected attention: [tokens][topk] positions of idx_bytes each
@@ -135,6 +136,12 @@ struct PagedQuery {
   int64_t idx_stride;
   int idx_bytes, topk;
 };
+
+// r / group for r below 2^16 (groups up to 2^10): r (magic group - 2^32) < 2^32 / group holds, so
+// the high half of r * magic is the quotient.
+__device__ __forceinline__ int row_token(const PagedQuery& q, int r) {
+  return q.group_magic ? static_cast<int>(__umulhi(static_cast<uint32_t>(r), q.group_magic)) : r;
+}
 
 // One item: rows [r0, r0 + rows) of the (token, head) rows of a sequence and key/value head.
 struct PagedItem {

@@ -270,9 +270,12 @@ __device__ __forceinline__ float2 exp2_poly2(uint64_t x2) {
 // A segment of an item, published by the copy warp to the others.
 struct ChunkSegment {
   int unit0, units;    // first unit and number of units (0: the CTA's list ends)
-  int item_units, pad;
+  int item_units, rows;
   int64_t item_u0;     // the item's first unit in the call's list
-  int head, tok0, r0, rows, pos0, k0, k1, pad2;
+  // row r of the item: rl = sub + r; token tok + rl / group at position pos + rl / group, query
+  // head head0 + rl % group
+  int head0, tok, pos, sub;
+  int k0, k1;          // keys any row sees
 };
 
 template <bool kBF16, int D>
@@ -376,9 +379,13 @@ __global__ void __launch_bounds__(kPcThreads, 1)
         g.units = seg;
         g.item_units = n;
         g.item_u0 = u - off;
-        g.head = it.head, g.tok0 = it.tok0, g.r0 = it.r0, g.rows = it.rows, g.pos0 = it.pos0;
+        g.rows = it.rows;
+        const int t0 = it.r0 / a.q.group;
+        g.head0 = it.head * a.q.group;
+        g.tok = it.tok0 + t0;
+        g.pos = it.pos0 + t0;
+        g.sub = it.r0 - t0 * a.q.group;
         g.k0 = it.k0, g.k1 = it.k1;
-        g.pad = g.pad2 = 0;
         s_seg[gs] = g;
         mbar_arrive(&gfull[gs]);
       }
@@ -468,29 +475,45 @@ __global__ void __launch_bounds__(kPcThreads, 1)
         if (lane == 0) mbar_arrive(&gempty[n_seg & 1u]);
         continue;
       }
-      const bool valid = t * kPcTile + row < sg->rows;
+      const int g = a.q.group;
+      const int w_row0 = t * kPcTile + (warp & 3) * 32;    // the warp's first row
+      const int w_rows = min(32, sg->rows - w_row0);       // its rows (none: <= 0)
+      const bool valid = lane < w_rows;
+      // the address of 16 bytes of row r of the warp's, chunk c: whole rows side by side
+      constexpr int kLanes = D / 8;
+      const int my_c = lane % kLanes;
+      auto row_at = [&](auto* p, int64_t ts, int64_t hs, int r) {
+        const int rl = sg->sub + w_row0 + r, tk = row_token(a.q, rl);
+        return p + static_cast<int64_t>(sg->tok + tk) * ts + (sg->head0 + rl - tk * g) * hs +
+               my_c * 8;
+      };
+      // the warp's rows of the query tile (later of the output): chunk c of row r
+      uint8_t* const s_rows = s_q + t * C::kTileBytes + (warp & 3) * 32 * 128;
+      auto staged = [&](int r, int c) {
+        return reinterpret_cast<uint4*>(s_rows + (c >> 3) * kPcHalf + r * 128 +
+                                        (((c & 7) ^ (r & 7)) << 4));
+      };
       int lo, hi, all_lo, all_hi;  // keys this row sees; keys every row of the tile sees
       {
-        const int g = a.q.group, r = sg->r0 + t * kPcTile + row;
-        const uint4* src = reinterpret_cast<const uint4*>(
-            a.q.q + (valid ? static_cast<int64_t>(sg->tok0 + r / g) * a.q.q_ts +
-                                 (sg->head * g + r % g) * a.q.q_hs
-                           : 0));
-        uint8_t* dst = s_q + t * C::kTileBytes + row * 128;
-#pragma unroll
-        for (int c = 0; c < D / 8; ++c) {
-          const uint4 x = valid ? src[c] : make_uint4(0u, 0u, 0u, 0u);
-          *reinterpret_cast<uint4*>(dst + (c >> 3) * kPcHalf + (((c & 7) ^ (row & 7)) << 4)) = x;
+#pragma unroll 8
+        for (int r = lane / kLanes; r < 32; r += 32 / kLanes) {
+          uint4 x = make_uint4(0u, 0u, 0u, 0u);
+          if (r < w_rows)
+            x = *reinterpret_cast<const uint4*>(row_at(a.q.q, a.q.q_ts, a.q.q_hs, r));
+          *staged(r, my_c) = x;
         }
         fence_proxy_async_smem();
         __syncwarp();
         if (lane == 0) mbar_arrive(&qfull[t]);
-        const int pos = sg->pos0 + r / g, w = a.q.window;
-        const int last = min(sg->rows, (t + 1) * kPcTile) - 1;
+        const int w = a.q.window;
+        const int pos = sg->pos + row_token(a.q, sg->sub + w_row0 + lane);
+        const int first = sg->pos + row_token(a.q, sg->sub + t * kPcTile);
+        const int last =
+            sg->pos + row_token(a.q, sg->sub + min(sg->rows, (t + 1) * kPcTile) - 1);
         hi = valid ? min(pos + 1, sg->k1) : sg->k1;
         lo = valid && w > 0 ? max(0, pos - (w - 1)) : 0;
-        all_hi = min(sg->k1, sg->pos0 + (sg->r0 + t * kPcTile) / g + 1);
-        all_lo = w > 0 ? max(sg->k0, sg->pos0 + (sg->r0 + last) / g - (w - 1)) : sg->k0;
+        all_hi = min(sg->k1, first + 1);
+        all_lo = w > 0 ? max(sg->k0, last - (w - 1)) : sg->k0;
       }
       float ref = -INFINITY, sum = 0.f;
       int base = sg->unit0 * kPcUnit;
@@ -636,7 +659,6 @@ __global__ void __launch_bounds__(kPcThreads, 1)
       s_ph ^= 3u;
       if (!ok) break;
       tc_fence_after();
-      const int g = a.q.group;
       const int r_item = t * kPcTile + row;  // row of the item
       const int c_first = slice_owner(sl.units, sl.ctas, sg->item_u0);
       const int c_last = slice_owner(sl.units, sl.ctas, sg->item_u0 + sg->item_units - 1);
@@ -695,11 +717,6 @@ __global__ void __launch_bounds__(kPcThreads, 1)
         const float inv = 1.f / l;
         // 16-bit rows by way of the warp's own rows of the queries, which nothing reads any
         // more, then whole rows side by side to memory
-        uint8_t* stage = s_q + t * C::kTileBytes + (warp & 3) * 32 * 128;
-        auto staged = [&](int r, int c) {  // 16 bytes: chunk c of the warp's row r
-          return reinterpret_cast<uint4*>(stage + (c >> 3) * kPcHalf + r * 128 +
-                                          (((c & 7) ^ (r & 7)) << 4));
-        };
 #pragma unroll 1
         for (int c = 0; c < D / 32; ++c) {
           float v[32];
@@ -734,20 +751,13 @@ __global__ void __launch_bounds__(kPcThreads, 1)
           }
         }
         __syncwarp();
-        constexpr int kLanes = D / 8;  // lanes per row
-        const int part_of = lane % kLanes;
-        const int rows = min(32, sg->rows - t * kPcTile - (warp & 3) * 32);
 #pragma unroll 4
-        for (int x = lane / kLanes; x < rows; x += 32 / kLanes) {
-          const int r = sg->r0 + t * kPcTile + (warp & 3) * 32 + x;
-          *(reinterpret_cast<uint4*>(a.q.out + static_cast<int64_t>(sg->tok0 + r / g) * a.q.o_ts +
-                                     (sg->head * g + r % g) * a.q.o_hs) +
-            part_of) = *staged(x, part_of);
-        }
+        for (int r = lane / kLanes; r < w_rows; r += 32 / kLanes)
+          *reinterpret_cast<uint4*>(row_at(a.q.out, a.q.o_ts, a.q.o_hs, r)) = *staged(r, my_c);
         __syncwarp();
         if (valid && a.q.lse) {
-          const int r = sg->r0 + r_item;
-          a.q.lse[static_cast<int64_t>(sg->tok0 + r / g) * a.q.heads + sg->head * g + r % g] =
+          const int rl = sg->sub + r_item, tk = row_token(a.q, rl);
+          a.q.lse[static_cast<int64_t>(sg->tok + tk) * a.q.heads + sg->head0 + rl - tk * g] =
               none ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f;
         }
       }

@@ -283,6 +283,8 @@ int paged_query(const tdsa_paged_cache* c, int tokens, const tdsa_token_rows* q,
   int rc = check_token_rows(q, q_heads, c->head_dim, "q");
   if (!rc) rc = check_token_rows(out, q_heads, c->head_dim, "out");
   if (rc) return rc;
+  if (q->data == out->data)
+    return fail(TDSA_ERR_INVALID, "out must not be q: a row may be read after others are written");
   if (!(scale > 0.f) || scale > 1e30f)
     return fail(TDSA_ERR_INVALID, "scale must be positive and finite");
   if (!ws || ws_bytes < tdsa_paged_workspace_bytes(c->head_dim) ||

@@ -495,13 +495,18 @@ __global__ void __launch_bounds__(kPcThreads, 1)
       };
       int lo, hi, all_lo, all_hi;  // keys this row sees; keys every row of the tile sees
       {
-#pragma unroll 8
-        for (int r = lane / kLanes; r < 32; r += 32 / kLanes) {
-          uint4 x = make_uint4(0u, 0u, 0u, 0u);
-          if (r < w_rows)
-            x = *reinterpret_cast<const uint4*>(row_at(a.q.q, a.q.q_ts, a.q.q_hs, r));
-          *staged(r, my_c) = x;
+        // every load is under way before the first is stored
+        constexpr int kStep = 32 / kLanes;
+        uint4 x[kLanes];
+#pragma unroll
+        for (int i = 0; i < kLanes; ++i) {
+          const int r = lane / kLanes + i * kStep;
+          x[i] = r < w_rows
+                     ? *reinterpret_cast<const uint4*>(row_at(a.q.q, a.q.q_ts, a.q.q_hs, r))
+                     : make_uint4(0u, 0u, 0u, 0u);
         }
+#pragma unroll
+        for (int i = 0; i < kLanes; ++i) *staged(lane / kLanes + i * kStep, my_c) = x[i];
         fence_proxy_async_smem();
         __syncwarp();
         if (lane == 0) mbar_arrive(&qfull[t]);
@@ -616,17 +621,15 @@ __global__ void __launch_bounds__(kPcThreads, 1)
             ok = warp_wait(&full[st], (vi / C::kStages) & 1u, abort_flag);
             if (!ok) break;
             const uint8_t* sv = smem + st * C::kTileBytes + b * kPcPart * 128;
-            const int key = row & (kPcPart - 1);
             bool odd = false;
-            if (base + key >= sg->k0 && base + key < sg->k1) {
 #pragma unroll
-              for (int x = 0; x < D / 16; ++x) {  // half a row of V per thread
-                const int c = (row / kPcPart) * (D / 16) + x;
-                const uint4 w = *reinterpret_cast<const uint4*>(sv + (c >> 3) * kPcHalf +
-                                                                key * 128 + (c & 7) * 16);
-                odd |= nonfinite16<kBF16>(w.x) || nonfinite16<kBF16>(w.y) ||
-                       nonfinite16<kBF16>(w.z) || nonfinite16<kBF16>(w.w);
-              }
+            for (int x = 0; x < D / 16; ++x) {  // 16 bytes at a time, side by side
+              const int c = (x & 3) * kPcTile + row;
+              const int key = base + (c >> 3);
+              const uint4 w = *reinterpret_cast<const uint4*>(sv + (x >> 2) * kPcHalf + c * 16);
+              odd |= key >= sg->k0 && key < sg->k1 &&
+                     (nonfinite16<kBF16>(w.x) || nonfinite16<kBF16>(w.y) ||
+                      nonfinite16<kBF16>(w.z) || nonfinite16<kBF16>(w.w));
             }
             // three ballots in turn: the next one was last read before the meeting before this
             if (__any_sync(0xffffffffu, odd) && lane == 0) s_odd[3 * t + vote] = 1;
@@ -751,9 +754,18 @@ __global__ void __launch_bounds__(kPcThreads, 1)
           }
         }
         __syncwarp();
-#pragma unroll 4
-        for (int r = lane / kLanes; r < w_rows; r += 32 / kLanes)
-          *reinterpret_cast<uint4*>(row_at(a.q.out, a.q.o_ts, a.q.o_hs, r)) = *staged(r, my_c);
+        {
+          constexpr int kStep = 32 / kLanes;
+          uint4 x[kLanes];
+#pragma unroll
+          for (int i = 0; i < kLanes; ++i) x[i] = *staged(lane / kLanes + i * kStep, my_c);
+#pragma unroll
+          for (int i = 0; i < kLanes; ++i) {
+            const int r = lane / kLanes + i * kStep;
+            if (r < w_rows)
+              *reinterpret_cast<uint4*>(row_at(a.q.out, a.q.o_ts, a.q.o_hs, r)) = x[i];
+          }
+        }
         __syncwarp();
         if (valid && a.q.lse) {
           const int rl = sg->sub + r_item, tk = row_token(a.q, rl);

@@ -661,7 +661,7 @@ int tdsa_paged_append(const tdsa_paged_cache* cache, const tdsa_paged_batch* bat
  *   out[t][h] = sum_j softmax_j(scale * q[t][h] . K[j][h / g]) V[j][h / g],  g = q_heads /
  *   kv_heads;  lse[t][h] = log sum_j exp(scale * q . K[j]) (float32, [tokens][q_heads], NULL:
  *   not wanted).
- * A token that sees no key gets out 0 and lse -inf.  float32 scores, maxima and sums; the
+ * A token that sees no key gets out 0 and lse -inf.  out must not overlap q.  float32 scores, maxima and sums; the
  * softmax weights are rounded to the cache's type for the product with V.  scale > 0.
  * workspace: tdsa_paged_workspace_bytes bytes, 256-byte aligned, zero before its first use;
  * every call leaves it ready for the next one on the same stream.

@@ -40,7 +40,8 @@ def _rows(data=4096, token=1024, head=128):
 def _attend(lib, cache, batch, q=None, out=None, heads=8, scale=1.0, window=0, ws=4096,
             ws_bytes=1 << 40):
     return lib.tdsa_paged_attention(C.byref(cache), C.byref(batch), C.byref(q or _rows()), heads,
-                                    scale, window, C.byref(out or _rows()), None, ws, ws_bytes,
+                                    scale, window, C.byref(out or _rows(data=16384)),
+                                    None, ws, ws_bytes,
                                     None)
 
 
@@ -75,6 +76,8 @@ def test_attention_checks(lib):
     assert _attend(lib, c, b, q=_rows(data=None)) == INVALID
     assert _attend(lib, c, b, q=_rows(data=4098)) == ALIGN
     assert _attend(lib, c, b, out=_rows(token=1025)) == ALIGN
+    assert _attend(lib, c, b, out=_rows()) == INVALID  # q itself
+    assert _attend(lib, c, b, heads=4096) == UNSUP     # 2048 query heads per key/value head
     assert _attend(lib, c, b, out=_rows(token=-1024)) == INVALID
     assert _attend(lib, c, b, scale=0.0) == INVALID
     assert _attend(lib, c, b, scale=float("nan")) == INVALID
@@ -92,7 +95,7 @@ def test_selected_checks(lib):
     def call(idx=4096, nbytes=4, stride=16, k=16):
         return lib.tdsa_selected_attention(
             C.byref(_cache()), C.byref(_batch()), C.byref(_rows()), 8, 1.0, idx, nbytes, stride, k,
-            C.byref(_rows()), None, 4096, 1 << 40, None)
+            C.byref(_rows(data=16384)), None, 4096, 1 << 40, None)
 
     assert call(idx=None) == INVALID
     assert call(nbytes=2) == INVALID

@@ -18,6 +18,8 @@ from __future__ import annotations
 
 import ctypes as C
 import math
+import struct
+import threading
 
 import torch
 
@@ -43,7 +45,8 @@ class PagedKV:
             raise ValueError("keys and values must have the same strides, 1 on the last axis")
         self.keys, self.values = keys, values
         self.pages, self.page_size, self.kv_heads, self.head_dim = keys.shape
-        self.dtype, self.device = keys.dtype, keys.device
+        self.dtype, self.device, self._index = keys.dtype, keys.device, keys.get_device()
+        self._scale = 1.0 / math.sqrt(self.head_dim) if self.head_dim else 1.0
         self._c = capi.TdsaPagedCache(keys.data_ptr(), values.data_ptr(), *keys.stride()[:3],
                                       *keys.shape, _DTYPES[keys.dtype])
         self._ref = C.byref(self._c)
@@ -83,55 +86,77 @@ class PagedBatch:
             raise ValueError("max_new must be >= 0")
         self.page_table, self.query_starts, self.lengths = page_table, query_starts, lengths
         self.batch, self.max_new, self.device = batch, max_new, page_table.device
-        self._c = capi.TdsaPagedBatch(page_table.data_ptr(), page_table.stride(0),
-                                      query_starts.data_ptr(), lengths.data_ptr(), batch,
-                                      page_table.shape[1], 0, 0)
-        self._ref = C.byref(self._c)
+        self._index = page_table.get_device()
+        self._last = (None, None, None)
 
     def _for(self, tokens: int):
-        self._c.tokens = tokens
-        self._c.max_new = tokens if self.max_new is None else min(self.max_new, tokens)
-        return self._ref
+        """The C batch for a call of ``tokens`` rows (kept until the number changes)."""
+        known, limit, ref = self._last
+        if known != tokens or limit != self.max_new:
+            limit, table = self.max_new, self.page_table
+            ref = C.byref(capi.TdsaPagedBatch(
+                table.data_ptr(), table.stride(0), self.query_starts.data_ptr(),
+                self.lengths.data_ptr(), self.batch, table.shape[1], tokens,
+                tokens if limit is None else min(limit, tokens)))
+            self._last = (tokens, limit, ref)
+        return ref
 
 
-def _rows(t: torch.Tensor, cache: PagedKV, heads: int | None, tokens: int | None,
-          name: str) -> capi.TdsaTokenRows:
-    """``t`` [tokens, heads, head_dim] as C rows; strides and alignment are the library's check."""
+class _Rows(threading.local):
+    """This thread's C row descriptors (four tdsa_token_rows), written anew for every call."""
+
+    def __init__(self):
+        self.buffer = (C.c_int64 * 12)()
+        self.address = C.addressof(self.buffer)
+
+
+_ROWS = _Rows()
+_PACK6, _PACK12 = struct.Struct("6q").pack_into, struct.Struct("12q").pack_into
+
+
+def _check_rows(t: torch.Tensor, cache: PagedKV, heads: int | None, tokens: int | None,
+                name: str) -> None:
+    """Why ``t`` is not [tokens, heads, head_dim] rows of the cache's kind, if it is not; strides
+    and alignment are the library's check."""
+    require_cuda(t)
     shape = t.shape
     if len(shape) != 3 or shape[2] != cache.head_dim or (
             heads is not None and shape[1] != heads) or (
             tokens is not None and shape[0] != tokens):
-        raise ValueError(f"{name} must be [tokens, {heads or 'heads'}, {cache.head_dim}], "
-                         f"got {list(shape)}")
+        raise ValueError(f"{name} must be [{'tokens' if tokens is None else tokens}, "
+                         f"{heads or 'heads'}, {cache.head_dim}], got {list(shape)}")
     if t.dtype != cache.dtype:
         raise ValueError(f"{name} must have the cache's dtype")
     if t.device != cache.device:
         raise ValueError(f"{name} must be on the cache's device")
-    ts, hs, ds = t.stride()
-    if ds != 1:
+    if t.stride(-1) != 1:
         raise ValueError(f"{name} needs unit stride on the last axis")
-    return capi.TdsaTokenRows(t.data_ptr(), ts, hs)
 
 
 def _check_batch(batch: PagedBatch, cache: PagedKV) -> None:
-    if batch.device != cache.device:
+    if batch._index != cache._index:
         raise ValueError("batch and cache must be on one device")
 
 
-_WORKSPACES: dict[tuple[int, int, int], torch.Tensor] = {}
+_WORKSPACES: dict[tuple[int, int, int], tuple[torch.Tensor, int, int]] = {}
 
 
-def paged_workspace(device: torch.device, head_dim: int) -> torch.Tensor:
-    """Zeroed scratch of the attention calls.  Outside CUDA-graph capture one buffer per
-    (device, stream, head_dim) is kept: calls on one stream run in order and each leaves it
-    ready for the next.  During a capture a fresh one is returned, which the graph keeps."""
-    key = (device.index, stream_ptr(device), head_dim)
+def paged_workspace(device: torch.device, head_dim: int,
+                    stream: int | None = None) -> tuple[torch.Tensor, int, int]:
+    """Zeroed scratch of the attention calls -> (buffer, address, bytes).  Outside CUDA-graph
+    capture one buffer per (device, stream, head_dim) is kept: calls on one stream run in order
+    and each leaves it ready for the next.  During a capture a fresh one is returned, which the
+    graph keeps."""
+    if stream is None:
+        stream = stream_ptr(device)
+    key = (device.index, stream, head_dim)
     ws = _WORKSPACES.get(key)
     capturing = torch.cuda.is_current_stream_capturing()
     if ws is None or capturing:
         with torch.cuda.device(device):
             nbytes = capi.lib().tdsa_paged_workspace_bytes(head_dim)
-        ws = torch.zeros(max(nbytes, 1), device=device, dtype=torch.uint8)
+        buffer = torch.zeros(max(nbytes, 1), device=device, dtype=torch.uint8)
+        ws = (buffer, buffer.data_ptr(), nbytes)
         if not capturing:
             _WORKSPACES[key] = ws
     return ws
@@ -159,8 +184,9 @@ class PagedAppender:
         if (inv_freq.shape != (half,) or inv_freq.dtype != torch.float32
                 or inv_freq.device != cache.device):
             raise ValueError("inv_freq must be float32 [rope_dim / 2] on the cache's device")
-        self.cache, self.rope_dim, self.interleaved = cache, int(rope_dim), bool(interleaved)
+        self.cache, self.rope_dim, self.interleaved = cache, int(rope_dim), int(bool(interleaved))
         self.inv_freq = inv_freq.contiguous()
+        self._freq = self.inv_freq.data_ptr()
         self._fn = capi.lib().tdsa_paged_append
 
     def append(self, batch: PagedBatch, k: torch.Tensor, v: torch.Tensor,
@@ -171,19 +197,36 @@ class PagedAppender:
         ``positions`` int64 ``[tokens]`` replaces the tokens' positions in the angles."""
         cache = self.cache
         _check_batch(batch, cache)
-        tokens = k.shape[0]
-        kr = _rows(k, cache, cache.kv_heads, None, "k")
-        vr = _rows(v, cache, cache.kv_heads, tokens, "v")
-        qr = qo = None
-        q_heads = 0
+        dtype, index, shape = cache.dtype, cache._index, k.shape
+        ks, vs = k.stride(), v.stride()
+        if not (len(shape) == 3 and shape == v.shape and shape[1] == cache.kv_heads
+                and shape[2] == cache.head_dim and k.dtype is dtype and v.dtype is dtype
+                and k.get_device() == index and v.get_device() == index and ks[2] == 1
+                and vs[2] == 1):
+            _check_rows(k, cache, cache.kv_heads, None, "k")
+            _check_rows(v, cache, cache.kv_heads, shape[0], "v")
+        tokens = shape[0]
+        rows = _ROWS.address
         if q is not None:
-            qr = _rows(q, cache, None, tokens, "q")
-            q_heads = q.shape[1]
+            qshape = q.shape
             if q_out is None:
-                q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-            qo = _rows(q_out, cache, q_heads, tokens, "q_out")
-        elif q_out is not None:
-            raise ValueError("q_out needs q")
+                q_out = torch.empty_like(q)
+            qs, os = q.stride(), q_out.stride()
+            if not (len(qshape) == 3 and qshape[0] == tokens and qshape[2] == cache.head_dim
+                    and q_out.shape == qshape and q.dtype is dtype and q_out.dtype is dtype
+                    and q.get_device() == index and q_out.get_device() == index
+                    and qs[2] == 1 and os[2] == 1):
+                _check_rows(q, cache, None, tokens, "q")
+                _check_rows(q_out, cache, qshape[1], tokens, "q_out")
+            _PACK12(_ROWS.buffer, 0, k.data_ptr(), ks[0], ks[1], v.data_ptr(), vs[0], vs[1],
+                    q.data_ptr(), qs[0], qs[1], q_out.data_ptr(), os[0], os[1])
+            q_rows, o_rows, q_heads = rows + 48, rows + 72, qshape[1]
+        else:
+            if q_out is not None:
+                raise ValueError("q_out needs q")
+            _PACK6(_ROWS.buffer, 0, k.data_ptr(), ks[0], ks[1], v.data_ptr(), vs[0], vs[1])
+            q_rows = o_rows = None
+            q_heads = 0
         pos = None
         if positions is not None:
             if (positions.dtype != torch.int64 or positions.shape != (tokens,)
@@ -191,26 +234,30 @@ class PagedAppender:
                 raise ValueError("positions must be contiguous int64 [tokens] on the cache's "
                                  "device")
             pos = positions.data_ptr()
-        capi.check(self._fn(cache._ref, batch._for(tokens), C.byref(kr), C.byref(vr),
-                            None if qr is None else C.byref(qr),
-                            None if qo is None else C.byref(qo), q_heads,
-                            self.inv_freq.data_ptr(), self.rope_dim, int(self.interleaved), pos,
-                            stream_ptr(cache.device)))
+        rc = self._fn(cache._ref, batch._for(tokens), rows, rows + 24, q_rows, o_rows, q_heads,
+                      self._freq, self.rope_dim, self.interleaved, pos,
+                      stream_ptr(cache.device))
+        if rc:
+            capi.check(rc)
         return q_out
 
 
-def _attention_args(q, cache, batch, scale, out, return_lse):
+def _attention_args(q, cache, batch, out, return_lse):
+    """Checks and descriptors shared by the attention calls."""
     _check_batch(batch, cache)
-    qr = _rows(q, cache, None, None, "q")
-    tokens, heads = q.shape[0], q.shape[1]
+    shape, dtype, index = q.shape, cache.dtype, cache._index
     if out is None:
-        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    orr = _rows(out, cache, heads, tokens, "out")
-    lse = (torch.empty(tokens, heads, dtype=torch.float32, device=q.device) if return_lse
-           else None)
-    if scale is None:
-        scale = 1.0 / math.sqrt(cache.head_dim)
-    return qr, orr, out, lse, tokens, heads, scale, paged_workspace(cache.device, cache.head_dim)
+        out = torch.empty_like(q)
+    qs, os = q.stride(), out.stride()
+    if not (len(shape) == 3 and shape[2] == cache.head_dim and out.shape == shape
+            and q.dtype is dtype and out.dtype is dtype and q.get_device() == index
+            and out.get_device() == index and qs[2] == 1 and os[2] == 1):
+        _check_rows(q, cache, None, None, "q")
+        _check_rows(out, cache, shape[1], shape[0], "out")
+    _PACK6(_ROWS.buffer, 0, q.data_ptr(), qs[0], qs[1], out.data_ptr(), os[0], os[1])
+    lse = (torch.empty(shape[:2], dtype=torch.float32, device=q.device) if return_lse else None)
+    stream = stream_ptr(cache.device)
+    return out, lse, shape, stream, paged_workspace(cache.device, cache.head_dim, stream)
 
 
 def paged_attention(q: torch.Tensor, cache: PagedKV, batch: PagedBatch, *,
@@ -227,12 +274,14 @@ def paged_attention(q: torch.Tensor, cache: PagedKV, batch: PagedBatch, *,
     """
     if window is not None and window < 1:
         raise ValueError("window must be >= 1")
-    qr, orr, out, lse, tokens, heads, scale, ws = _attention_args(q, cache, batch, scale, out,
-                                                                  return_lse)
-    capi.check(capi.lib().tdsa_paged_attention(
-        cache._ref, batch._for(tokens), C.byref(qr), heads, scale, window or 0, C.byref(orr),
-        None if lse is None else lse.data_ptr(), ws.data_ptr(), ws.numel(),
-        stream_ptr(cache.device)))
+    out, lse, shape, stream, ws = _attention_args(q, cache, batch, out, return_lse)
+    rows = _ROWS.address
+    rc = capi.lib().tdsa_paged_attention(
+        cache._ref, batch._for(shape[0]), rows, shape[1],
+        cache._scale if scale is None else scale, window or 0, rows + 24,
+        None if lse is None else lse.data_ptr(), ws[1], ws[2], stream)
+    if rc:
+        capi.check(rc)
     return (out, lse) if return_lse else out
 
 
@@ -242,18 +291,20 @@ def selected_attention(q: torch.Tensor, cache: PagedKV, batch: PagedBatch,
     """Attention of every new token over the positions it lists: ``indices`` int32 or int64
     ``[tokens, k]``, positions of the token's own sequence in any order, negative entries
     skipped -- what ``topk`` and ``ScoreTopkPlan`` return.  The rest as ``paged_attention``."""
-    require_cuda(indices)
-    qr, orr, out, lse, tokens, heads, scale, ws = _attention_args(q, cache, batch, scale, out,
-                                                                  return_lse)
-    if indices.dim() != 2 or indices.shape[0] != tokens or indices.shape[1] < 1:
+    out, lse, shape, stream, ws = _attention_args(q, cache, batch, out, return_lse)
+    ishape, itype = indices.shape, indices.dtype
+    if len(ishape) != 2 or ishape[0] != shape[0] or ishape[1] < 1:
         raise ValueError("indices must be [tokens, k]")
-    if indices.dtype not in (torch.int32, torch.int64):
+    if itype is not torch.int32 and itype is not torch.int64:
         raise ValueError("indices must be int32 or int64")
-    if indices.stride(-1) != 1 or indices.device != cache.device:
+    if indices.stride(1) != 1 or indices.get_device() != cache._index:
         raise ValueError("indices need unit last stride, on the cache's device")
-    capi.check(capi.lib().tdsa_selected_attention(
-        cache._ref, batch._for(tokens), C.byref(qr), heads, scale, indices.data_ptr(),
-        indices.element_size(), indices.stride(0), indices.shape[1], C.byref(orr),
-        None if lse is None else lse.data_ptr(), ws.data_ptr(), ws.numel(),
-        stream_ptr(cache.device)))
+    rows = _ROWS.address
+    rc = capi.lib().tdsa_selected_attention(
+        cache._ref, batch._for(shape[0]), rows, shape[1],
+        cache._scale if scale is None else scale, indices.data_ptr(), indices.element_size(),
+        indices.stride(0), ishape[1], rows + 24, None if lse is None else lse.data_ptr(), ws[1],
+        ws[2], stream)
+    if rc:
+        capi.check(rc)
     return (out, lse) if return_lse else out

@@ -7,8 +7,7 @@
 //
 // The angle is formed and reduced by 2 pi in float64 (a float32 product is off by up to 2^-24 p
 // radians, 0.002 at p = 32768), the hardware sine and cosine take the reduced angle, and the
-// products are float32 with one rounding at the end.  The angles of a token are computed once,
-// by one thread each, into shared memory and used by all its heads.
+// products are float32 with one rounding at the end.
 #include <algorithm>
 
 #include "paged.cuh"
@@ -17,7 +16,11 @@ namespace tdsa {
 
 namespace {
 
-constexpr int kPaThreads = 256;
+// Threads of a CTA and the rows a lane loads ahead: long calls take fewer threads with more loads
+// under way each (8698 tokens of 48 heads: 38 us with 128, 42 with 256), short ones more threads
+// (64 tokens: 4.0 us with 128, 3.1 with 256).
+constexpr int kPaShort = 256, kPaLong = 128;
+constexpr int kPaHeldRows = 768;  // threads times rows ahead
 
 struct AppendArgs {
   PagedView p;
@@ -33,98 +36,119 @@ struct AppendArgs {
   int* status;
 };
 
-// 8 features (16 bytes) of one row: out = R x for the pairs in it
-template <bool kBF16>
-__device__ __forceinline__ uint4 turn_pairs(uint4 x, const float2* cs) {
-  uint32_t r[4] = {x.x, x.y, x.z, x.w};
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const float2 v = unpack16<kBF16>(r[i]), c = cs[i];
-    r[i] = pack16<kBF16>(v.x * c.x - v.y * c.y, v.y * c.x + v.x * c.y);
-  }
-  return make_uint4(r[0], r[1], r[2], r[3]);
-}
-
-template <bool kBF16>
-__device__ __forceinline__ void turn_halves(uint4& a, uint4& b, const float2* cs) {
-  uint32_t x[4] = {a.x, a.y, a.z, a.w}, y[4] = {b.x, b.y, b.z, b.w};
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const float2 u = unpack16<kBF16>(x[i]), w = unpack16<kBF16>(y[i]);
-    const float2 c0 = cs[2 * i], c1 = cs[2 * i + 1];
-    x[i] = pack16<kBF16>(u.x * c0.x - w.x * c0.y, u.y * c1.x - w.y * c1.y);
-    y[i] = pack16<kBF16>(w.x * c0.x + u.x * c0.y, w.y * c1.x + u.y * c1.y);
-  }
-  a = make_uint4(x[0], x[1], x[2], x[3]);
-  b = make_uint4(y[0], y[1], y[2], y[3]);
-}
-
-template <bool kBF16, int D>
-__global__ void __launch_bounds__(kPaThreads) paged_append_kernel(const AppendArgs a) {
+// A CTA takes one token.  A lane keeps one 16-byte vector of the row for all the rows it handles --
+// K's, Q's, then V's heads, 32 / (D / 8) of them per warp and step -- so its angles sit in
+// registers and a row costs a load, the products and a store; the partner of a feature in the
+// other half comes from the lane that holds it.  The first kPaHeld rows per lane are loaded before
+// anything is known about the token, so the loads from HBM run while its sequence, its page and
+// its angles are found (three dependent reads).
+//
+// HBM bound: 8698 tokens of 32 + 8 + 8 heads of 128 (214 MB) take 38 us, 5.6 TB/s, against the 33 us
+// that a copy of as many bytes takes; a few tokens take the time of the three reads, 3.1 us.
+template <bool kBF16, int D, int kPaThreads>
+__global__ void __launch_bounds__(kPaThreads, kPaThreads == kPaShort ? 5 : 9)
+    paged_append_kernel(const AppendArgs a) {
+  constexpr int kPaHeld = kPaHeldRows / kPaThreads;
   __shared__ float2 cs[64];
-  constexpr int kVecs = D / 8;
+  __shared__ int64_t s_row;
+  __shared__ int s_pos, s_page;             // s_page < 0: no slot
+  constexpr int kVecs = D / 8;              // lanes of a row
+  constexpr int kStep = kPaThreads / kVecs; // rows a step of the CTA takes
   pdl_wait();
   pdl_launch_dependents();
-  const int t = blockIdx.x, tid = threadIdx.x;
+  const int tid = threadIdx.x, lane = tid & 31;
+  const int64_t t = blockIdx.x;
   const int half = a.rope_dim >> 1, hv = half >> 3;
-  // the token's sequence: the number of sequences that end at or before it
-  int seq = 0;
-  for (int b0 = 0; b0 < a.p.batch; b0 += kPaThreads) {
-    const int b = b0 + tid;
-    seq += __syncthreads_count(b < a.p.batch && __ldg(a.p.starts + b + 1) <= t);
-  }
-  if (seq >= a.p.batch) return;  // a row past the last sequence
-  const SeqSpan s = load_span(a.p, seq);
-  const int pos = s.len - s.n + (t - s.q0);
-  const bool in = pos >= 0 && t >= s.q0 && t < s.q0 + s.n;
-  const int64_t turn = a.positions ? a.positions[t] : pos;
-  if (tid < half) {
-    const double x = static_cast<double>(turn) * static_cast<double>(a.inv_freq[tid]);
-    const double m = rint(x * 0.15915494309189535);
-    const float r = static_cast<float>(fma(-m, 6.283185307179586, x));
-    cs[tid] = make_float2(__cosf(r), __sinf(r));
-  }
-  int64_t row = -1;
-  if (in) {
-    const int entry = __ldg(a.p.table + seq * a.p.table_stride + (pos >> a.p.page_shift));
-    row = paged_row(a.p, entry, pos);
-  }
-  if (row < 0 && tid == 0) atomicOr(a.status, TDSA_STATUS_RANGE);
-  __syncthreads();
+  const int v = tid % kVecs, r0 = tid / kVecs;
+  const int hkv = a.p.kv_heads, rows = 2 * hkv + a.q_heads;
+  auto source = [&](int r) {
+    const uint16_t* p = r < hkv ? a.k + t * a.k_ts + r * a.k_hs
+                                : (r < hkv + a.q_heads ? a.q + t * a.q_ts + (r - hkv) * a.q_hs
+                                                       : a.v + t * a.v_ts +
+                                                             (r - hkv - a.q_heads) * a.v_hs);
+    return reinterpret_cast<const uint4*>(p + v * 8);
+  };
+  uint4 x[kPaHeld];
+#pragma unroll
+  for (int n = 0; n < kPaHeld; ++n)
+    if (r0 + n * kStep < rows) x[n] = *source(r0 + n * kStep);
 
-  // Work of the token: per head, the vectors of the row; with halves, a thread takes a vector
-  // of the first half and its partner, so only vectors [0, hv) and [2 hv, kVecs) lead.
-  const int lead = a.pairs ? kVecs : kVecs - hv;
-  const int total = (a.p.kv_heads + (a.q ? a.q_heads : 0)) * lead;
-  for (int i = tid; i < total; i += kPaThreads) {
-    const int h = i / lead, l = i - h * lead;
-    const bool key = h < a.p.kv_heads;
-    const uint16_t* src = key ? a.k + t * a.k_ts + h * a.k_hs
-                              : a.q + t * a.q_ts + (h - a.p.kv_heads) * a.q_hs;
-    uint16_t* dst = key ? (row < 0 ? nullptr : a.keys + row + h * a.p.head_stride)
-                        : a.q_out + t * a.qo_ts + (h - a.p.kv_heads) * a.qo_hs;
-    if (!dst) continue;
-    if (a.pairs) {
-      uint4 x = *reinterpret_cast<const uint4*>(src + l * 8);
-      if (l * 8 < a.rope_dim) x = turn_pairs<kBF16>(x, cs + l * 4);
-      *reinterpret_cast<uint4*>(dst + l * 8) = x;
-    } else if (l < hv) {
-      uint4 x = *reinterpret_cast<const uint4*>(src + l * 8);
-      uint4 y = *reinterpret_cast<const uint4*>(src + half + l * 8);
-      turn_halves<kBF16>(x, y, cs + l * 8);
-      *reinterpret_cast<uint4*>(dst + l * 8) = x;
-      *reinterpret_cast<uint4*>(dst + half + l * 8) = y;
-    } else {
-      const int v = l + hv;
-      *reinterpret_cast<uint4*>(dst + v * 8) = *reinterpret_cast<const uint4*>(src + v * 8);
+  // the token's sequence: the one whose rows hold it
+  bool found = false;
+  for (int b = tid; b < a.p.batch; b += kPaThreads) {
+    const SeqSpan s = load_span(a.p, b);
+    if (t >= s.q0 && t < s.q0 + s.n) {
+      const int pos = s.len - s.n + static_cast<int>(t - s.q0);
+      s_pos = pos;
+      s_page = pos >= 0 ? __ldg(a.p.table + b * a.p.table_stride + (pos >> a.p.page_shift)) : -1;
+      found = true;
     }
   }
-  if (row < 0) return;
-  for (int i = tid; i < a.p.kv_heads * kVecs; i += kPaThreads) {
-    const int h = i / kVecs, l = i - h * kVecs;
-    *reinterpret_cast<uint4*>(a.values + row + h * a.p.head_stride + l * 8) =
-        *reinterpret_cast<const uint4*>(a.v + t * a.v_ts + h * a.v_hs + l * 8);
+  if (!__syncthreads_or(found)) return;  // a row of no sequence
+  if (tid < half) {
+    const int64_t turn = a.positions ? a.positions[t] : s_pos;
+    const double z = static_cast<double>(turn) * static_cast<double>(a.inv_freq[tid]);
+    const double m = rint(z * 0.15915494309189535);
+    const float r = static_cast<float>(fma(-m, 6.283185307179586, z));
+    cs[tid] = make_float2(__cosf(r), __sinf(r));
   }
+  if (tid == kPaThreads - 1) {
+    s_row = paged_row(a.p, s_page, s_pos);
+    if (s_row < 0) atomicOr(a.status, TDSA_STATUS_RANGE);
+  }
+  __syncthreads();
+
+  const bool mine = a.pairs ? v * 8 < a.rope_dim : v < 2 * hv;  // this vector is turned
+  const bool upper = v >= hv;                                   // (halves) of the second half
+  const int partner = a.pairs || !mine ? lane : (upper ? lane - hv : lane + hv);
+  const int64_t row = s_row;
+  float2 c[8];  // feature e of the vector becomes x c.x + partner c.y
+  if (mine) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      c[e] = cs[a.pairs ? v * 4 + e / 2 : (upper ? v - hv : v) * 8 + e];
+      if (a.pairs ? !(e & 1) : !upper) c[e].y = -c[e].y;
+    }
+  }
+  auto finish = [&](int r, uint4 u) {
+    uint16_t* dst = r < hkv ? a.keys + row + r * a.p.head_stride
+                            : (r < hkv + a.q_heads
+                                   ? a.q_out + t * a.qo_ts + (r - hkv) * a.qo_hs
+                                   : a.values + row + (r - hkv - a.q_heads) * a.p.head_stride);
+    const bool there = row >= 0 || (r >= hkv && r < hkv + a.q_heads);
+    uint32_t w[4] = {u.x, u.y, u.z, u.w};
+    if (a.rope_dim) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const uint32_t other = __shfl_sync(0xffffffffu, w[e], partner);
+        if (mine && r < hkv + a.q_heads) {
+          const float2 f = unpack16<kBF16>(w[e]);
+          float2 o = unpack16<kBF16>(other);
+          if (a.pairs) o = make_float2(o.y, o.x);
+          w[e] = pack16<kBF16>(fmaf(f.x, c[2 * e].x, o.x * c[2 * e].y),
+                               fmaf(f.y, c[2 * e + 1].x, o.y * c[2 * e + 1].y));
+        }
+      }
+    }
+    if (there && r < rows)
+      *reinterpret_cast<uint4*>(dst + v * 8) = make_uint4(w[0], w[1], w[2], w[3]);
+  };
+#pragma unroll
+  for (int n = 0; n < kPaHeld; ++n)
+    if (n * kStep < rows) finish(r0 + n * kStep, x[n]);
+  for (int r = kPaHeld * kStep; r < rows; r += kStep) {
+    uint4 u = make_uint4(0u, 0u, 0u, 0u);
+    if (r0 + r < rows) u = *source(r0 + r);
+    finish(r0 + r, u);
+  }
+}
+
+template <int kThreads>
+auto append_kernel(bool bf16, int dim) {
+  return dim == 128 ? (bf16 ? paged_append_kernel<true, 128, kThreads>
+                            : paged_append_kernel<false, 128, kThreads>)
+                    : (bf16 ? paged_append_kernel<true, 64, kThreads>
+                            : paged_append_kernel<false, 64, kThreads>);
 }
 
 }  // namespace
@@ -152,10 +176,11 @@ int launch_paged_append(const PagedView& p, void* keys, void* values, int dtype,
   a.pairs = pairs;
   a.status = status;
   const bool bf16 = dtype == TDSA_BF16;
-  auto kern = dim == 128 ? (bf16 ? paged_append_kernel<true, 128> : paged_append_kernel<false, 128>)
-                         : (bf16 ? paged_append_kernel<true, 64> : paged_append_kernel<false, 64>);
-  TDSA_CUDA_CHECK(
-      launch_pdl(kern, dim3(static_cast<unsigned>(p.tokens)), dim3(kPaThreads), 0, stream, a));
+  // short: every CTA of the call can be resident at once
+  const bool brief = p.tokens <= 5 * device_sm_count(current_device());
+  auto kern = brief ? append_kernel<kPaShort>(bf16, dim) : append_kernel<kPaLong>(bf16, dim);
+  TDSA_CUDA_CHECK(launch_pdl(kern, dim3(static_cast<unsigned>(p.tokens)),
+                             dim3(brief ? kPaShort : kPaLong), 0, stream, a));
   TDSA_CUDA_CHECK(cudaGetLastError());
   return TDSA_OK;
 }

@@ -299,13 +299,14 @@ def test_selection_of_every_position_equals_the_attention():
 
 @pytest.mark.parametrize("dtype,dim,hq,hkv,page", [
     (BF16, 128, 8, 2, 16), (F16, 64, 3, 3, 32), (BF16, 64, 20, 4, 64), (F16, 128, 1, 1, 128)])
-@pytest.mark.parametrize("rope", [0, 16, 64])
+@pytest.mark.parametrize("rope", [0, 16, 48, 64])
 @pytest.mark.parametrize("interleaved", [False, True])
-def test_append(dtype, dim, hq, hkv, page, rope, interleaved):
+@pytest.mark.parametrize("news,lens", [([1, 0, 5, 40], [1, 3, 70, 41]),
+                                       ([400, 0, 500], [450, 3, 600])])
+def test_append(dtype, dim, hq, hkv, page, rope, interleaved, news, lens):
     from dsa_b200.paged import PagedAppender
 
-    c = Case([1, 0, 5, 40], [1, 3, 70, 41], dtype=dtype, dim=dim, hq=hq, hkv=hkv, page=page,
-             seed=40)
+    c = Case(news, lens, dtype=dtype, dim=dim, hq=hq, hkv=hkv, page=page, seed=40)
     g = torch.Generator().manual_seed(41)
     k = torch.randn(c.tokens, hkv, dim, generator=g).to(dtype)
     v = torch.randn(c.tokens, hkv, dim, generator=g).to(dtype)

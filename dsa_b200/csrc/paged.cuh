@@ -102,7 +102,7 @@ __device__ __forceinline__ int slice_owner(int64_t units, int ctas, int64_t u) {
 // Workspace of a split call: one arrival counter per CTA (an item that is split is known by
 // the CTA it starts in; zero between calls), then two partial results per CTA (slot 0: the
 // item the CTA's slice begins inside of, slot 1: the item it ends inside of).
-constexpr int kPagedCounters = 1024;
+constexpr int kPagedCounters = TDSA_PAGED_COUNTER_BYTES / 4;
 struct PagedPartials {
   uint32_t* counters;
   float2* ml;   // [slot][rows]: running maximum (log2 units), sum
@@ -119,6 +119,19 @@ inline PagedPartials paged_partials(void* ws, int ctas, int rows) {
   p.ml = reinterpret_cast<float2*>(p.counters + kPagedCounters);
   p.o = reinterpret_cast<float*>(p.ml + static_cast<size_t>(ctas) * 2 * rows);
   return p;
+}
+
+// One more part of a split item has arrived, whose stores (the whole block's, behind a barrier)
+// are visible to whoever sees the count; true for the last of n, which then sees all the others'
+// and leaves the counter at zero.
+__device__ __forceinline__ bool paged_arrive(uint32_t* counter, uint32_t n) {
+  uint32_t old;
+  asm volatile("atom.acq_rel.gpu.global.add.u32 %0, [%1], 1;"
+               : "=r"(old)
+               : "l"(counter)
+               : "memory");
+  if (old == n - 1) *counter = 0u;
+  return old == n - 1;
 }
 
 struct PagedQuery {
@@ -286,6 +299,64 @@ __device__ __forceinline__ PagedSlice paged_find_slice(const PagedView& p, const
       s_found[0] = b;
       s_found[1] = rt;
       const int64_t head = quotient(rest, n);
+      s_found[2] = static_cast<int>(head);
+      s_found[3] = static_cast<int>(rest - head * n);
+      return false;
+    });
+  }
+  __syncthreads();
+  r.seq = s_found[0];
+  r.row_tile = s_found[1];
+  r.head = s_found[2];
+  r.off = s_found[3];
+  return r;
+}
+
+// The same for calls whose sequences have a row tile or two each (the decode step): a thread
+// counts its sequences' units itself, which saves a pass over the block.
+template <int kThreads, int kRows, int kUnit>
+__device__ __forceinline__ PagedSlice paged_find_slice_few(const PagedView& p,
+                                                           const PagedQuery& q, int ctas,
+                                                           int cta, int64_t* s_scan,
+                                                           int* s_found) {
+  const int tid = threadIdx.x;
+  const int chunk = (p.batch + kThreads - 1) / kThreads;
+  const int b0 = min(p.batch, tid * chunk), b1 = min(p.batch, b0 + chunk);
+  // calls f(sequence, row tile, units) until it returns false
+  auto each = [&](auto&& f) {
+    for (int b = b0; b < b1; ++b) {
+      const SeqSpan s = load_span(p, b);
+      PagedItem x;
+      for (int t = 0; t * kRows < s.n * q.group; ++t) {
+        paged_range_item<kRows, kUnit>(q, s, t, x);
+        if (!f(b, t, x.u1 - x.u0)) return;
+      }
+    }
+  };
+  int64_t mine = 0, all;
+  each([&](int, int, int n) {
+    mine += n;
+    return true;
+  });
+  int64_t at = block_scan<kThreads>(mine, s_scan, all) * p.kv_heads;
+  PagedSlice r;
+  r.units = all * p.kv_heads;
+  r.ctas = static_cast<int>(min(static_cast<int64_t>(ctas), r.units));
+  r.begin = r.end = 0;
+  r.seq = r.row_tile = r.head = r.off = 0;
+  if (cta >= r.ctas) return r;
+  r.begin = slice_begin(r.units, r.ctas, cta);
+  r.end = slice_begin(r.units, r.ctas, cta + 1);
+  if (r.begin >= at && r.begin < at + mine * p.kv_heads) {
+    each([&](int b, int t, int n) {
+      const int64_t w = static_cast<int64_t>(n) * p.kv_heads;
+      if (r.begin >= at + w) {
+        at += w;
+        return true;
+      }
+      const int64_t rest = r.begin - at, head = quotient(rest, n);
+      s_found[0] = b;
+      s_found[1] = t;
       s_found[2] = static_cast<int>(head);
       s_found[3] = static_cast<int>(rest - head * n);
       return false;

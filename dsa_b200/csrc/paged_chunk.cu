@@ -684,15 +684,9 @@ __global__ void __launch_bounds__(kPcThreads, 1)
                             __uint_as_float(o[4 * x + 2]), __uint_as_float(o[4 * x + 3]));
         }
         if (!meet()) break;
-        if (row == 0) {
-          __threadfence();
-          uint32_t* counter = a.part.counters + 2 * c_first + t;
-          const uint32_t n = static_cast<uint32_t>(c_last - c_first + 1);
-          const uint32_t old = atomicAdd(counter, 1u);
-          if (old == n - 1) *counter = 0u;
-          s_last[t] = old == n - 1;
-          __threadfence();
-        }
+        if (row == 0)
+          s_last[t] = paged_arrive(a.part.counters + 2 * c_first + t,
+                                   static_cast<uint32_t>(c_last - c_first + 1));
         if (!meet()) break;
         write = s_last[t] != 0;
       }

@@ -101,16 +101,23 @@ __device__ __forceinline__ void cp_async_wait() {
   asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
 }
 
-template <bool kBF16, int D, int MT, bool kSel>
+// kSolo (selected attention): a warp takes items of its own instead of a quarter of the CTA's, so
+// that nothing waits for the other warps where items are short and many.
+template <bool kBF16, int D, int MT, bool kSel, bool kSolo>
 __global__ void __launch_bounds__(kPrThreads, 2) paged_rows_kernel(const RowsArgs a) {
   using C = RowsCfg<D, MT>;
+  static_assert(kSel || !kSolo, "");
+  constexpr int kTeam = kSolo ? 1 : kPrWarps;      // warps that share an item
+  constexpr int kUnitTiles = kPrWarps / kTeam;     // tiles of a unit per warp
   constexpr int kRows = C::kRows, kStages = C::kStages;
   constexpr int kKs = D / 16;   // 16-wide steps of the head dimension
   constexpr int kNt = D / 8;    // 8-wide output tiles
   constexpr int kLanesPerRow = D / 8;
   constexpr int kRowsPerCopy = 32 / kLanesPerRow;
   extern __shared__ __align__(128) uint8_t smem[];
-  float2* s_ml = reinterpret_cast<float2*>(smem + C::kRing);  // [warp][row]
+  // [warp of the team][row]
+  float2* s_ml =
+      reinterpret_cast<float2*>(smem + C::kRing) + (kSolo ? (threadIdx.x >> 5) * kRows : 0);
   int* s_meta = reinterpret_cast<int*>(smem + C::kRing + C::kMl);
   int64_t* s_scan = reinterpret_cast<int64_t*>(s_meta + 8);   // [4] warp totals
   // [warp][stage]: bit r is set when row r of the stage's tile holds a key of the cache
@@ -120,8 +127,15 @@ __global__ void __launch_bounds__(kPrThreads, 2) paged_rows_kernel(const RowsArg
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int quad = lane >> 2, ql = lane & 3;
   const int g = a.q.group, hkv = a.p.kv_heads;
-  int ctas = gridDim.x;  // CTAs that get work: no more than there are units
-  const int cta = blockIdx.x;
+  // the team, of so many; as many as there are units get work
+  int ctas = gridDim.x * (kPrWarps / kTeam);
+  const int cta = kSolo ? blockIdx.x * kPrWarps + warp : blockIdx.x;
+  const int share = kSolo ? 0 : warp;         // of the team's warps
+  const int member = kSolo ? lane : tid;      // of the team's threads
+  auto team_sync = [&]() {
+    if (kSolo) __syncwarp();
+    else __syncthreads();
+  };
   pdl_wait();
   pdl_launch_dependents();
 
@@ -132,8 +146,8 @@ __global__ void __launch_bounds__(kPrThreads, 2) paged_rows_kernel(const RowsArg
   int rt = 0;          // row tile of the current item
   int off;             // unit of the item the slice begins at
   SeqSpan span;
-  const int sel_units = kSel ? max(1, (a.q.topk + kPrUnit - 1) / kPrUnit) : 0;
-  const int sel_rts = kSel ? (g + kRows - 1) / kRows : 0;
+  const int sel_units = kSel ? max(1, (a.q.topk + kPrUnit - 1) / kPrUnit) : 1;
+  const int sel_rts = kSel ? (g + kRows - 1) / kRows : 1;
   int64_t sel_item = 0;
   // selected attention: item i is (token, row tile, head); its sequence comes from the starts
   auto sel_load = [&](int64_t i) {
@@ -168,8 +182,8 @@ __global__ void __launch_bounds__(kPrThreads, 2) paged_rows_kernel(const RowsArg
     off = static_cast<int>(u_begin - sel_item * sel_units);
     sel_load(sel_item);
   } else {
-    const PagedSlice sl = paged_find_slice<kPrThreads, kRows, kPrUnit>(
-        a.p, a.q, ctas, cta, s_scan, reinterpret_cast<int*>(smem), s_meta);
+    const PagedSlice sl = paged_find_slice_few<kPrThreads, kRows, kPrUnit>(a.p, a.q, ctas,
+                                                                           cta, s_scan, s_meta);
     units = sl.units;
     ctas = sl.ctas;
     if (cta >= ctas) return;
@@ -221,12 +235,16 @@ __global__ void __launch_bounds__(kPrThreads, 2) paged_rows_kernel(const RowsArg
     const int32_t* table = a.p.table + it.seq * a.p.table_stride;
     const int cap = a.p.max_pages << a.p.page_shift;
     const int64_t head_off = it.head * a.p.head_stride;
+    const int n_tiles = seg * kUnitTiles;
+    auto tile_base = [&](int i) {  // first key of the warp's tile i
+      return kSolo ? unit0 * kPrUnit + i * kPrTile : (unit0 + i) * kPrUnit + warp * kPrTile;
+    };
     auto key_slot = [&](int pr) {  // index of lane l's key in the item's key list
-      return (unit0 + 2 * pr + (lane >> 4)) * kPrUnit + warp * kPrTile + (lane & 15);
+      return tile_base(2 * pr + (lane >> 4)) + (lane & 15);
     };
     auto load_raw = [&](int pr) -> int {
       const int s = key_slot(pr);
-      if (2 * pr + (lane >> 4) >= seg) return -1;
+      if (2 * pr + (lane >> 4) >= n_tiles) return -1;
       if (!kSel) return s >= it.k0 && s < it.k1 ? s : -1;
       if (s >= it.k1) return -1;
       const int64_t at = static_cast<int64_t>(it.tok0) * a.q.idx_stride + s;
@@ -261,7 +279,7 @@ __global__ void __launch_bounds__(kPrThreads, 2) paged_rows_kernel(const RowsArg
 
     // issue the copies of tile i of the segment (one group, empty past the end)
     auto issue = [&](int i) {
-      if (i < seg) {
+      if (i < n_tiles) {
         const int pr = i >> 1;
         if (pr != load_pair) {
           load_pair = pr;
@@ -298,10 +316,11 @@ __global__ void __launch_bounds__(kPrThreads, 2) paged_rows_kernel(const RowsArg
     for (int m = 0; m < MT; ++m) {
       const int ra = it.r0 + m * 16 + quad, rb = ra + 8;
       const int lim = it.r0 + it.rows;
-      const uint16_t* pa = a.q.q + static_cast<int64_t>(it.tok0 + ra / g) * a.q.q_ts +
-                           (it.head * g + ra % g) * a.q.q_hs + ql * 2;
-      const uint16_t* pb = a.q.q + static_cast<int64_t>(it.tok0 + rb / g) * a.q.q_ts +
-                           (it.head * g + rb % g) * a.q.q_hs + ql * 2;
+      const int ta = kSel ? 0 : ra / g, tb = kSel ? 0 : rb / g;
+      const uint16_t* pa = a.q.q + static_cast<int64_t>(it.tok0 + ta) * a.q.q_ts +
+                           (it.head * g + ra - ta * g) * a.q.q_hs + ql * 2;
+      const uint16_t* pb = a.q.q + static_cast<int64_t>(it.tok0 + tb) * a.q.q_ts +
+                           (it.head * g + rb - tb * g) * a.q.q_hs + ql * 2;
 #pragma unroll
       for (int k = 0; k < kKs; ++k) {
         qf[m][k][0] = ra < lim ? *reinterpret_cast<const uint32_t*>(pa + k * 16) : 0u;
@@ -322,13 +341,13 @@ __global__ void __launch_bounds__(kPrThreads, 2) paged_rows_kernel(const RowsArg
       mx[m][0] = mx[m][1] = -INFINITY;
       sum[m][0] = sum[m][1] = 0.f;
     }
-    for (int i = 0; i < seg; ++i) {
+    for (int i = 0; i < n_tiles; ++i) {
       issue(i + kStages - 1);
       cp_async_wait<kStages - 1>();
       __syncwarp();
       const uint32_t st = ring_u + (i % kStages) * C::kStageBytes;
       const uint32_t vmask = s_valid[i % kStages];
-      const int base = (unit0 + i) * kPrUnit + warp * kPrTile;
+      const int base = tile_base(i);
       float s[MT][2][4];
 #pragma unroll
       for (int m = 0; m < MT; ++m)
@@ -487,7 +506,7 @@ __global__ void __launch_bounds__(kPrThreads, 2) paged_rows_kernel(const RowsArg
         t += __shfl_xor_sync(0xffffffffu, t, 1);
         t += __shfl_xor_sync(0xffffffffu, t, 2);
         const int r = m * 16 + quad + 8 * e;
-        if (ql == 0) s_ml[warp * kRows + r] = make_float2(mx[m][e], t);
+        if (ql == 0) s_ml[share * kRows + r] = make_float2(mx[m][e], t);
         if (r < it.rows) {
 #pragma unroll
           for (int n = 0; n < kNt; ++n)
@@ -495,111 +514,151 @@ __global__ void __launch_bounds__(kPrThreads, 2) paged_rows_kernel(const RowsArg
                 make_float2(o[m][n][2 * e], o[m][n][2 * e + 1]);
         }
       }
-    __syncthreads();
+    team_sync();
     const bool entire = seg == n_units;
     const int64_t item_u0 = u - off;  // the item's first unit in the call's list
     const int c_first = slice_owner(units, ctas, item_u0);
     const int c_last = slice_owner(units, ctas, item_u0 + n_units - 1);
     const int slot = 2 * cta + (cta == c_first ? 1 : 0);
-    constexpr int kV = D / 4;            // float4 columns
-    constexpr int kG = kPrThreads / kV;  // row groups
-    const int col = tid % kV, rg = tid / kV;
-    auto store_row = [&](int r, float m, float l, float4 v) {
-      const int row = it.r0 + r;
-      const int64_t t = it.tok0 + row / g;
-      const int h = it.head * g + row % g;
-      const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);  // NaN stays NaN
-      uint2 w;
-      w.x = pack16<kBF16>(v.x * inv, v.y * inv);
-      w.y = pack16<kBF16>(v.z * inv, v.w * inv);
-      if (l == 0.f) w = make_uint2(0u, 0u);
-      *reinterpret_cast<uint2*>(a.q.out + t * a.q.o_ts + h * a.q.o_hs + col * 4) = w;
-      if (a.q.lse && col == 0)
-        a.q.lse[t * a.q.heads + h] = l == 0.f ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f;
-    };
-    for (int r = rg; r < it.rows; r += kG) {
-      float m = -INFINITY;
+    constexpr int kV = D / 4;              // float4 columns
+    constexpr int kG = kTeam * 32 / kV;    // row groups
+    const int col = member % kV, rg = member / kV;
+    // adds up the team's results in shared memory and writes rows of the output, or a partial
+    auto combine = [&](bool to_out) {
+      for (int r = rg; r < it.rows; r += kG) {
+        float m = -INFINITY;
 #pragma unroll
-      for (int w = 0; w < kPrWarps; ++w) m = fmaxf(m, s_ml[w * kRows + r].x);
-      const float ref = m == -INFINITY ? 0.f : m;
-      float l = 0.f;
-      float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (int w = 0; w < kTeam; ++w) m = fmaxf(m, s_ml[w * kRows + r].x);
+        const float ref = m == -INFINITY ? 0.f : m;
+        float l = 0.f;
+        float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-      for (int w = 0; w < kPrWarps; ++w) {
-        const float2 ml = s_ml[w * kRows + r];
-        const float f = exp2_approx(ml.x - ref);
-        const float4 x = *reinterpret_cast<const float4*>(
-            reinterpret_cast<const float*>(smem + w * C::kWarpBytes) + r * D + col * 4);
-        if (ml.x != -INFINITY) {
-          l += ml.y * f;
-          v.x += x.x * f, v.y += x.y * f, v.z += x.z * f, v.w += x.w * f;
-        } else {
-          l += ml.y;  // zero, or NaN when a score was NaN
-        }
-      }
-      if (entire) {
-        store_row(r, m, l, v);
-      } else {
-        if (col == 0) a.part.ml[static_cast<int64_t>(slot) * kRows + r] = make_float2(m, l);
-        *reinterpret_cast<float4*>(a.part.o + (static_cast<int64_t>(slot) * kRows + r) * D +
-                                   col * 4) = v;
-      }
-    }
-    if (!entire) {
-      __syncthreads();
-      if (tid == 0) {
-        __threadfence();
-        const uint32_t n = static_cast<uint32_t>(c_last - c_first + 1);
-        const uint32_t old = atomicAdd(a.part.counters + c_first, 1u);
-        s_meta[4] = old == n - 1;
-        if (old == n - 1) a.part.counters[c_first] = 0u;
-        __threadfence();
-      }
-      __syncthreads();
-      if (s_meta[4]) {
-        // the last to arrive: partials of CTAs c_first .. c_last, in that order.  First every
-        // row's maximum, sum and the partials' factors (a warp per row, a lane per partial),
-        // then the rows themselves.
-        const int parts = c_last - c_first + 1;
-        float* fac = reinterpret_cast<float*>(smem);  // [row][parts]; the ring is idle
-        auto slot_of = [&](int p) { return 2 * static_cast<int64_t>(c_first + p) + (p == 0); };
-        for (int r = warp; r < it.rows; r += kPrWarps) {
-          float m = -INFINITY, l = 0.f;
-          for (int p = lane; p < parts; p += 32)
-            m = fmaxf(m, __ldcg(&a.part.ml[slot_of(p) * kRows + r]).x);
-#pragma unroll
-          for (int o2 = 16; o2 > 0; o2 >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o2));
-          const float ref = m == -INFINITY ? 0.f : m;
-          for (int p = lane; p < parts; p += 32) {
-            const float2 ml = __ldcg(&a.part.ml[slot_of(p) * kRows + r]);
-            const float f = exp2_approx(ml.x - ref);
-            fac[r * parts + p] = f;
+        for (int w = 0; w < kTeam; ++w) {
+          const float2 ml = s_ml[w * kRows + r];
+          const float f = exp2_approx(ml.x - ref);
+          const uint8_t* from = kSolo ? ring : smem + w * C::kWarpBytes;
+          const float4 x = *reinterpret_cast<const float4*>(
+              reinterpret_cast<const float*>(from) + r * D + col * 4);
+          if (ml.x != -INFINITY) {
             l += ml.y * f;
+            v.x += x.x * f, v.y += x.y * f, v.z += x.z * f, v.w += x.w * f;
+          } else {
+            l += ml.y;  // zero, or NaN when a score was NaN
+          }
+        }
+        if (to_out) {
+          const int row = it.r0 + r, tk = kSel ? 0 : row / g;
+          const int64_t t = it.tok0 + tk;
+          const int h = it.head * g + row - tk * g;
+          const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);  // NaN stays NaN
+          uint2 w;
+          w.x = pack16<kBF16>(v.x * inv, v.y * inv);
+          w.y = pack16<kBF16>(v.z * inv, v.w * inv);
+          if (l == 0.f) w = make_uint2(0u, 0u);
+          *reinterpret_cast<uint2*>(a.q.out + t * a.q.o_ts + h * a.q.o_hs + col * 4) = w;
+          if (a.q.lse && col == 0)
+            a.q.lse[t * a.q.heads + h] =
+                l == 0.f ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f;
+        } else {
+          if (col == 0) a.part.ml[static_cast<int64_t>(slot) * kRows + r] = make_float2(m, l);
+          *reinterpret_cast<float4*>(a.part.o + (static_cast<int64_t>(slot) * kRows + r) * D +
+                                     col * 4) = v;
+        }
+      }
+    };
+    combine(entire);
+    if (!entire) {
+      team_sync();
+      bool last = false;
+      if (member == 0)
+        last = paged_arrive(a.part.counters + c_first, static_cast<uint32_t>(c_last - c_first + 1));
+      if (kSolo) {
+        last = __shfl_sync(0xffffffffu, last, 0);
+      } else {
+        if (member == 0) s_meta[4] = last;
+        __syncthreads();
+        last = s_meta[4] != 0;
+      }
+      if (last) {
+        // The last to arrive adds the partials of teams c_first .. c_last up, four rows at a
+        // time: a warp takes every kTeam-th partial where there are many, else every kTeam-th
+        // group of rows; then the warps' sums meet as the segment's did.
+        const int parts = c_last - c_first + 1;
+        const bool by_part = parts >= 2 * kTeam;
+        auto slot_of = [&](int p) { return 2 * static_cast<int64_t>(c_first + p) + (p == 0); };
+        const int first = by_part ? share : 0, step = by_part ? kTeam : 1;
+        const int count = (parts - first + step - 1) / step;
+        for (int r = lane; r < kRows; r += 32) s_ml[share * kRows + r] = make_float2(-INFINITY, 0.f);
+        __syncwarp();
+        for (int r0 = by_part ? 0 : share * 4; r0 < it.rows; r0 += by_part ? 4 : 4 * kTeam) {
+          float m[4], l[4];
+#pragma unroll
+          for (int x = 0; x < 4; ++x) m[x] = -INFINITY, l[x] = 0.f;
+          float4 v[4];
+#pragma unroll
+          for (int x = 0; x < 4; ++x) v[x] = make_float4(0.f, 0.f, 0.f, 0.f);
+          for (int j0 = 0; j0 < count; j0 += 32) {
+            const int p = first + (j0 + lane) * step;
+            const bool in = j0 + lane < count;
+            float2 ml[4];
+#pragma unroll
+            for (int x = 0; x < 4; ++x)
+              ml[x] = in && r0 + x < it.rows ? __ldcg(&a.part.ml[slot_of(p) * kRows + r0 + x])
+                                             : make_float2(-INFINITY, 0.f);
+            float f[4];
+#pragma unroll
+            for (int x = 0; x < 4; ++x) {
+              float now = ml[x].x;
+#pragma unroll
+              for (int o2 = 16; o2 > 0; o2 >>= 1)
+                now = fmaxf(now, __shfl_xor_sync(0xffffffffu, now, o2));
+              now = fmaxf(now, m[x]);
+              const float ref = now == -INFINITY ? 0.f : now;
+              const float keep = exp2_approx(m[x] - ref);
+              f[x] = exp2_approx(ml[x].x - ref);
+              l[x] = l[x] * keep + ml[x].y * f[x];  // this lane's partials
+              v[x].x *= keep, v[x].y *= keep, v[x].z *= keep, v[x].w *= keep;
+              m[x] = now;
+            }
+            const int n = min(32, count - j0);
+            const int lc = lane % kV;
+#pragma unroll 4
+            for (int j = 0; j < n; ++j) {
+              const int64_t sl_j = slot_of(first + (j0 + j) * step) * kRows;
+#pragma unroll
+              for (int x = 0; x < 4; ++x) {
+                const float fx = __shfl_sync(0xffffffffu, f[x], j);
+                if (r0 + x < it.rows) {
+                  const float4 w = __ldcg(
+                      reinterpret_cast<const float4*>(a.part.o + (sl_j + r0 + x) * D) + lc);
+                  v[x].x += w.x * fx, v[x].y += w.y * fx;
+                  v[x].z += w.z * fx, v[x].w += w.w * fx;
+                }
+              }
+            }
           }
 #pragma unroll
-          for (int o2 = 16; o2 > 0; o2 >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o2);
-          if (lane == 0) s_ml[r] = make_float2(m, l);
-        }
-        __syncthreads();
-        for (int r = rg; r < it.rows; r += kG) {
-          const float2 ml = s_ml[r];
-          float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 8
-          for (int p = 0; p < parts; ++p) {
-            const float4 x = __ldcg(
-                reinterpret_cast<const float4*>(a.part.o + (slot_of(p) * kRows + r) * D) + col);
-            const float f = fac[r * parts + p];
-            v.x += x.x * f, v.y += x.y * f, v.z += x.z * f, v.w += x.w * f;
+          for (int x = 0; x < 4; ++x) {
+            float t = l[x];
+#pragma unroll
+            for (int o2 = 16; o2 > 0; o2 >>= 1) t += __shfl_xor_sync(0xffffffffu, t, o2);
+            if (r0 + x < it.rows) {
+              if (lane == 0) s_ml[share * kRows + r0 + x] = make_float2(m[x], t);
+              if (lane < kV)
+                *reinterpret_cast<float4*>(reinterpret_cast<float*>(ring) + (r0 + x) * D +
+                                           lane * 4) = v[x];
+            }
           }
-          store_row(r, ml.x, ml.y, v);
         }
+        team_sync();
+        combine(true);
       }
     }
 
     // ------------------------------------------------------------ the next item
     u += seg;
     if (u >= u_end) break;
-    __syncthreads();  // the ring and s_ml are free again
+    team_sync();  // the ring and s_ml are free again
     off = 0;
     if (kSel) {
       sel_load(++sel_item);
@@ -610,11 +669,11 @@ __global__ void __launch_bounds__(kPrThreads, 2) paged_rows_kernel(const RowsArg
   if (__any_sync(0xffffffffu, bad) && lane == 0) atomicOr(a.status, TDSA_STATUS_RANGE);
 }
 
-template <bool kBF16, int D, int MT, bool kSel>
+template <bool kBF16, int D, int MT, bool kSel, bool kSolo>
 int launch_rows_t(RowsArgs a, int ctas, void* ws, cudaStream_t stream) {
   using C = RowsCfg<D, MT>;
-  a.part = paged_partials(ws, ctas, C::kRows);
-  auto kern = paged_rows_kernel<kBF16, D, MT, kSel>;
+  a.part = paged_partials(ws, ctas * (kSolo ? kPrWarps : 1), C::kRows);
+  auto kern = paged_rows_kernel<kBF16, D, MT, kSel, kSolo>;
   TDSA_CUDA_CHECK(ensure_dynamic_smem(reinterpret_cast<const void*>(kern), C::kSmem));
   TDSA_CUDA_CHECK(launch_pdl(kern, dim3(static_cast<unsigned>(ctas)), dim3(kPrThreads), C::kSmem,
                              stream, a));
@@ -622,20 +681,25 @@ int launch_rows_t(RowsArgs a, int ctas, void* ws, cudaStream_t stream) {
   return TDSA_OK;
 }
 
-template <bool kBF16, int D>
-int launch_rows_d(const RowsArgs& a, int mt, bool sel, int ctas, void* ws, cudaStream_t stream) {
-  if (sel)
-    return mt == 1 ? launch_rows_t<kBF16, D, 1, true>(a, ctas, ws, stream)
-                   : launch_rows_t<kBF16, D, 2, true>(a, ctas, ws, stream);
-  return mt == 1 ? launch_rows_t<kBF16, D, 1, false>(a, ctas, ws, stream)
-                 : launch_rows_t<kBF16, D, 2, false>(a, ctas, ws, stream);
+template <bool kBF16, int D, int MT>
+int launch_rows_d(const RowsArgs& a, int ctas, void* ws, cudaStream_t stream) {
+  if (!a.q.idx) return launch_rows_t<kBF16, D, MT, false, false>(a, ctas, ws, stream);
+  // a warp per item once every warp has one: nothing then waits for the CTA's other warps
+  // (683 tokens x 2 heads x 512 positions: @@ us against @@)
+  const int64_t items = static_cast<int64_t>(a.p.tokens) * a.p.kv_heads *
+                        ((a.q.group + 16 * MT - 1) / (16 * MT));
+  if (items >= static_cast<int64_t>(ctas) * kPrWarps)
+    return launch_rows_t<kBF16, D, MT, true, true>(a, ctas, ws, stream);
+  return launch_rows_t<kBF16, D, MT, true, false>(a, ctas, ws, stream);
 }
 
 int rows_ctas() { return 2 * device_sm_count(current_device()); }
 
 }  // namespace
 
-size_t paged_rows_workspace_bytes(int dim) { return paged_partial_bytes(rows_ctas(), 32, dim); }
+size_t paged_rows_workspace_bytes(int dim) {
+  return paged_partial_bytes(rows_ctas() * kPrWarps, 32, dim);
+}
 
 int launch_paged_rows(const PagedView& p, const PagedQuery& q, int dtype, int dim, int rows,
                       void* ws, int* status, cudaStream_t stream) {
@@ -643,14 +707,20 @@ int launch_paged_rows(const PagedView& p, const PagedQuery& q, int dtype, int di
   a.p = p;
   a.q = q;
   a.status = status;
-  const int mt = rows <= 16 ? 1 : 2;
-  const bool sel = q.idx != nullptr;
   const int ctas = rows_ctas();
-  if (dtype == TDSA_BF16)
-    return dim == 128 ? launch_rows_d<true, 128>(a, mt, sel, ctas, ws, stream)
-                      : launch_rows_d<true, 64>(a, mt, sel, ctas, ws, stream);
-  return dim == 128 ? launch_rows_d<false, 128>(a, mt, sel, ctas, ws, stream)
-                    : launch_rows_d<false, 64>(a, mt, sel, ctas, ws, stream);
+  const bool narrow = rows <= 16;
+  if (dtype == TDSA_BF16) {
+    if (dim == 128)
+      return narrow ? launch_rows_d<true, 128, 1>(a, ctas, ws, stream)
+                    : launch_rows_d<true, 128, 2>(a, ctas, ws, stream);
+    return narrow ? launch_rows_d<true, 64, 1>(a, ctas, ws, stream)
+                  : launch_rows_d<true, 64, 2>(a, ctas, ws, stream);
+  }
+  if (dim == 128)
+    return narrow ? launch_rows_d<false, 128, 1>(a, ctas, ws, stream)
+                  : launch_rows_d<false, 128, 2>(a, ctas, ws, stream);
+  return narrow ? launch_rows_d<false, 64, 1>(a, ctas, ws, stream)
+                : launch_rows_d<false, 64, 2>(a, ctas, ws, stream);
 }
 
 }  // namespace tdsa

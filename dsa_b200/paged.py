@@ -143,7 +143,7 @@ _WORKSPACES: dict[tuple[int, int, int], tuple[torch.Tensor, int, int]] = {}
 
 def paged_workspace(device: torch.device, head_dim: int,
                     stream: int | None = None) -> tuple[torch.Tensor, int, int]:
-    """Zeroed scratch of the attention calls -> (buffer, address, bytes).  Outside CUDA-graph
+    """Scratch of the attention calls, its counters zeroed -> (buffer, address, bytes).  Outside CUDA-graph
     capture one buffer per (device, stream, head_dim) is kept: calls on one stream run in order
     and each leaves it ready for the next.  During a capture a fresh one is returned, which the
     graph keeps."""
@@ -155,7 +155,8 @@ def paged_workspace(device: torch.device, head_dim: int,
     if ws is None or capturing:
         with torch.cuda.device(device):
             nbytes = capi.lib().tdsa_paged_workspace_bytes(head_dim)
-        buffer = torch.zeros(max(nbytes, 1), device=device, dtype=torch.uint8)
+        buffer = torch.empty(max(nbytes, 1), device=device, dtype=torch.uint8)
+        buffer[:capi.TDSA_PAGED_COUNTER_BYTES].zero_()
         ws = (buffer, buffer.data_ptr(), nbytes)
         if not capturing:
             _WORKSPACES[key] = ws

@@ -638,6 +638,8 @@ typedef struct tdsa_token_rows {
   int64_t head_stride;
 } tdsa_token_rows;
 
+#define TDSA_PAGED_COUNTER_BYTES 8192
+
 /*
  * Writes the keys (rotated) and values of every new token into its slot of the cache and, when
  * q is not NULL, its rotated queries into q_out (which may be q).  The rotation turns the
@@ -663,8 +665,9 @@ int tdsa_paged_append(const tdsa_paged_cache* cache, const tdsa_paged_batch* bat
  *   not wanted).
  * A token that sees no key gets out 0 and lse -inf.  out must not overlap q.  float32 scores, maxima and sums; the
  * softmax weights are rounded to the cache's type for the product with V.  scale > 0.
- * workspace: tdsa_paged_workspace_bytes bytes, 256-byte aligned, zero before its first use;
- * every call leaves it ready for the next one on the same stream.
+ * workspace: tdsa_paged_workspace_bytes bytes, 256-byte aligned, its first
+ * TDSA_PAGED_COUNTER_BYTES zero before its first use; every call leaves it ready for the next
+ * one on the same stream.
  */
 int tdsa_paged_attention(const tdsa_paged_cache* cache, const tdsa_paged_batch* batch,
                          const tdsa_token_rows* q, int q_heads, float scale, int window,

@@ -43,12 +43,16 @@ struct RowsArgs {
   int* status;
 };
 
-template <int D, int MT>
+template <int D, int MT, bool kSel>
 struct RowsCfg {
   static constexpr int kRowBytes = D * 2;
   static constexpr int kTileBytes = kPrTile * kRowBytes;       // K or V tile
   static constexpr int kStageBytes = 2 * kTileBytes;
-  static constexpr int kStages = D == 128 ? 3 : 6;
+  // CTAs per SM, and tiles of a warp's ring (96 KB of ring per SM and more): selected keys of 64
+  // features gain from more warps (683 tokens x 2 heads x 512: 38 us with 4 CTAs, 44 with 2), runs
+  // of pages do not (11 sequences x 16 heads x 16461: 150 us against 141).
+  static constexpr int kCtas = D == 64 && MT == 1 && kSel ? 4 : 2;
+  static constexpr int kStages = D == 128 || kCtas == 4 ? 3 : 6;
   static constexpr int kWarpBytes = kStages * kStageBytes;
   static constexpr int kRows = 16 * MT;
   static constexpr int kMergeO = kRows * D * 4;                // a warp's output, float32
@@ -104,8 +108,9 @@ __device__ __forceinline__ void cp_async_wait() {
 // kSolo (selected attention): a warp takes items of its own instead of a quarter of the CTA's, so
 // that nothing waits for the other warps where items are short and many.
 template <bool kBF16, int D, int MT, bool kSel, bool kSolo>
-__global__ void __launch_bounds__(kPrThreads, 2) paged_rows_kernel(const RowsArgs a) {
-  using C = RowsCfg<D, MT>;
+__global__ void __launch_bounds__(kPrThreads, RowsCfg<D, MT, kSel>::kCtas)
+    paged_rows_kernel(const RowsArgs a) {
+  using C = RowsCfg<D, MT, kSel>;
   static_assert(kSel || !kSolo, "");
   constexpr int kTeam = kSolo ? 1 : kPrWarps;      // warps that share an item
   constexpr int kUnitTiles = kPrWarps / kTeam;     // tiles of a unit per warp
@@ -148,29 +153,22 @@ __global__ void __launch_bounds__(kPrThreads, 2) paged_rows_kernel(const RowsArg
   SeqSpan span;
   const int sel_units = kSel ? max(1, (a.q.topk + kPrUnit - 1) / kPrUnit) : 1;
   const int sel_rts = kSel ? (g + kRows - 1) / kRows : 1;
-  int64_t sel_item = 0;
-  // selected attention: item i is (token, row tile, head); its sequence comes from the starts
-  auto sel_load = [&](int64_t i) {
-    const int h = static_cast<int>(i % hkv);
-    const int64_t tr = i / hkv;
-    const int t = static_cast<int>(tr / sel_rts);
-    rt = static_cast<int>(tr - static_cast<int64_t>(t) * sel_rts);
+  // selected attention: items are (token, row tile, head); a token's sequence comes from the starts
+  auto sel_token = [&](int t) {
     int c = 0;
     for (int b = lane; b < a.p.batch; b += 32) c += __ldg(a.p.starts + b + 1) <= t;
     c = __reduce_add_sync(0xffffffffu, c);
     it.seq = min(c, a.p.batch - 1);
-    it.head = h;
     span = load_span(a.p, it.seq);
     it.tok0 = t;
-    it.r0 = rt * kRows;
-    it.rows = min(kRows, g - it.r0);
-    it.pos0 = 0;
-    it.k0 = 0;
-    it.k1 = a.q.topk;
-    it.u0 = 0;
-    it.u1 = sel_units;
     // a row before the first sequence or past the last one: nothing is read or written
-    if (c >= a.p.batch || t < span.q0) it.k1 = it.rows = 0;
+    it.k1 = c >= a.p.batch || t < span.q0 ? 0 : a.q.topk;
+    it.pos0 = it.k0 = it.u0 = 0;
+    it.u1 = sel_units;
+  };
+  auto sel_rows = [&]() {
+    it.r0 = rt * kRows;
+    it.rows = it.k1 ? min(kRows, g - it.r0) : 0;
   };
   if (kSel) {
     units = static_cast<int64_t>(a.p.tokens) * sel_rts * hkv * sel_units;
@@ -178,9 +176,14 @@ __global__ void __launch_bounds__(kPrThreads, 2) paged_rows_kernel(const RowsArg
     if (cta >= ctas) return;
     u_begin = slice_begin(units, ctas, cta);
     u_end = slice_begin(units, ctas, cta + 1);
-    sel_item = u_begin / sel_units;
-    off = static_cast<int>(u_begin - sel_item * sel_units);
-    sel_load(sel_item);
+    const int64_t item = quotient(u_begin, sel_units);
+    off = static_cast<int>(u_begin - item * sel_units);
+    const int64_t tr = quotient(item, hkv);  // token and row tile
+    const int t = static_cast<int>(quotient(tr, sel_rts));
+    it.head = static_cast<int>(item - tr * hkv);
+    rt = static_cast<int>(tr - static_cast<int64_t>(t) * sel_rts);
+    sel_token(t);
+    sel_rows();
   } else {
     const PagedSlice sl = paged_find_slice_few<kPrThreads, kRows, kPrUnit>(a.p, a.q, ctas,
                                                                            cta, s_scan, s_meta);
@@ -517,8 +520,8 @@ __global__ void __launch_bounds__(kPrThreads, 2) paged_rows_kernel(const RowsArg
     team_sync();
     const bool entire = seg == n_units;
     const int64_t item_u0 = u - off;  // the item's first unit in the call's list
-    const int c_first = slice_owner(units, ctas, item_u0);
-    const int c_last = slice_owner(units, ctas, item_u0 + n_units - 1);
+    const int c_first = entire ? cta : slice_owner(units, ctas, item_u0);
+    const int c_last = entire ? cta : slice_owner(units, ctas, item_u0 + n_units - 1);
     const int slot = 2 * cta + (cta == c_first ? 1 : 0);
     constexpr int kV = D / 4;              // float4 columns
     constexpr int kG = kTeam * 32 / kV;    // row groups
@@ -661,7 +664,14 @@ __global__ void __launch_bounds__(kPrThreads, 2) paged_rows_kernel(const RowsArg
     team_sync();  // the ring and s_ml are free again
     off = 0;
     if (kSel) {
-      sel_load(++sel_item);
+      if (++it.head == hkv) {
+        it.head = 0;
+        if (++rt == sel_rts) {
+          rt = 0;
+          sel_token(it.tok0 + 1);
+        }
+        sel_rows();
+      }
     } else {
       paged_next_item<kRows, kPrUnit>(a.p, a.q, span, rt, it);
     }
@@ -670,8 +680,9 @@ __global__ void __launch_bounds__(kPrThreads, 2) paged_rows_kernel(const RowsArg
 }
 
 template <bool kBF16, int D, int MT, bool kSel, bool kSolo>
-int launch_rows_t(RowsArgs a, int ctas, void* ws, cudaStream_t stream) {
-  using C = RowsCfg<D, MT>;
+int launch_rows_t(RowsArgs a, void* ws, cudaStream_t stream) {
+  using C = RowsCfg<D, MT, kSel>;
+  const int ctas = C::kCtas * device_sm_count(current_device());
   a.part = paged_partials(ws, ctas * (kSolo ? kPrWarps : 1), C::kRows);
   auto kern = paged_rows_kernel<kBF16, D, MT, kSel, kSolo>;
   TDSA_CUDA_CHECK(ensure_dynamic_smem(reinterpret_cast<const void*>(kern), C::kSmem));
@@ -682,23 +693,27 @@ int launch_rows_t(RowsArgs a, int ctas, void* ws, cudaStream_t stream) {
 }
 
 template <bool kBF16, int D, int MT>
-int launch_rows_d(const RowsArgs& a, int ctas, void* ws, cudaStream_t stream) {
-  if (!a.q.idx) return launch_rows_t<kBF16, D, MT, false, false>(a, ctas, ws, stream);
+int launch_rows_d(const RowsArgs& a, void* ws, cudaStream_t stream) {
+  if (!a.q.idx) return launch_rows_t<kBF16, D, MT, false, false>(a, ws, stream);
   // a warp per item once every warp has one: nothing then waits for the CTA's other warps
   // (683 tokens x 2 heads x 512 positions: @@ us against @@)
   const int64_t items = static_cast<int64_t>(a.p.tokens) * a.p.kv_heads *
                         ((a.q.group + 16 * MT - 1) / (16 * MT));
-  if (items >= static_cast<int64_t>(ctas) * kPrWarps)
-    return launch_rows_t<kBF16, D, MT, true, true>(a, ctas, ws, stream);
-  return launch_rows_t<kBF16, D, MT, true, false>(a, ctas, ws, stream);
+  if (items >= static_cast<int64_t>(RowsCfg<D, MT, true>::kCtas) * kPrWarps *
+                   device_sm_count(current_device()))
+    return launch_rows_t<kBF16, D, MT, true, true>(a, ws, stream);
+  return launch_rows_t<kBF16, D, MT, true, false>(a, ws, stream);
 }
-
-int rows_ctas() { return 2 * device_sm_count(current_device()); }
 
 }  // namespace
 
 size_t paged_rows_workspace_bytes(int dim) {
-  return paged_partial_bytes(rows_ctas() * kPrWarps, 32, dim);
+  // the most of any variant: CTAs of an SM times rows, and teams of one warp
+  const int sms = device_sm_count(current_device());
+  return dim == 128 ? std::max(paged_partial_bytes(RowsCfg<128, 1, true>::kCtas * sms * kPrWarps, 16, dim),
+                               paged_partial_bytes(RowsCfg<128, 2, true>::kCtas * sms * kPrWarps, 32, dim))
+                    : std::max(paged_partial_bytes(RowsCfg<64, 1, true>::kCtas * sms * kPrWarps, 16, dim),
+                               paged_partial_bytes(RowsCfg<64, 2, true>::kCtas * sms * kPrWarps, 32, dim));
 }
 
 int launch_paged_rows(const PagedView& p, const PagedQuery& q, int dtype, int dim, int rows,
@@ -707,20 +722,19 @@ int launch_paged_rows(const PagedView& p, const PagedQuery& q, int dtype, int di
   a.p = p;
   a.q = q;
   a.status = status;
-  const int ctas = rows_ctas();
   const bool narrow = rows <= 16;
   if (dtype == TDSA_BF16) {
     if (dim == 128)
-      return narrow ? launch_rows_d<true, 128, 1>(a, ctas, ws, stream)
-                    : launch_rows_d<true, 128, 2>(a, ctas, ws, stream);
-    return narrow ? launch_rows_d<true, 64, 1>(a, ctas, ws, stream)
-                  : launch_rows_d<true, 64, 2>(a, ctas, ws, stream);
+      return narrow ? launch_rows_d<true, 128, 1>(a, ws, stream)
+                    : launch_rows_d<true, 128, 2>(a, ws, stream);
+    return narrow ? launch_rows_d<true, 64, 1>(a, ws, stream)
+                  : launch_rows_d<true, 64, 2>(a, ws, stream);
   }
   if (dim == 128)
-    return narrow ? launch_rows_d<false, 128, 1>(a, ctas, ws, stream)
-                  : launch_rows_d<false, 128, 2>(a, ctas, ws, stream);
-  return narrow ? launch_rows_d<false, 64, 1>(a, ctas, ws, stream)
-                : launch_rows_d<false, 64, 2>(a, ctas, ws, stream);
+    return narrow ? launch_rows_d<false, 128, 1>(a, ws, stream)
+                  : launch_rows_d<false, 128, 2>(a, ws, stream);
+  return narrow ? launch_rows_d<false, 64, 1>(a, ws, stream)
+                : launch_rows_d<false, 64, 2>(a, ws, stream);
 }
 
 }  // namespace tdsa

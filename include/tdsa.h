@@ -638,7 +638,7 @@ typedef struct tdsa_token_rows {
   int64_t head_stride;
 } tdsa_token_rows;
 
-#define TDSA_PAGED_COUNTER_BYTES 8192
+#define TDSA_PAGED_COUNTER_BYTES 16384
 
 /*
  * Writes the keys (rotated) and values of every new token into its slot of the cache and, when

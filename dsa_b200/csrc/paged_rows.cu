@@ -695,8 +695,8 @@ int launch_rows_t(RowsArgs a, void* ws, cudaStream_t stream) {
 template <bool kBF16, int D, int MT>
 int launch_rows_d(const RowsArgs& a, void* ws, cudaStream_t stream) {
   if (!a.q.idx) return launch_rows_t<kBF16, D, MT, false, false>(a, ws, stream);
-  // a warp per item once every warp has one: nothing then waits for the CTA's other warps
-  // (683 tokens x 2 heads x 512 positions: @@ us against @@)
+  // a warp per item once every warp has one: nothing then waits for the CTA's other warps (6225
+  // tokens x 8 heads x 22 positions: 146 us against 253; with 512 positions both take 36 us)
   const int64_t items = static_cast<int64_t>(a.p.tokens) * a.p.kv_heads *
                         ((a.q.group + 16 * MT - 1) / (16 * MT));
   if (items >= static_cast<int64_t>(RowsCfg<D, MT, true>::kCtas) * kPrWarps *

@@ -31,10 +31,8 @@ namespace tdsa {
 
 namespace {
 
-constexpr int kPrWarps = 4;
-constexpr int kPrThreads = kPrWarps * 32;
+constexpr int kPrNarrow = 4, kPrWide = 8;       // warps of a CTA (see launch_rows_d)
 constexpr int kPrTile = 16;                     // keys per warp and tile
-constexpr int kPrUnit = kPrWarps * kPrTile;     // keys per unit of work
 
 struct RowsArgs {
   PagedView p;
@@ -43,7 +41,7 @@ struct RowsArgs {
   int* status;
 };
 
-template <int D, int MT, bool kSel>
+template <int D, int MT, bool kSel, int kWarps>
 struct RowsCfg {
   static constexpr int kRowBytes = D * 2;
   static constexpr int kTileBytes = kPrTile * kRowBytes;       // K or V tile
@@ -51,14 +49,15 @@ struct RowsCfg {
   // CTAs per SM, and tiles of a warp's ring (96 KB of ring per SM and more): selected keys of 64
   // features gain from more warps (683 tokens x 2 heads x 512: 38 us with 4 CTAs, 44 with 2), runs
   // of pages do not (11 sequences x 16 heads x 16461: 150 us against 141).
-  static constexpr int kCtas = D == 64 && MT == 1 && kSel ? 4 : 2;
-  static constexpr int kStages = D == 128 || kCtas == 4 ? 3 : 6;
+  static constexpr int kSmWarps = D == 64 && MT == 1 && kSel ? 16 : 8;
+  static constexpr int kCtas = kSmWarps / kWarps;
+  static constexpr int kStages = D == 128 || kSmWarps == 16 ? 3 : 6;
   static constexpr int kWarpBytes = kStages * kStageBytes;
   static constexpr int kRows = 16 * MT;
   static constexpr int kMergeO = kRows * D * 4;                // a warp's output, float32
-  static constexpr int kRing = kPrWarps * kWarpBytes;
-  static constexpr int kMl = kPrWarps * kRows * 8;
-  static constexpr int kSmem = kRing + kMl + 256 + kPrWarps * kStages * 4;
+  static constexpr int kRing = kWarps * kWarpBytes;
+  static constexpr int kMl = kWarps * kRows * 8;
+  static constexpr int kSmem = kRing + kMl + 256 + kWarps * kStages * 4;
   static_assert(kMergeO <= kWarpBytes, "a warp's output fits its ring");
 };
 
@@ -107,10 +106,12 @@ __device__ __forceinline__ void cp_async_wait() {
 
 // kSolo (selected attention): a warp takes items of its own instead of a quarter of the CTA's, so
 // that nothing waits for the other warps where items are short and many.
-template <bool kBF16, int D, int MT, bool kSel, bool kSolo>
-__global__ void __launch_bounds__(kPrThreads, RowsCfg<D, MT, kSel>::kCtas)
+template <bool kBF16, int D, int MT, bool kSel, bool kSolo, int kPrWarps>
+__global__ void __launch_bounds__(kPrWarps * 32, RowsCfg<D, MT, kSel, kPrWarps>::kCtas)
     paged_rows_kernel(const RowsArgs a) {
-  using C = RowsCfg<D, MT, kSel>;
+  using C = RowsCfg<D, MT, kSel, kPrWarps>;
+  constexpr int kPrThreads = kPrWarps * 32;
+  constexpr int kPrUnit = kPrWarps * kPrTile;      // keys per unit of work
   static_assert(kSel || !kSolo, "");
   constexpr int kTeam = kSolo ? 1 : kPrWarps;      // warps that share an item
   constexpr int kUnitTiles = kPrWarps / kTeam;     // tiles of a unit per warp
@@ -124,7 +125,7 @@ __global__ void __launch_bounds__(kPrThreads, RowsCfg<D, MT, kSel>::kCtas)
   float2* s_ml =
       reinterpret_cast<float2*>(smem + C::kRing) + (kSolo ? (threadIdx.x >> 5) * kRows : 0);
   int* s_meta = reinterpret_cast<int*>(smem + C::kRing + C::kMl);
-  int64_t* s_scan = reinterpret_cast<int64_t*>(s_meta + 8);   // [4] warp totals
+  int64_t* s_scan = reinterpret_cast<int64_t*>(s_meta + 8);   // [warp] totals
   // [warp][stage]: bit r is set when row r of the stage's tile holds a key of the cache
   uint32_t* s_valid = reinterpret_cast<uint32_t*>(smem + C::kRing + C::kMl + 256) +
                       (threadIdx.x >> 5) * kStages;
@@ -679,41 +680,51 @@ __global__ void __launch_bounds__(kPrThreads, RowsCfg<D, MT, kSel>::kCtas)
   if (__any_sync(0xffffffffu, bad) && lane == 0) atomicOr(a.status, TDSA_STATUS_RANGE);
 }
 
-template <bool kBF16, int D, int MT, bool kSel, bool kSolo>
+template <bool kBF16, int D, int MT, bool kSel, bool kSolo, int kWarps>
 int launch_rows_t(RowsArgs a, void* ws, cudaStream_t stream) {
-  using C = RowsCfg<D, MT, kSel>;
+  using C = RowsCfg<D, MT, kSel, kWarps>;
   const int ctas = C::kCtas * device_sm_count(current_device());
-  a.part = paged_partials(ws, ctas * (kSolo ? kPrWarps : 1), C::kRows);
-  auto kern = paged_rows_kernel<kBF16, D, MT, kSel, kSolo>;
+  a.part = paged_partials(ws, ctas * (kSolo ? kWarps : 1), C::kRows);
+  auto kern = paged_rows_kernel<kBF16, D, MT, kSel, kSolo, kWarps>;
   TDSA_CUDA_CHECK(ensure_dynamic_smem(reinterpret_cast<const void*>(kern), C::kSmem));
-  TDSA_CUDA_CHECK(launch_pdl(kern, dim3(static_cast<unsigned>(ctas)), dim3(kPrThreads), C::kSmem,
+  TDSA_CUDA_CHECK(launch_pdl(kern, dim3(static_cast<unsigned>(ctas)), dim3(kWarps * 32), C::kSmem,
                              stream, a));
   TDSA_CUDA_CHECK(cudaGetLastError());
   return TDSA_OK;
 }
 
+// Three layouts by the number of items a call can have (`most`).  With fewer than SMs, every item
+// is split, and CTAs of eight warps leave half the parts to join of CTAs of four (one sequence of
+// 32768 positions x 8 heads: @@ us against 35.7); with more, smaller CTAs fill each other's
+// pauses between items (64 sequences x 8 heads x 2048 selected: 94 us against @@).  Selected
+// attention with an item for every warp leaves the teams out: 6225 tokens x 8 heads x 22
+// positions take 146 us against 253; with 512 positions both take 36 us.
 template <bool kBF16, int D, int MT>
-int launch_rows_d(const RowsArgs& a, void* ws, cudaStream_t stream) {
-  if (!a.q.idx) return launch_rows_t<kBF16, D, MT, false, false>(a, ws, stream);
-  // a warp per item once every warp has one: nothing then waits for the CTA's other warps (6225
-  // tokens x 8 heads x 22 positions: 146 us against 253; with 512 positions both take 36 us)
-  const int64_t items = static_cast<int64_t>(a.p.tokens) * a.p.kv_heads *
-                        ((a.q.group + 16 * MT - 1) / (16 * MT));
-  if (items >= static_cast<int64_t>(RowsCfg<D, MT, true>::kCtas) * kPrWarps *
-                   device_sm_count(current_device()))
-    return launch_rows_t<kBF16, D, MT, true, true>(a, ws, stream);
-  return launch_rows_t<kBF16, D, MT, true, false>(a, ws, stream);
+int launch_rows_d(const RowsArgs& a, int rows, void* ws, cudaStream_t stream) {
+  const int sms = device_sm_count(current_device());
+  const int64_t tiles = (rows + 16 * MT - 1) / (16 * MT);
+  const int64_t most = (a.q.idx ? a.p.tokens : a.p.batch) * tiles * a.p.kv_heads;
+  if (!a.q.idx) {
+    if (most <= sms) return launch_rows_t<kBF16, D, MT, false, false, kPrWide>(a, ws, stream);
+    return launch_rows_t<kBF16, D, MT, false, false, kPrNarrow>(a, ws, stream);
+  }
+  if (most <= sms) return launch_rows_t<kBF16, D, MT, true, false, kPrWide>(a, ws, stream);
+  if (most >= static_cast<int64_t>(RowsCfg<D, MT, true, kPrNarrow>::kSmWarps) * sms)
+    return launch_rows_t<kBF16, D, MT, true, true, kPrNarrow>(a, ws, stream);
+  return launch_rows_t<kBF16, D, MT, true, false, kPrNarrow>(a, ws, stream);
 }
 
 }  // namespace
 
 size_t paged_rows_workspace_bytes(int dim) {
-  // the most of any variant: CTAs of an SM times rows, and teams of one warp
+  // the most of any variant: teams of one warp, and their rows
   const int sms = device_sm_count(current_device());
-  return dim == 128 ? std::max(paged_partial_bytes(RowsCfg<128, 1, true>::kCtas * sms * kPrWarps, 16, dim),
-                               paged_partial_bytes(RowsCfg<128, 2, true>::kCtas * sms * kPrWarps, 32, dim))
-                    : std::max(paged_partial_bytes(RowsCfg<64, 1, true>::kCtas * sms * kPrWarps, 16, dim),
-                               paged_partial_bytes(RowsCfg<64, 2, true>::kCtas * sms * kPrWarps, 32, dim));
+  const int warps = dim == 128 ? RowsCfg<128, 1, true, kPrNarrow>::kSmWarps
+                               : RowsCfg<64, 1, true, kPrNarrow>::kSmWarps;
+  const int wide_rows = dim == 128 ? RowsCfg<128, 2, true, kPrNarrow>::kSmWarps
+                                   : RowsCfg<64, 2, true, kPrNarrow>::kSmWarps;
+  return std::max(paged_partial_bytes(warps * sms, 16, dim),
+                  paged_partial_bytes(wide_rows * sms, 32, dim));
 }
 
 int launch_paged_rows(const PagedView& p, const PagedQuery& q, int dtype, int dim, int rows,
@@ -725,16 +736,16 @@ int launch_paged_rows(const PagedView& p, const PagedQuery& q, int dtype, int di
   const bool narrow = rows <= 16;
   if (dtype == TDSA_BF16) {
     if (dim == 128)
-      return narrow ? launch_rows_d<true, 128, 1>(a, ws, stream)
-                    : launch_rows_d<true, 128, 2>(a, ws, stream);
-    return narrow ? launch_rows_d<true, 64, 1>(a, ws, stream)
-                  : launch_rows_d<true, 64, 2>(a, ws, stream);
+      return narrow ? launch_rows_d<true, 128, 1>(a, rows, ws, stream)
+                    : launch_rows_d<true, 128, 2>(a, rows, ws, stream);
+    return narrow ? launch_rows_d<true, 64, 1>(a, rows, ws, stream)
+                  : launch_rows_d<true, 64, 2>(a, rows, ws, stream);
   }
   if (dim == 128)
-    return narrow ? launch_rows_d<false, 128, 1>(a, ws, stream)
-                  : launch_rows_d<false, 128, 2>(a, ws, stream);
-  return narrow ? launch_rows_d<false, 64, 1>(a, ws, stream)
-                : launch_rows_d<false, 64, 2>(a, ws, stream);
+    return narrow ? launch_rows_d<false, 128, 1>(a, rows, ws, stream)
+                  : launch_rows_d<false, 128, 2>(a, rows, ws, stream);
+  return narrow ? launch_rows_d<false, 64, 1>(a, rows, ws, stream)
+                : launch_rows_d<false, 64, 2>(a, rows, ws, stream);
 }
 
 }  // namespace tdsa

@@ -258,6 +258,7 @@ int paged_setup(const tdsa_paged_cache* c, const tdsa_paged_batch* b, PagedView&
   p.batch = b->batch;
   p.max_pages = b->max_pages;
   p.tokens = b->tokens;
+  p.status = nullptr;
   return TDSA_OK;
 }
 
@@ -1201,6 +1202,7 @@ int tdsa_paged_append(const tdsa_paged_cache* cache, const tdsa_paged_batch* bat
   if (rc) return rc;
   int* status = device_status_ptr();
   if (!status) return fail(TDSA_ERR_CUDA, "device status word not available");
+  p.status = status;
   return launch_paged_append(p, cache->keys, cache->values, cache->dtype, cache->head_dim,
                              k->data, k->token_stride, k->head_stride, v->data,
                              v->token_stride, v->head_stride, q ? q->data : nullptr,
@@ -1229,6 +1231,7 @@ int tdsa_paged_attention(const tdsa_paged_cache* cache, const tdsa_paged_batch* 
   d.window = window;
   int* status = device_status_ptr();
   if (!status) return fail(TDSA_ERR_CUDA, "device status word not available");
+  p.status = status;
   const int64_t rows = static_cast<int64_t>(batch->max_new) * d.group;
   if (rows > 32)
     return launch_paged_chunk(p, d, cache->dtype, cache->head_dim, workspace, status,
@@ -1262,6 +1265,7 @@ int tdsa_selected_attention(const tdsa_paged_cache* cache, const tdsa_paged_batc
   d.topk = k;
   int* status = device_status_ptr();
   if (!status) return fail(TDSA_ERR_CUDA, "device status word not available");
+  p.status = status;
   return launch_paged_rows(p, d, cache->dtype, cache->head_dim, d.group, workspace, status,
                            static_cast<cudaStream_t>(stream));
 }

@@ -78,9 +78,10 @@ __global__ void __launch_bounds__(kPaThreads, kPaThreads == kPaShort ? 5 : 9)
   for (int b = tid; b < a.p.batch; b += kPaThreads) {
     const SeqSpan s = load_span(a.p, b);
     if (t >= s.q0 && t < s.q0 + s.n) {
-      const int pos = s.len - s.n + static_cast<int>(t - s.q0);
-      s_pos = pos;
-      s_page = pos >= 0 ? __ldg(a.p.table + b * a.p.table_stride + (pos >> a.p.page_shift)) : -1;
+      const int64_t pos = static_cast<int64_t>(s.told) - s.n + (t - s.q0);
+      const bool in = pos >= 0 && (pos >> a.p.page_shift) < a.p.max_pages;
+      s_pos = static_cast<int>(max(int64_t(-1), min(pos, int64_t(0x7FFFFFFF))));
+      s_page = in ? __ldg(a.p.table + b * a.p.table_stride + (pos >> a.p.page_shift)) : -1;
       found = true;
     }
   }

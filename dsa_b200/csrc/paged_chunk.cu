@@ -22,9 +22,19 @@
 // rescales its row of O in place, which it does only when the row's maximum has grown by a
 // factor of more than 2^8 of weight (rare after the first units).
 //
+// What bounds it.  A unit of both tiles is 2048 cycles of tensor work (2560 with S in parts of 64,
+// whose operands shared memory delivers in 48 cycles instead of 32) and 3600 cycles of the rows'
+// warps: 64 scores of a row and part are read, compared and exponentiated in 1830 cycles with two
+// warps on an SM quarter, 1150 of them the exponentials, where the special-function pipe, the fma
+// pipe (a third of the exponentials) and the latency of either add up.  Sixteen warps of rows with
+// half a part each, and turns between the two tiles' exponentials, both measured the same.  4096
+// tokens over 16384 positions (32 heads in groups of 4, 128 features, 962 GFLOP): 0.86 ms alone,
+// 1.12 PFLOP/s against the 1.67 of a library product; 0.99 ms, 0.97 PFLOP/s, in a loop that holds
+// the card at its power limit, where the library product reaches 1.39.
+//
 // Scores, maxima, sums and O are float32.  P is rounded to the cache's type for the second
-// product (2^-8 relative in bf16, 2^-11 in f16, the rounding that the output gets too); the sum
-// adds the unrounded P.
+// product (2^-8 relative in bf16, 2^-11 in f16, the rounding that the output gets too; a second
+// term for what it leaves would be half as much tensor work again); the sum adds the unrounded P.
 #include <algorithm>
 
 #include "paged.cuh"

@@ -7,22 +7,31 @@
 // key/value head (times the sequence's new tokens), 16 MT of them, so every key and value is
 // read from the cache once.
 //
-// Layout.  A CTA is four warps.  Each warp runs its own stream of 16-key tiles (unit u of an
-// item is 64 keys, 16 per warp) with its own ring of tiles in shared memory, filled by 16-byte
-// asynchronous copies -- a row of the cache is gathered by address, so pages and selected
-// positions cost the same -- and its own running maximum, sum and output in registers; warps
-// meet only at the end of an item's segment.  No block-wide barrier is in the key loop.  S = Q K^T
-// and O += P V are warp-level 16x8x16 matrix instructions with float32 accumulators: with 1 to
-// 32 rows the tensor work is a fifth of the time the keys take to arrive, and their operands
-// and results stay in registers, which a tile of fewer rows than the 64 to 128 of a tcgen05
-// instruction could not.  P is rounded to the cache's type for the second product (relative
-// 2^-8 in bf16 and 2^-11 in f16, the rounding that the output gets too); maxima and sums are
-// float32, the sum of the unrounded P.
+// HBM bound: a key and its value are 4 D bytes for 4 D rows multiply-adds.  32 ragged sequences
+// (979 MB) take 161 us, 6.1 TB/s of the 6.55 that a copy reaches; 2048 selected positions for 64
+// sequences (537 MB in pieces of 256 bytes) 95 us, 5.7 TB/s; one sequence of 32768 positions (134
+// MB) 36 us, 9 of them before the first tile is there and after the last, and the slowest SM a
+// third later than the fastest.
+//
+// Layout.  A CTA is four or eight warps.  Each warp runs its own stream of 16-key tiles (a unit is
+// a tile per warp) with its own ring of tiles in shared memory, filled by 16-byte asynchronous
+// copies -- a row of the cache is gathered by address, so pages and selected positions cost the
+// same -- and its own running maximum, sum and output in registers; warps meet only at the end of
+// an item's segment.  No block-wide barrier is in the key loop.  S = Q K^T and O += P V are
+// warp-level 16x8x16 matrix instructions with float32 accumulators: with 1 to 32 rows they keep
+// the tensor pipe busy for a quarter of the time the keys take to arrive, and their operands and
+// results stay in registers, which a tile of fewer rows than the 64 to 128 of a tcgen05
+// instruction could not.
+//
+// Scores, maxima, sums and O are float32.  P enters the second product as a 16-bit value and a
+// second one that holds what its rounding left (2^-16 relative in bf16, 2^-22 in f16, below the
+// output's rounding): twice the products, which are not what bounds this kernel -- 161 us against
+// 160 with one term at 128 features, 149 against 142 at 64 -- for errors 0.7 times as large.
 //
 // Values of keys that no row of the item sees (past the length, or of a page that is not one)
 // are zero-filled on arrival.  In a tile that some rows see and others do not, a value that is
 // not finite would turn the zero weight of the others into NaN; such a tile's product is formed
-// element by element (add_visible).
+// element by element.
 #include <algorithm>
 
 #include "paged.cuh"
@@ -414,7 +423,7 @@ __global__ void __launch_bounds__(kPrWarps * 32, RowsCfg<D, MT, kSel, kPrWarps>:
             }
           }
       }
-      uint32_t pf[MT][4];
+      uint32_t pf[MT][4], pl[MT][4];  // P rounded, and what the rounding left
 #pragma unroll
       for (int m = 0; m < MT; ++m) {
 #pragma unroll
@@ -429,10 +438,13 @@ __global__ void __launch_bounds__(kPrWarps * 32, RowsCfg<D, MT, kSel, kPrWarps>:
               sum[m][e] += p;
             }
         }
-        pf[m][0] = pack16<kBF16>(s[m][0][0], s[m][0][1]);
-        pf[m][1] = pack16<kBF16>(s[m][0][2], s[m][0][3]);
-        pf[m][2] = pack16<kBF16>(s[m][1][0], s[m][1][1]);
-        pf[m][3] = pack16<kBF16>(s[m][1][2], s[m][1][3]);
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+          const float u = s[m][x >> 1][2 * (x & 1)], w = s[m][x >> 1][2 * (x & 1) + 1];
+          pf[m][x] = pack16<kBF16>(u, w);
+          const float2 r = unpack16<kBF16>(pf[m][x]);
+          pl[m][x] = pack16<kBF16>(u - r.x, w - r.y);
+        }
       }
       const uint32_t sv = st + C::kTileBytes;
       bool slow = false;
@@ -458,6 +470,8 @@ __global__ void __launch_bounds__(kPrWarps * 32, RowsCfg<D, MT, kSel, kPrWarps>:
           for (int m = 0; m < MT; ++m) {
             mma16816<kBF16>(o[m][2 * c], pf[m], b[0], b[1]);
             mma16816<kBF16>(o[m][2 * c + 1], pf[m], b[2], b[3]);
+            mma16816<kBF16>(o[m][2 * c], pl[m], b[0], b[1]);
+            mma16816<kBF16>(o[m][2 * c + 1], pl[m], b[2], b[3]);
           }
         }
       } else {
@@ -694,11 +708,11 @@ int launch_rows_t(RowsArgs a, void* ws, cudaStream_t stream) {
 }
 
 // Three layouts by the number of items a call can have (`most`).  With fewer than SMs, every item
-// is split, and CTAs of eight warps leave half the parts to join of CTAs of four (one sequence of
-// 32768 positions x 8 heads: @@ us against 35.7); with more, smaller CTAs fill each other's
-// pauses between items (64 sequences x 8 heads x 2048 selected: 94 us against @@).  Selected
-// attention with an item for every warp leaves the teams out: 6225 tokens x 8 heads x 22
-// positions take 146 us against 253; with 512 positions both take 36 us.
+// is split, and CTAs of eight warps leave half the parts to join of CTAs of four (2048 selected
+// positions for one sequence: 10.9 us against 13.7); with more, smaller CTAs fill each other's
+// pauses between items (32 ragged sequences x 8 heads: 160 us against 171).  Selected attention
+// with an item for every warp leaves the teams out: 6225 tokens x 8 heads x 22 positions take 146
+// us against 253; with 512 positions both take 36 us.
 template <bool kBF16, int D, int MT>
 int launch_rows_d(const RowsArgs& a, int rows, void* ws, cudaStream_t stream) {
   const int sms = device_sm_count(current_device());

@@ -604,7 +604,7 @@ int tdsa_query_prep(const void* qraw, int64_t qraw_stride, const void* hidden,
  * max_new is the host's bound on a sequence's new tokens: it chooses a kernel, and results do
  * not depend on it.  max_pages * page_size <= 2^30.  Table entries are read only where a
  * position is needed; a page outside [0, pages) raises TDSA_STATUS_RANGE and its positions
- * count as absent.
+ * count as absent, and so do positions past max_pages * page_size and a negative length's.
  */
 typedef struct tdsa_paged_cache {
   void* keys;
@@ -663,11 +663,12 @@ int tdsa_paged_append(const tdsa_paged_cache* cache, const tdsa_paged_batch* bat
  *   out[t][h] = sum_j softmax_j(scale * q[t][h] . K[j][h / g]) V[j][h / g],  g = q_heads /
  *   kv_heads;  lse[t][h] = log sum_j exp(scale * q . K[j]) (float32, [tokens][q_heads], NULL:
  *   not wanted).
- * A token that sees no key gets out 0 and lse -inf.  out must not overlap q.  float32 scores, maxima and sums; the
- * softmax weights are rounded to the cache's type for the product with V.  scale > 0.
+ * A token that sees no key gets out 0 and lse -inf.  out must not overlap q.  float32 scores,
+ * maxima and sums; in long chunks the softmax weights are rounded to the cache's type for the
+ * product with V.  scale > 0.
  * workspace: tdsa_paged_workspace_bytes bytes, 256-byte aligned, its first
  * TDSA_PAGED_COUNTER_BYTES zero before its first use; every call leaves it ready for the next
- * one on the same stream.
+ * one on the same stream (after a TDSA_ERR_TIMEOUT, zero them again).
  */
 int tdsa_paged_attention(const tdsa_paged_cache* cache, const tdsa_paged_batch* batch,
                          const tdsa_token_rows* q, int q_heads, float scale, int window,

@@ -198,6 +198,40 @@ def test_a_page_outside_the_cache_is_absent_and_reported():
         assert_attention(out, None, c.reference(indices=ind), BF16)
 
 
+@pytest.mark.parametrize("n", [1, 2, 40])
+def test_many_sequences(n):
+    # more sequences than a block has threads, some with no new token or no position
+    lens = [(7 * i) % 90 for i in range(900)]
+    news = [0 if i % 5 == 2 else min(1 + i % n, max(lens[i], 1)) for i in range(900)]
+    c = Case(news, lens, dim=64, hq=4, hkv=1, seed=14)
+    assert_attention(*_attend(c), c.reference(), BF16)
+
+
+@pytest.mark.parametrize("n", [1, 40])
+def test_a_length_past_the_page_table_is_reported(n):
+    from dsa_b200 import _capi as capi
+    from dsa_b200 import device_status
+    from dsa_b200.paged import PagedAppender
+
+    c = Case([n, 1], [96, 20], page=32, seed=15)
+    width = c.batch.page_table.shape[1] * 32
+    for wrong in (width + 5, -3):
+        c.batch.lengths[0] = wrong
+        _attend(c)
+        assert device_status() & capi.TDSA_STATUS_RANGE
+        before = c.cache.keys.clone()
+        k = torch.ones(n + 1, 2, 128, dtype=BF16, device="cuda")
+        PagedAppender(c.cache, rope_dim=0).append(c.batch, k, k)
+        assert device_status() & capi.TDSA_STATUS_RANGE
+        changed = (c.cache.keys.view(torch.int16) != before.view(torch.int16)).any(-1).any(-1)
+        # the other sequence's token, and those of the first that the table still reaches
+        slots = {(int(c.table[1, 19 // 32]), 19)}
+        assert {tuple(x) for x in changed.nonzero().tolist()} <= slots | {
+            (int(c.table[0, p // 32]), p % 32) for p in range(96)}
+    c.batch.lengths[0] = 96
+    device_status()
+
+
 def test_offsets_past_32_bits():
     from dsa_b200.paged import PagedBatch, PagedKV, paged_attention
 

@@ -82,6 +82,13 @@ __device__ __forceinline__ bool nonfinite16(uint32_t p) {
   return (p & e) == e || ((p >> 16) & e) == e;
 }
 
+// The same of several pairs: bits of 0x80008000 in the or of nonfinite_bits(p).  An exponent of
+// ones carries into the sign's place, which the mask has cleared, and no further.
+template <bool kBF16>
+__device__ __forceinline__ uint32_t nonfinite_bits(uint32_t p) {
+  return kBF16 ? (p & 0x7F807F80u) + 0x00800080u : (p & 0x7C007C00u) + 0x04000400u;
+}
+
 __device__ __forceinline__ float exp2_approx(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));

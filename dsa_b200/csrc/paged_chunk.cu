@@ -553,14 +553,21 @@ __global__ void __launch_bounds__(kPcThreads, 1)
           }
           tmem_wait_ld();
           if (masked) {
+            // the keys of the part that the row sees, a bit each
+            const int from = max(0, lo - base), to = min(kPcPart, hi - base);
+            const uint64_t below_to = to >= 64 ? ~0ull : (to <= 0 ? 0ull : (1ull << to) - 1);
+            const uint64_t below_from = from >= 64 ? ~0ull : (1ull << from) - 1;
+            uint64_t seen = below_to & ~below_from;
 #pragma unroll
-            for (int c = 0; c < 2; ++c)
+            for (int x = 0; x < 4; ++x)
+              if ((gone >> x) & 1u) seen &= ~(0xFFFFull << (16 * x));
 #pragma unroll
-              for (int j = 0; j < 32; ++j) {
-                const int k = base + c * 32 + j;
-                if (k < lo || k >= hi || ((gone >> (2 * c + (j >> 4))) & 1u))
-                  s[c][j] = 0xFF800000u;  // -infinity
-              }
+            for (int c = 0; c < 2; ++c) {
+              const uint32_t w = static_cast<uint32_t>(seen >> (32 * c));
+#pragma unroll
+              for (int j = 0; j < 32; ++j)
+                if (!((w >> j) & 1u)) s[c][j] = 0xFF800000u;  // -infinity
+            }
           }
           float tops[4];
 #pragma unroll
@@ -624,31 +631,31 @@ __global__ void __launch_bounds__(kPcThreads, 1)
           }
           tmem_wait_st();
           if (masked) {
-            // a value that only some rows see and that is not finite: zero weights times it
-            // would be NaN for the others, so the threads form this part's product themselves
+            // A value that only some rows see and that is not finite: zero weights times it
+            // would be NaN for the others, so the threads then form this part's product
+            // themselves.
             const uint32_t vi = 2 * (n_unit + i) + 1;  // K, V, K, V, ... fill the ring
             const uint32_t st = vi % C::kStages;
             ok = warp_wait(&full[st], (vi / C::kStages) & 1u, abort_flag);
             if (!ok) break;
             const uint8_t* sv = smem + st * C::kTileBytes + b * kPcPart * 128;
-            bool odd = false;
+            const int key0 = sg->k0 - base, key1 = sg->k1 - base;
+            uint32_t odd = 0u;
 #pragma unroll
             for (int x = 0; x < D / 16; ++x) {  // 16 bytes at a time, side by side
               const int c = (x & 3) * kPcTile + row;
-              const int key = base + (c >> 3);
               const uint4 w = *reinterpret_cast<const uint4*>(sv + (x >> 2) * kPcHalf + c * 16);
-              odd |= key >= sg->k0 && key < sg->k1 &&
-                     (nonfinite16<kBF16>(w.x) || nonfinite16<kBF16>(w.y) ||
-                      nonfinite16<kBF16>(w.z) || nonfinite16<kBF16>(w.w));
+              const uint32_t bits = nonfinite_bits<kBF16>(w.x) | nonfinite_bits<kBF16>(w.y) |
+                                    nonfinite_bits<kBF16>(w.z) | nonfinite_bits<kBF16>(w.w);
+              if ((c >> 3) >= key0 && (c >> 3) < key1) odd |= bits;
             }
             // three ballots in turn: the next one was last read before the meeting before this
-            if (__any_sync(0xffffffffu, odd) && lane == 0) s_odd[3 * t + vote] = 1;
-            const int next_vote = vote == 2 ? 0 : vote + 1;
-            if (row == 0) s_odd[3 * t + next_vote] = 0;
+            if (__any_sync(0xffffffffu, odd & 0x80008000u) && lane == 0) s_odd[3 * t + vote] = 1;
+            if (row == 0) s_odd[3 * t + (vote == 2 ? 0 : vote + 1)] = 0;
             ok = meet();
             if (!ok) break;
             const bool alone = s_odd[3 * t + vote] != 0;
-            vote = next_vote;
+            vote = vote == 2 ? 0 : vote + 1;
             if (alone) {
               ok = warp_wait(&sfull[2 * t + (b ^ 1)], (s_ph >> (b ^ 1)) & 1u, abort_flag);
               if (!ok) break;
@@ -673,10 +680,11 @@ __global__ void __launch_bounds__(kPcThreads, 1)
       if (!ok) break;
       tc_fence_after();
       const int r_item = t * kPcTile + row;  // row of the item
-      const int c_first = slice_owner(sl.units, sl.ctas, sg->item_u0);
-      const int c_last = slice_owner(sl.units, sl.ctas, sg->item_u0 + sg->item_units - 1);
+      int c_first = 0, c_last = 0;  // CTAs that hold parts of the item
       bool write = true;
       if (units != sg->item_units) {
+        c_first = slice_owner(sl.units, sl.ctas, sg->item_u0);
+        c_last = slice_owner(sl.units, sl.ctas, sg->item_u0 + sg->item_units - 1);
         // a part of the item: float32, the rows of a column quad side by side
         const int cta = blockIdx.x;
         const int64_t slot = 2 * cta + (cta == c_first ? 1 : 0);

@@ -26,6 +26,10 @@ import torch
 from . import _capi as capi
 from .indexer import require_cuda, stream_ptr
 
+# torch.cuda.is_current_stream_capturing without its Python frame
+_capturing = getattr(torch._C, "_cuda_isCurrentStreamCapturing",
+                     torch.cuda.is_current_stream_capturing)
+
 _DTYPES = {torch.float16: capi.TDSA_F16, torch.bfloat16: capi.TDSA_BF16}
 
 
@@ -133,11 +137,6 @@ def _check_rows(t: torch.Tensor, cache: PagedKV, heads: int | None, tokens: int 
         raise ValueError(f"{name} needs unit stride on the last axis")
 
 
-def _check_batch(batch: PagedBatch, cache: PagedKV) -> None:
-    if batch._index != cache._index:
-        raise ValueError("batch and cache must be on one device")
-
-
 _WORKSPACES: dict[tuple[int, int, int], tuple[torch.Tensor, int, int]] = {}
 
 
@@ -151,7 +150,7 @@ def paged_workspace(device: torch.device, head_dim: int,
         stream = stream_ptr(device)
     key = (device.index, stream, head_dim)
     ws = _WORKSPACES.get(key)
-    capturing = torch.cuda.is_current_stream_capturing()
+    capturing = _capturing()
     if ws is None or capturing:
         with torch.cuda.device(device):
             nbytes = capi.lib().tdsa_paged_workspace_bytes(head_dim)
@@ -197,8 +196,9 @@ class PagedAppender:
         ``q_out``, a new tensor by default, ``q`` itself allowed) or None without ``q``.
         ``positions`` int64 ``[tokens]`` replaces the tokens' positions in the angles."""
         cache = self.cache
-        _check_batch(batch, cache)
         dtype, index, shape = cache.dtype, cache._index, k.shape
+        if batch._index != index:
+            raise ValueError("batch and cache must be on one device")
         ks, vs = k.stride(), v.stride()
         if not (len(shape) == 3 and shape == v.shape and shape[1] == cache.kv_heads
                 and shape[2] == cache.head_dim and k.dtype is dtype and v.dtype is dtype
@@ -245,8 +245,9 @@ class PagedAppender:
 
 def _attention_args(q, cache, batch, out, return_lse):
     """Checks and descriptors shared by the attention calls."""
-    _check_batch(batch, cache)
     shape, dtype, index = q.shape, cache.dtype, cache._index
+    if batch._index != index:
+        raise ValueError("batch and cache must be on one device")
     if out is None:
         out = torch.empty_like(q)
     qs, os = q.stride(), out.stride()

@@ -44,6 +44,18 @@ def test_one_token_per_sequence(dtype, dim, hq, hkv, page):
     assert_attention(*_attend(c), c.reference(), dtype)
 
 
+@pytest.mark.parametrize("dtype,dim,hq,hkv", [(BF16, 128, 16, 4), (F16, 64, 32, 4),
+                                              (F16, 128, 32, 4), (BF16, 64, 4, 4)])
+@pytest.mark.parametrize("batch", [3, 50])
+@pytest.mark.parametrize("window", [None, 5, 70])
+def test_a_few_tokens_per_sequence(dtype, dim, hq, hkv, batch, window):
+    # up to 16 and up to 32 rows per key/value head, fewer and more items than SMs
+    lens = [(37 * i) % 400 + 4 for i in range(batch)]
+    c = Case([1 + i % 4 for i in range(batch)], lens, dtype=dtype, dim=dim, hq=hq, hkv=hkv,
+             window=window, seed=16)
+    assert_attention(*_attend(c), c.reference(), dtype)
+
+
 @pytest.mark.parametrize("dtype,dim,hq,hkv,page", [
     (BF16, 128, 8, 2, 16), (F16, 64, 12, 4, 32), (BF16, 64, 7, 1, 16), (F16, 128, 10, 2, 64),
     (BF16, 128, 4, 4, 128), (BF16, 128, 132, 1, 256)])
@@ -275,6 +287,28 @@ def test_selected_positions(dtype, dim, hq, hkv, page, index, k):
     assert_attention(out, lse, c.reference(indices=ind), dtype)
 
 
+@pytest.mark.parametrize("dtype,dim,hq,hkv", [(BF16, 128, 16, 8), (F16, 64, 16, 8),
+                                              (F16, 128, 160, 8), (BF16, 64, 8, 8)])
+@pytest.mark.parametrize("tokens", [30, 420])
+@pytest.mark.parametrize("k", [22, 130])
+def test_selected_positions_of_many_tokens(dtype, dim, hq, hkv, tokens, k):
+    # an item per team of warps, split and whole, and an item per warp
+    from dsa_b200.paged import selected_attention
+
+    c = Case([tokens - 7, 0, 7], [tokens + 100, 3, 500], dtype=dtype, dim=dim, hq=hq, hkv=hkv,
+             page=32, seed=21)
+    g = torch.Generator().manual_seed(k)
+    ind = torch.full((tokens, k), -1)
+    for t in range(tokens):
+        b = 0 if t < tokens - 7 else 2
+        n = int(torch.randint(0, k + 1, (1,), generator=g))
+        take = torch.randperm(c.lens[b], generator=g)[:n]
+        ind[t, :take.numel()] = take
+    out, lse = selected_attention(c.qd, c.cache, c.batch, ind.to("cuda", torch.int32),
+                                  return_lse=True)
+    assert_attention(out, lse, c.reference(indices=ind), dtype)
+
+
 def test_selected_lists_in_any_order_with_gaps_and_repeats():
     from dsa_b200.paged import selected_attention
 
@@ -446,6 +480,8 @@ def test_refusals():
             paged_attention(q, c.cache, c.batch, scale=scale)
     with pytest.raises(ValueError):
         paged_attention(q, c.cache, c.batch, out=torch.empty(3, 8, 128, dtype=BF16, device="cuda"))
+    with pytest.raises(ValueError):
+        paged_attention(q, c.cache, c.batch, out=q)
     ind = torch.zeros(2, 4, dtype=torch.int32, device="cuda")
     for bad in (ind[:1], ind.float(), ind[0], ind.cpu(), ind[:, :0], ind.t().contiguous().t()):
         with pytest.raises(ValueError):

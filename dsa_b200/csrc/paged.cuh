@@ -35,17 +35,19 @@ struct SeqSpan {
   int q0;   // first row of the sequence's new tokens
   int n;    // new tokens
   int len;  // positions with them, as far as the page table reaches
-  int told; // ... as the caller says
 };
 
 // The batch arrays come from the device, so every value is clamped to what its buffer holds; a
 // length that is none, or past the page table's end, is reported.
+__device__ __forceinline__ void load_rows(const PagedView& p, int b, int& q0, int& n) {
+  const int a = __ldg(p.starts + b), e = __ldg(p.starts + b + 1);
+  q0 = min(max(a, 0), p.tokens);
+  n = min(max(e, q0), p.tokens) - q0;
+}
 __device__ __forceinline__ SeqSpan load_span(const PagedView& p, int b) {
   SeqSpan s;
-  const int a = __ldg(p.starts + b), e = __ldg(p.starts + b + 1), l = __ldg(p.lengths + b);
-  s.q0 = min(max(a, 0), p.tokens);
-  s.n = min(max(e, s.q0), p.tokens) - s.q0;
-  s.told = l;
+  const int l = __ldg(p.lengths + b);
+  load_rows(p, b, s.q0, s.n);
   s.len = min(max(l, 0), p.max_pages << p.page_shift);  // the host bounds this product
   if (s.len != l) atomicOr(p.status, TDSA_STATUS_RANGE);
   return s;

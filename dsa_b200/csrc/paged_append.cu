@@ -43,7 +43,7 @@ struct AppendArgs {
 // anything is known about the token, so the loads from HBM run while its sequence, its page and
 // its angles are found (three dependent reads).
 //
-// HBM bound: 8698 tokens of 32 + 8 + 8 heads of 128 (214 MB) take 38 us, 5.6 TB/s, against the 33 us
+// HBM bound: 8698 tokens of 32 + 8 + 8 heads of 128 (214 MB) take 39 us, 5.5 TB/s, against the 33 us
 // that a copy of as many bytes takes; a few tokens take the time of the three reads, 3.1 us.
 template <bool kBF16, int D, int kPaThreads>
 __global__ void __launch_bounds__(kPaThreads, kPaThreads == kPaShort ? 5 : 9)
@@ -76,9 +76,11 @@ __global__ void __launch_bounds__(kPaThreads, kPaThreads == kPaShort ? 5 : 9)
   // the token's sequence: the one whose rows hold it
   bool found = false;
   for (int b = tid; b < a.p.batch; b += kPaThreads) {
-    const SeqSpan s = load_span(a.p, b);
-    if (t >= s.q0 && t < s.q0 + s.n) {
-      const int64_t pos = static_cast<int64_t>(s.told) - s.n + (t - s.q0);
+    int q0, n;
+    load_rows(a.p, b, q0, n);
+    const int len = __ldg(a.p.lengths + b);
+    if (t >= q0 && t < q0 + n) {
+      const int64_t pos = static_cast<int64_t>(len) - n + (t - q0);
       const bool in = pos >= 0 && (pos >> a.p.page_shift) < a.p.max_pages;
       s_pos = static_cast<int>(max(int64_t(-1), min(pos, int64_t(0x7FFFFFFF))));
       s_page = in ? __ldg(a.p.table + b * a.p.table_stride + (pos >> a.p.page_shift)) : -1;

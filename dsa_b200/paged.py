@@ -67,9 +67,10 @@ class PagedBatch:
     """The sequences of a call.  ``page_table`` int32 ``[batch, max_pages]``: position ``p`` of
     sequence ``b`` is row ``p % page_size`` of page ``page_table[b, p // page_size]``.
     ``query_starts`` int32 ``[batch + 1]`` and ``lengths`` int32 ``[batch]`` (positions with the
-    new tokens, which are the last ones).  The tensors may be rewritten in place between calls.
+    new tokens, which are the last ones).  The tensors may be rewritten in place between calls; other
+    tensors need a new batch.
     ``max_new``: the most new tokens a sequence has (default: no bound is known); it chooses
-    the kernel, results do not depend on it."""
+    the kernel, which changes results by rounding at most."""
 
     def __init__(self, page_table: torch.Tensor, query_starts: torch.Tensor,
                  lengths: torch.Tensor, *, max_new: int | None = None):
@@ -142,10 +143,10 @@ _WORKSPACES: dict[tuple[int, int, int], tuple[torch.Tensor, int, int]] = {}
 
 def paged_workspace(device: torch.device, head_dim: int,
                     stream: int | None = None) -> tuple[torch.Tensor, int, int]:
-    """Scratch of the attention calls, its counters zeroed -> (buffer, address, bytes).  Outside CUDA-graph
-    capture one buffer per (device, stream, head_dim) is kept: calls on one stream run in order
-    and each leaves it ready for the next.  During a capture a fresh one is returned, which the
-    graph keeps."""
+    """Scratch of the attention calls, its counters zeroed -> (buffer, address, bytes).  Outside
+    CUDA-graph capture one buffer per (device, stream, head_dim) is kept: calls on one stream run
+    in order and each leaves it ready for the next.  During a capture a fresh one is returned,
+    which the graph keeps."""
     if stream is None:
         stream = stream_ptr(device)
     key = (device.index, stream, head_dim)

@@ -601,8 +601,8 @@ int tdsa_query_prep(const void* qraw, int64_t qraw_stride, const void* hidden,
  * tokens are rows query_starts[b] .. query_starts[b + 1] - 1 of the packed [tokens] arrays
  * (ascending; rows outside every sequence are neither read nor written); lengths [batch]
  * device int32, positions of each sequence with its new tokens, which are its last ones.
- * max_new is the host's bound on a sequence's new tokens: it chooses a kernel, and results do
- * not depend on it.  max_pages * page_size <= 2^30.  Table entries are read only where a
+ * max_new is the host's bound on a sequence's new tokens: it chooses a kernel, which changes
+ * results by rounding at most.  max_pages * page_size <= 2^30.  Table entries are read only where a
  * position is needed; a page outside [0, pages) raises TDSA_STATUS_RANGE and its positions
  * count as absent, and so do positions past max_pages * page_size and a negative length's.
  */

@@ -197,9 +197,15 @@ __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
   asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
   return r;
 }
-__device__ __forceinline__ float max3(float a, float b, float c) {
+// Largest of three (two) values, NaN when one of them is.
+__device__ __forceinline__ float max3_nan(float a, float b, float c) {
   float r;
-  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+__device__ __forceinline__ float max2_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
   return r;
 }
 
@@ -573,13 +579,14 @@ __global__ void __launch_bounds__(kPcThreads, 1)
 #pragma unroll
           for (int c = 0; c < 4; ++c) {
             const uint32_t* x = s[c >> 1] + (c & 1) * 16;
-            tops[c] = max3(__uint_as_float(x[0]), __uint_as_float(x[1]), __uint_as_float(x[2]));
+            tops[c] =
+                max3_nan(__uint_as_float(x[0]), __uint_as_float(x[1]), __uint_as_float(x[2]));
 #pragma unroll
             for (int j = 3; j < 15; j += 2)
-              tops[c] = max3(tops[c], __uint_as_float(x[j]), __uint_as_float(x[j + 1]));
-            tops[c] = fmaxf(tops[c], __uint_as_float(x[15]));
+              tops[c] = max3_nan(tops[c], __uint_as_float(x[j]), __uint_as_float(x[j + 1]));
+            tops[c] = max2_nan(tops[c], __uint_as_float(x[15]));
           }
-          const float top = fmaxf(max3(tops[0], tops[1], tops[2]), tops[3]) * scale;
+          const float top = max2_nan(max3_nan(tops[0], tops[1], tops[2]), tops[3]) * scale;
           if (__any_sync(0xffffffffu, top > ref + 8.f)) {
             const float now = fmaxf(ref, top);
             const float f = now == ref ? 1.f : exp2_approx(ref - now);
@@ -601,7 +608,10 @@ __global__ void __launch_bounds__(kPcThreads, 1)
               }
             }
           }
-          const float neg = ref == -INFINITY ? 0.f : -ref;
+          // A score that is NaN or +infinity makes the whole row NaN: the polynomial below would
+          // drop it, so it is the reference that carries it into every weight of the part.
+          const float neg = !(top < INFINITY) ? __int_as_float(0x7FFFFFFF)
+                                              : (ref == -INFINITY ? 0.f : -ref);
           const uint64_t scale2 = pair(scale, scale), neg2 = pair(neg, neg);
           uint64_t part[2] = {0ull, 0ull};
           // a third of the pairs take the polynomial

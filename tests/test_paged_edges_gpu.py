@@ -1,0 +1,116 @@
+"""Paged cache on the GPU where it can go wrong: keys, queries and values that are not finite or
+huge, weights far below a row's largest, windows and lengths at the ends of their ranges, long
+chunks.  Against the float64 forms of _paged_util, whose bounds hold unless a test says more."""
+
+from __future__ import annotations
+
+import math
+
+import pytest
+import torch
+
+from tests._paged_util import ROUND, Case
+
+pytestmark = pytest.mark.gpu
+BF16, F16 = torch.bfloat16, torch.float16
+
+
+@pytest.fixture(scope="module", autouse=True)
+def _lib():
+    if not torch.cuda.is_available():
+        pytest.skip("needs a CUDA device")
+    from dsa_b200 import device_status
+    from dsa_b200.build import build
+
+    build()
+    device_status()
+    yield
+    assert device_status() == 0
+
+
+def _attend(c, **kw):
+    from dsa_b200.paged import paged_attention
+
+    return paged_attention(c.qd, c.cache, c.batch, window=c.window, return_lse=True, **kw)
+
+
+def _set(c, which, b, pos, head, feature, value):
+    """One number of the cache, in its pages and in the float64 copy."""
+    store, copy = (c.cache.keys, c.k) if which == "k" else (c.cache.values, c.v)
+    store[int(c.table[b, pos // c.page]), pos % c.page, head, feature] = value
+    copy[b][pos, head, feature] = value
+
+
+def _check(c, got, want, extra=0.0):
+    """Like assert_attention, where the reference's sums may be NaN or infinite: NaN has to be
+    NaN, infinity the same infinity, a log-sum-exp that is not finite any such number.  extra:
+    more room for the outputs."""
+    (out, lse), (ref, mag, ref_lse) = got, want
+    out, u = out.double().cpu(), ROUND[c.dtype]
+    lim = (u + 2.0 ** -12) * mag + u * (1 + u) * ref.abs() + 2.0 ** -24 + extra
+    fine = torch.isfinite(ref)
+    assert bool(((out - ref).abs() <= lim)[fine].all())
+    assert torch.equal(torch.isnan(out), torch.isnan(ref))
+    assert torch.equal(out[torch.isinf(ref)], ref[torch.isinf(ref)])
+    lse = lse.double().cpu()
+    empty, odd = ref_lse == -math.inf, torch.isnan(ref_lse) | (ref_lse == math.inf)
+    assert torch.equal(lse == -math.inf, empty)
+    assert not torch.isfinite(lse[odd]).any()
+    e = (lse - ref_lse)[~empty & ~odd].abs()
+    assert bool((e <= 2.0 ** -12 + 2.0 ** -22 * ref_lse[~empty & ~odd].abs()).all())
+
+
+# ------------------------------------------------------------------ scores that are not finite
+
+@pytest.mark.parametrize("dtype,dim", [(BF16, 128), (F16, 64)])
+@pytest.mark.parametrize("n", [1, 8, 40])
+@pytest.mark.parametrize("value", [math.nan, math.inf])
+def test_a_key_that_is_not_finite_reaches_the_rows_that_see_it(dtype, dim, n, value):
+    # at each of 32 consecutive positions, the last of which only some of the tokens see: a NaN
+    # or +inf score makes its row NaN, a score of -inf weighs nothing
+    c = Case([n, 2], [160, 30], dtype=dtype, dim=dim, seed=60)
+    for pos in range(160 - 16 - 32, 160 - 16) if n > 16 else range(100, 132):
+        was = float(c.k[0][pos, 1, 3])
+        _set(c, "k", 0, pos, 1, 3, value)
+        _check(c, _attend(c), c.reference())
+        _set(c, "k", 0, pos, 1, 3, was)
+
+
+@pytest.mark.parametrize("n", [1, 40])
+def test_a_key_that_is_not_finite_outside_the_window(n):
+    c = Case([n], [300], seed=61, window=33)
+    for pos in (5, 255, 259, 262, 264, 266, 280, 299):
+        was = float(c.k[0][pos, 0, 7])
+        _set(c, "k", 0, pos, 0, 7, math.nan)
+        _check(c, _attend(c), c.reference())
+        _set(c, "k", 0, pos, 0, 7, was)
+
+
+@pytest.mark.parametrize("n", [1, 40])
+@pytest.mark.parametrize("value", [math.nan, math.inf])
+def test_a_query_that_is_not_finite_stays_in_its_row(n, value):
+    c = Case([n, n], [200, 77], dtype=F16, seed=62)
+    c.q[n // 2, 3, 9] = value
+    c.qd = c.q.cuda()
+    _check(c, _attend(c), c.reference())
+
+
+@pytest.mark.parametrize("value", [math.nan, math.inf])
+def test_a_key_that_is_not_finite_in_a_split_sequence(value):
+    # many parts of one item, one of which holds it
+    c = Case([40], [3000], dim=64, hq=4, hkv=1, seed=63)
+    for pos in (2, 1025, 2990):
+        was = float(c.k[0][pos, 0, 0])
+        _set(c, "k", 0, pos, 0, 0, value)
+        _check(c, _attend(c), c.reference())
+        _set(c, "k", 0, pos, 0, 0, was)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("value", [math.nan, math.inf])
+def test_keys_that_are_not_finite_in_whole_items(dtype, value):
+    # items of one unit each, of which none is split: sequence b has it at position 50 + b
+    c = Case([40] * 36, [100] * 36, dtype=dtype, dim=64, hq=16, hkv=8, seed=75)
+    for b in range(36):
+        _set(c, "k", b, 50 + b, b % 8, 3, value)
+    _check(c, _attend(c), c.reference())

@@ -262,14 +262,16 @@ __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity,
   return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag));
 }
 
-// 2^x of two values on the fma pipe, for x well below 2^22; x below -126 is taken as -126, so a
-// key that a row does not see weighs 2^-126 instead of nothing (rows that see no key at all are
-// told by their maximum). x = n + f with n the nearest integer (read off the low bits of x + 1.5 2^23) and
-// |f| <= 1/2, 2^f by the degree-4 polynomial of least largest relative error (2.6e-6, found by
-// Remez exchange), n added to the exponent.
+// 2^x of two values on the fma pipe, for x well below 2^22. x = n + f with n the nearest integer
+// (read off the low bits of x + 1.5 2^23) and |f| <= 1/2, 2^f by the degree-4 polynomial of least
+// largest relative error (2.6e-6, found by Remez exchange), n added to the exponent. x below -127 is
+// taken as -127, whose sum of exponents is negative: the larger of it and 0 as integers makes the
+// weight of a key that a row does not see exactly 0, as the special-function pipe does, and between
+// -127 and -126 the result is some number below 2^-126. (A weight that stayed at 2^-126 would let
+// a value near the type's largest through.)
 __device__ __forceinline__ float2 exp2_poly2(uint64_t x2) {
   const float2 v = unpair(x2);
-  const uint64_t x = pair(fmaxf(v.x, -126.f), fmaxf(v.y, -126.f));
+  const uint64_t x = pair(fmaxf(v.x, -127.f), fmaxf(v.y, -127.f));
   const uint64_t magic = pair(12582912.f, 12582912.f);
   const uint64_t r = add2(x, magic);
   const uint64_t n = add2(r, pair(-12582912.f, -12582912.f));
@@ -279,8 +281,8 @@ __device__ __forceinline__ float2 exp2_poly2(uint64_t x2) {
   p = fma2(p, f, pair(0x1.62e0dcp-1f, 0x1.62e0dcp-1f));
   p = fma2(p, f, pair(0x1.ffffe8p-1f, 0x1.ffffe8p-1f));
   const float2 pv = unpair(p), rv = unpair(r);
-  return make_float2(__uint_as_float(__float_as_uint(pv.x) + (__float_as_uint(rv.x) << 23)),
-                     __uint_as_float(__float_as_uint(pv.y) + (__float_as_uint(rv.y) << 23)));
+  return make_float2(__int_as_float(max(__float_as_int(pv.x) + (__float_as_int(rv.x) << 23), 0)),
+                     __int_as_float(max(__float_as_int(pv.y) + (__float_as_int(rv.y) << 23), 0)));
 }
 
 // A segment of an item, published by the copy warp to the others.

@@ -114,3 +114,36 @@ def test_keys_that_are_not_finite_in_whole_items(dtype, value):
     for b in range(36):
         _set(c, "k", b, 50 + b, b % 8, 3, value)
     _check(c, _attend(c), c.reference())
+
+
+# ------------------------------------------------------------------ weights of nothing
+
+@pytest.mark.parametrize("n", [8, 40])
+def test_a_huge_value_reaches_only_the_tokens_that_see_it(n):
+    # the largest bfloat16 at each of the last positions: nothing of it in earlier tokens
+    c = Case([n], [160], seed=64)
+    clean = c.reference()
+    for pos in range(160 - min(n, 32), 160):
+        was = float(c.v[0][pos, 1, 5])
+        _set(c, "v", 0, pos, 1, 5, torch.finfo(BF16).max)
+        out, lse = _attend(c)
+        hidden = torch.arange(160 - n, 160) < pos
+        _check(c, (out[hidden.cuda()], lse[hidden.cuda()]), tuple(x[hidden] for x in clean))
+        _set(c, "v", 0, pos, 1, 5, was)
+
+
+@pytest.mark.parametrize("n", [1, 40])
+def test_a_weight_below_the_type_times_a_huge_value(n):
+    # scores 283 below the others': a weight of 2^-408 times the largest bfloat16 is nothing
+    c = Case([n], [200], dim=128, hq=2, hkv=1, seed=65)
+    c.q[..., 0] = 8.0
+    c.qd = c.q.cuda()
+    for pos in range(64, 96):
+        was = float(c.k[0][pos, 0, 0]), float(c.v[0][pos, 0, 2])
+        _set(c, "k", 0, pos, 0, 0, -400.0)
+        _set(c, "v", 0, pos, 0, 2, torch.finfo(BF16).max)
+        # the other scores' first products are up to 8 times a unit normal's
+        ref = c.reference()
+        _check(c, _attend(c), ref, extra=2.0 ** -9 * ref[1])
+        _set(c, "k", 0, pos, 0, 0, was[0])
+        _set(c, "v", 0, pos, 0, 2, was[1])

@@ -20,7 +20,7 @@
 // The products that one thread issues complete in order, so the completion of S(n + 1) also
 // says that O += P V of part n - 1 is done: the thread that owns a row waits for it before it
 // rescales its row of O in place, which it does only when the row's maximum has grown by a
-// factor of more than 2^8 of weight (rare after the first units).
+// factor of more than 2^8 of weight (2^4 in f16; rare after the first units).
 //
 // What bounds it.  A unit of both tiles is 2048 cycles of tensor work (2560 with S in parts of 64,
 // whose operands shared memory delivers in 48 cycles instead of 32) and 3600 cycles of the rows'
@@ -33,8 +33,9 @@
 // the card at its power limit, where the library product reaches 1.39.
 //
 // Scores, maxima, sums and O are float32.  P is rounded to the cache's type for the second
-// product (2^-8 relative in bf16, 2^-11 in f16, the rounding that the output gets too; a second
-// term for what it leaves would be half as much tensor work again); the sum adds the unrounded P.
+// product (2^-8 relative in bf16, 2^-11 in f16 or 2^-36 of the row's largest weight where that is
+// more: the rounding that the output gets too; a second term for what it leaves would be half as
+// much tensor work again); the sum adds the unrounded P.
 #include <algorithm>
 
 #include "paged.cuh"
@@ -301,6 +302,7 @@ __global__ void __launch_bounds__(kPcThreads, 1)
     paged_chunk_kernel(const __grid_constant__ CUtensorMap kmap,
                        const __grid_constant__ CUtensorMap vmap, const ChunkArgs a) {
   using C = ChunkCfg<D>;
+  constexpr float kGrow = WeightRange<kBF16>::kGrow, kBias = WeightRange<kBF16>::kBias;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>(
       (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -589,7 +591,7 @@ __global__ void __launch_bounds__(kPcThreads, 1)
             tops[c] = max2_nan(tops[c], __uint_as_float(x[15]));
           }
           const float top = max2_nan(max3_nan(tops[0], tops[1], tops[2]), tops[3]) * scale;
-          if (__any_sync(0xffffffffu, top > ref + 8.f)) {
+          if (__any_sync(0xffffffffu, top > ref + kGrow)) {
             const float now = fmaxf(ref, top);
             const float f = now == ref ? 1.f : exp2_approx(ref - now);
             ref = now;
@@ -613,7 +615,7 @@ __global__ void __launch_bounds__(kPcThreads, 1)
           // A score that is NaN or +infinity makes the whole row NaN: the polynomial below would
           // drop it, so it is the reference that carries it into every weight of the part.
           const float neg = !(top < INFINITY) ? __int_as_float(0x7FFFFFFF)
-                                              : (ref == -INFINITY ? 0.f : -ref);
+                                              : (ref == -INFINITY ? 0.f : kBias - ref);
           const uint64_t scale2 = pair(scale, scale), neg2 = pair(neg, neg);
           uint64_t part[2] = {0ull, 0ull};
           // a third of the pairs take the polynomial
@@ -794,7 +796,7 @@ __global__ void __launch_bounds__(kPcThreads, 1)
         if (valid && a.q.lse) {
           const int rl = sg->sub + r_item, tk = row_token(a.q, rl);
           a.q.lse[static_cast<int64_t>(sg->tok + tk) * a.q.heads + sg->head0 + rl - tk * g] =
-              none ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f;
+              none ? -INFINITY : (m - kBias + log2f(l)) * 0.6931471805599453f;
         }
       }
       tc_fence_before();

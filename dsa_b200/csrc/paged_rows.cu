@@ -24,8 +24,8 @@
 // instruction could not.
 //
 // Scores, maxima, sums and O are float32.  P enters the second product as a 16-bit value and a
-// second one that holds what its rounding left (2^-16 relative in bf16, 2^-22 in f16, below the
-// output's rounding): twice the products, which are not what bounds this kernel -- 161 us against
+// second one that holds what its rounding left (2^-16 relative in bf16; in f16 2^-22, or 2^-36 of
+// the row's largest weight where that is more): twice the products, which are not what bounds this kernel -- 161 us against
 // 160 with one term at 128 features, 149 against 142 at 64 -- for errors 0.7 times as large.
 //
 // Values of keys that no row of the item sees (past the length, or of a page that is not one)
@@ -125,6 +125,7 @@ __global__ void __launch_bounds__(kPrWarps * 32, RowsCfg<D, MT, kSel, kPrWarps>:
   constexpr int kTeam = kSolo ? 1 : kPrWarps;      // warps that share an item
   constexpr int kUnitTiles = kPrWarps / kTeam;     // tiles of a unit per warp
   constexpr int kRows = C::kRows, kStages = C::kStages;
+  constexpr float kGrow = WeightRange<kBF16>::kGrow, kBias = WeightRange<kBF16>::kBias;
   constexpr int kKs = D / 16;   // 16-wide steps of the head dimension
   constexpr int kNt = D / 8;    // 8-wide output tiles
   constexpr int kLanesPerRow = D / 8;
@@ -393,7 +394,7 @@ __global__ void __launch_bounds__(kPrWarps * 32, RowsCfg<D, MT, kSel, kPrWarps>:
             }
       }
       // running maximum: the reference moves only when a row's maximum has grown by more than
-      // a factor 2^8 of weight, so most tiles rescale nothing and P stays below 2^8
+      // a factor 2^kGrow of weight, so most tiles rescale nothing and P stays below 2^(kGrow + kBias)
       bool grow = false;
       float top[MT][2];
 #pragma unroll
@@ -405,7 +406,7 @@ __global__ void __launch_bounds__(kPrWarps * 32, RowsCfg<D, MT, kSel, kPrWarps>:
           t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 1));
           t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 2));
           top[m][e] = t * a.q.scale_log2;
-          grow |= top[m][e] > mx[m][e] + 8.f || (mx[m][e] == -INFINITY && top[m][e] > -INFINITY);
+          grow |= top[m][e] > mx[m][e] + kGrow || (mx[m][e] == -INFINITY && top[m][e] > -INFINITY);
         }
       if (__any_sync(0xffffffffu, grow)) {
 #pragma unroll
@@ -428,7 +429,7 @@ __global__ void __launch_bounds__(kPrWarps * 32, RowsCfg<D, MT, kSel, kPrWarps>:
       for (int m = 0; m < MT; ++m) {
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          const float ref = mx[m][e] == -INFINITY ? 0.f : mx[m][e];
+          const float ref = mx[m][e] == -INFINITY ? 0.f : mx[m][e] - kBias;
 #pragma unroll
           for (int n = 0; n < 2; ++n)
 #pragma unroll
@@ -576,7 +577,7 @@ __global__ void __launch_bounds__(kPrWarps * 32, RowsCfg<D, MT, kSel, kPrWarps>:
           *reinterpret_cast<uint2*>(a.q.out + t * a.q.o_ts + h * a.q.o_hs + col * 4) = w;
           if (a.q.lse && col == 0)
             a.q.lse[t * a.q.heads + h] =
-                l == 0.f ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f;
+                l == 0.f ? -INFINITY : (m - kBias + log2f(l)) * 0.6931471805599453f;
         } else {
           if (col == 0) a.part.ml[static_cast<int64_t>(slot) * kRows + r] = make_float2(m, l);
           *reinterpret_cast<float4*>(a.part.o + (static_cast<int64_t>(slot) * kRows + r) * D +

@@ -147,3 +147,56 @@ def test_a_weight_below_the_type_times_a_huge_value(n):
         _check(c, _attend(c), ref, extra=2.0 ** -9 * ref[1])
         _set(c, "k", 0, pos, 0, 0, was[0])
         _set(c, "v", 0, pos, 0, 2, was[1])
+
+
+# ------------------------------------------------------------------ a long tail of small weights
+
+def _sink(n, length, dtype, dim, gap, tail=0.0):
+    """One key ``gap`` above all the others with a value of zero, and values of 1 behind it."""
+    c = Case([n], [length], dtype=dtype, dim=dim, hq=4, hkv=1, page=64, seed=66)
+    c.q[..., 0], c.q[..., 1:] = math.sqrt(dim), c.q[..., 1:] * tail
+    c.qd = c.q.cuda()
+    keys, values = c.k[0], c.v[0]
+    keys[:, :, 0], keys[0, :, 0] = 0.0, gap
+    keys[:, :, 1:] *= tail
+    keys.copy_(keys.to(dtype).double())
+    values[:], values[0] = 1.0, 0.0
+    pages = c.table[0, :-(-length // 64)].long().cuda()
+    for store, rows in ((c.cache.keys, keys), (c.cache.values, values)):
+        room = torch.zeros(pages.numel() * 64, 1, dim, dtype=dtype)
+        room[:length] = rows.to(dtype)
+        store[pages] = room.view(-1, 64, 1, dim).cuda()
+    return c
+
+
+# 16-bit weights hold 2^-11 (or 2^-8) of themselves down to 2^-25 of the row's largest, and below
+# that, in float16, half of its smallest number, which stands for 2^-36 of the row's largest
+def _tail_room(c):
+    return 2.0 ** -36 * c.lens[0]
+
+
+@pytest.mark.parametrize("dtype,dim", [(F16, 64), (F16, 128), (BF16, 64)])
+@pytest.mark.parametrize("n", [1, 3, 40])
+@pytest.mark.parametrize("gap", [8.0, 13.9, 17.40625])
+def test_a_long_tail_of_small_weights_is_kept(dtype, dim, n, gap):
+    c = _sink(n, 20000 if n < 40 else 6000, dtype, dim, gap)
+    _check(c, _attend(c), c.reference(), extra=_tail_room(c))
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("n", [1, 40])
+def test_a_tail_of_many_weights_is_kept(dtype, n):
+    # scores that spread, so that a row's largest grows along the way
+    c = _sink(n, 6000, dtype, 64, 14.0, tail=0.6)
+    _check(c, _attend(c), c.reference(), extra=_tail_room(c))
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+def test_a_tail_of_selected_positions_is_kept(dtype):
+    from dsa_b200.paged import selected_attention
+
+    c = _sink(5, 4000, dtype, 64, 15.0)
+    ind = torch.stack([torch.randperm(4000, generator=torch.Generator().manual_seed(i))
+                       for i in range(5)])
+    got = selected_attention(c.qd, c.cache, c.batch, ind.cuda(), return_lse=True)
+    _check(c, got, c.reference(indices=ind), extra=_tail_room(c))

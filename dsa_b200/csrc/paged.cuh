@@ -100,13 +100,14 @@ __device__ __forceinline__ float exp2_approx(float x) {
 // A weight is held as 2^(x - ref + kBias), x the score and ref the running reference of its row (in
 // log2 units), which moves when a score exceeds it by more than kGrow.  The bias is in the sums,
 // the partials and the outputs alike and leaves with the division; a log-sum-exp takes it off.
-// bfloat16 has float32's exponents and needs none.  float16 would lose every weight below 2^-25 of
+// bfloat16 has float32's exponents, so no weight needs to be above 1, and with none above it a
+// value near the type's largest does not overflow a product.  float16 would lose every weight below 2^-25 of
 // the largest, which a long row has many of: with the bias the weights reach 2^15 of float16's
 // 2^16, those above 2^-25 of the reference's keep 11 bits, and a smaller one is off by no more than 2^-36.
 // A reference that moves at 2^4 instead of 2^8 is what makes the room.
 template <bool kBF16>
 struct WeightRange {
-  static constexpr float kGrow = kBF16 ? 8.f : 4.f, kBias = kBF16 ? 0.f : 11.f;
+  static constexpr float kGrow = kBF16 ? 8.f : 4.f, kBias = kBF16 ? -kGrow : 11.f;
 };
 
 // Slice of CTA c of `ctas` (at most `units`) over `units`, and the CTA whose slice holds unit u:

@@ -200,3 +200,20 @@ def test_a_tail_of_selected_positions_is_kept(dtype):
                        for i in range(5)])
     got = selected_attention(c.qd, c.cache, c.batch, ind.cuda(), return_lse=True)
     _check(c, got, c.reference(indices=ind), extra=_tail_room(c))
+
+
+@pytest.mark.parametrize("n", [1, 8, 40])
+def test_a_value_near_the_types_largest_does_not_overflow(n):
+    # half of a row's weight on the largest bfloat16: products with weights above 1 would be
+    # infinite
+    c = Case([n], [160], dim=64, hq=4, hkv=1, seed=76)
+    c.q[..., 0] = 8.0
+    c.qd = c.q.cuda()
+    for pos in (40, 50, 66, 83, 101, 118):
+        was = float(c.k[0][pos, 0, 0]), float(c.v[0][pos, 0, 2])
+        _set(c, "k", 0, pos, 0, 0, 5.0)
+        _set(c, "v", 0, pos, 0, 2, torch.finfo(BF16).max)
+        ref = c.reference()
+        _check(c, _attend(c), ref, extra=2.0 ** -9 * ref[1])  # scores 8 times a unit normal's
+        _set(c, "k", 0, pos, 0, 0, was[0])
+        _set(c, "v", 0, pos, 0, 2, was[1])

@@ -11,7 +11,8 @@ A cache is two page arrays ``[pages, page_size, kv_heads, head_dim]``; a batch n
 sequences of one call by a page table, the row ranges of their new tokens and their lengths.
 The new tokens of all sequences are packed: ``[tokens, heads, head_dim]``, sequence ``b`` in
 rows ``query_starts[b]`` to ``query_starts[b + 1] - 1``.  All kernels run on the current torch
-stream; the batch's tensors live on the device, and nothing here waits for it.
+stream of the current device, which has to be the cache's (``with torch.cuda.device(...)`` for
+another); the batch's tensors live on the device, and nothing here waits for it.
 """
 
 from __future__ import annotations
@@ -29,6 +30,9 @@ from .indexer import require_cuda, stream_ptr
 # torch.cuda.is_current_stream_capturing without its Python frame
 _capturing = getattr(torch._C, "_cuda_isCurrentStreamCapturing",
                      torch.cuda.is_current_stream_capturing)
+
+# and torch.cuda.current_device without its (0.1 us of a call of 9)
+_current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
 
 _DTYPES = {torch.float16: capi.TDSA_F16, torch.bfloat16: capi.TDSA_BF16}
 
@@ -105,6 +109,14 @@ class PagedBatch:
                 tokens if limit is None else min(limit, tokens)))
             self._last = (tokens, limit, ref)
         return ref
+
+
+def _refuse_device(cache: PagedKV, batch: PagedBatch) -> None:
+    """The library launches on the current device, and its status word is that device's."""
+    if batch._index != cache._index:
+        raise ValueError("batch and cache must be on one device")
+    raise ValueError(f"the cache is on cuda:{cache._index}, which is not the current device: make "
+                     "the call under torch.cuda.device(...)")
 
 
 class _Rows(threading.local):
@@ -198,8 +210,8 @@ class PagedAppender:
         ``positions`` int64 ``[tokens]`` replaces the tokens' positions in the angles."""
         cache = self.cache
         dtype, index, shape = cache.dtype, cache._index, k.shape
-        if batch._index != index:
-            raise ValueError("batch and cache must be on one device")
+        if batch._index != index or _current_device() != index:
+            _refuse_device(cache, batch)
         ks, vs = k.stride(), v.stride()
         if not (len(shape) == 3 and shape == v.shape and shape[1] == cache.kv_heads
                 and shape[2] == cache.head_dim and k.dtype is dtype and v.dtype is dtype
@@ -247,8 +259,8 @@ class PagedAppender:
 def _attention_args(q, cache, batch, out, return_lse):
     """Checks and descriptors shared by the attention calls."""
     shape, dtype, index = q.shape, cache.dtype, cache._index
-    if batch._index != index:
-        raise ValueError("batch and cache must be on one device")
+    if batch._index != index or _current_device() != index:
+        _refuse_device(cache, batch)
     if out is None:
         out = torch.empty_like(q)
     qs, os = q.stride(), out.stride()

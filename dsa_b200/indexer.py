@@ -314,5 +314,13 @@ class ScoreTopkPlan:
 
 
 def device_status(reset: bool = True) -> int:
-    """OR of error bits raised by kernels on the current device since the last reset."""
-    return capi.device_status(reset)
+    """OR of error bits raised by kernels on the current device since the last reset.
+
+    After a TDSA_ERR_TIMEOUT the paged attention's kept workspaces of the device are given up: a
+    call that ended early may have left counters in them that are not zero."""
+    status = capi.device_status(reset)
+    if status & capi.TDSA_ERR_TIMEOUT:
+        from .paged import release_paged_workspaces  # paged imports this module
+
+        release_paged_workspaces(torch.cuda.current_device())
+    return status

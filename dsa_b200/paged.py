@@ -161,6 +161,7 @@ def paged_workspace(device: torch.device, head_dim: int,
     which the graph keeps."""
     if stream is None:
         stream = stream_ptr(device)
+    # (a read of TDSA_ERR_TIMEOUT ends the buffers of its device: see device_status)
     key = (device.index, stream, head_dim)
     ws = _WORKSPACES.get(key)
     capturing = _capturing()
@@ -173,6 +174,13 @@ def paged_workspace(device: torch.device, head_dim: int,
         if not capturing:
             _WORKSPACES[key] = ws
     return ws
+
+
+def release_paged_workspaces(index: int | None = None) -> None:
+    """Forgets the kept workspaces of device ``index`` (default: of all): 20 to 39 MB for every
+    stream and head dimension in use, which the next call there allocates anew."""
+    for key in [k for k in _WORKSPACES if index is None or k[0] == index]:
+        _WORKSPACES.pop(key, None)
 
 
 class PagedAppender:

@@ -36,3 +36,23 @@ def test_a_batch_on_another_device_than_the_cache_is_refused(monkeypatch):
     monkeypatch.setattr(paged, "_current_device", lambda: 0)
     with pytest.raises(ValueError, match="one device"):
         paged.paged_attention(torch.zeros(1, 8, 128), _on(0)[0], _on(1)[1])
+
+
+@pytest.mark.parametrize("reset", [True, False])
+def test_a_timeout_ends_the_workspaces_of_its_device(monkeypatch, reset):
+    # a call that was cut off may leave its arrival counters above zero
+    from dsa_b200 import _capi as capi
+    from dsa_b200 import device_status
+
+    kept = {(0, 5, 64): "a", (0, 0, 128): "b", (1, 5, 64): "c"}
+    monkeypatch.setattr(paged, "_WORKSPACES", dict(kept))
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: 0)
+    status = capi.TDSA_STATUS_RANGE
+    monkeypatch.setattr(capi, "device_status", lambda r=True: status if r == reset else None)
+    assert device_status(reset) == status
+    assert paged._WORKSPACES == kept
+    status |= capi.TDSA_ERR_TIMEOUT
+    assert device_status(reset) == status
+    assert paged._WORKSPACES == {(1, 5, 64): "c"}
+    paged.release_paged_workspaces()
+    assert not paged._WORKSPACES

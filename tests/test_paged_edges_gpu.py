@@ -217,3 +217,24 @@ def test_a_value_near_the_types_largest_does_not_overflow(n):
         _check(c, _attend(c), ref, extra=2.0 ** -9 * ref[1])  # scores 8 times a unit normal's
         _set(c, "k", 0, pos, 0, 0, was[0])
         _set(c, "v", 0, pos, 0, 2, was[1])
+
+
+# ------------------------------------------------------------------ after a wait that ran out
+
+@pytest.mark.parametrize("n", [1, 40])
+def test_calls_after_a_timeout_do_not_find_its_counters(monkeypatch, n):
+    # arrival counters as a call that ended early may leave them, and the status that reports it
+    from dsa_b200 import _capi as capi
+    from dsa_b200 import device_status, paged
+
+    c = Case([n], [3000], dim=64, hq=4, hkv=1, seed=77)
+    _check(c, _attend(c), c.reference())
+    for buffer, _, _ in paged._WORKSPACES.values():
+        buffer[:capi.TDSA_PAGED_COUNTER_BYTES].view(torch.int32).fill_(999)
+    with monkeypatch.context() as m:
+        m.setattr(capi, "device_status", lambda reset=True: capi.TDSA_ERR_TIMEOUT)
+        assert device_status() == capi.TDSA_ERR_TIMEOUT
+    try:
+        _check(c, _attend(c, out=torch.full_like(c.qd, math.nan)), c.reference())
+    finally:
+        paged._WORKSPACES.clear()

@@ -1228,7 +1228,8 @@ int tdsa_paged_attention(const tdsa_paged_cache* cache, const tdsa_paged_batch* 
   rc = paged_query(cache, batch->tokens, q, q_heads, scale, out, lse, workspace, workspace_bytes, d);
   if (rc) return rc;
   if (window < 0) return fail(TDSA_ERR_INVALID, "window must be >= 0");
-  d.window = window;
+  // no table has more positions; position - window then stays within 32 bits
+  d.window = std::min(window, 1 << 30);
   int* status = device_status_ptr();
   if (!status) return fail(TDSA_ERR_CUDA, "device status word not available");
   p.status = status;

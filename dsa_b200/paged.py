@@ -283,6 +283,9 @@ def _attention_args(q, cache, batch, out, return_lse):
     return out, lse, shape, stream, paged_workspace(cache.device, cache.head_dim, stream)
 
 
+_ALL = 1 << 30  # positions that a page table can have: a window of so many is none
+
+
 def paged_attention(q: torch.Tensor, cache: PagedKV, batch: PagedBatch, *,
                     scale: float | None = None, window: int | None = None,
                     out: torch.Tensor | None = None, return_lse: bool = False):
@@ -295,13 +298,17 @@ def paged_attention(q: torch.Tensor, cache: PagedKV, batch: PagedBatch, *,
     A token that sees nothing gets zeros and ``-inf``.  The tokens must be in the cache already
     (``PagedAppender.append``).
     """
-    if window is not None and window < 1:
+    if window is None:
+        window = 0
+    elif window < 1:
         raise ValueError("window must be >= 1")
+    elif window > _ALL:  # before it is a C int
+        window = _ALL
     out, lse, shape, stream, ws = _attention_args(q, cache, batch, out, return_lse)
     rows = _ROWS.address
     rc = capi.lib().tdsa_paged_attention(
         cache._ref, batch._for(shape[0]), rows, shape[1],
-        cache._scale if scale is None else scale, window or 0, rows + 24,
+        cache._scale if scale is None else scale, window, rows + 24,
         None if lse is None else lse.data_ptr(), ws[1], ws[2], stream)
     if rc:
         capi.check(rc)

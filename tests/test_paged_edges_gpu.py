@@ -238,3 +238,37 @@ def test_calls_after_a_timeout_do_not_find_its_counters(monkeypatch, n):
         _check(c, _attend(c, out=torch.full_like(c.qd, math.nan)), c.reference())
     finally:
         paged._WORKSPACES.clear()
+
+
+# ------------------------------------------------------------------ ends of ranges
+
+@pytest.mark.parametrize("news,lens", [([1, 3], [300, 1]), ([40, 9], [300, 4])])
+@pytest.mark.parametrize("window", [2 ** 30, 2 ** 31 - 2, 2 ** 31 - 1, 2 ** 31, 2 ** 32,
+                                    2 ** 32 + 5, 2 ** 70])
+def test_a_window_past_every_position_is_none(news, lens, window):
+    # the second sequence has more new tokens than positions
+    c = Case(news, lens, seed=67)
+    c.window = window
+    got = _attend(c)
+    c.window = None
+    _check(c, got, c.reference())
+
+
+@pytest.mark.parametrize("n", [2, 9])
+def test_a_window_of_the_c_ints_range(n):
+    # the C entry's own range ends at 2^31 - 1
+    import ctypes as C
+
+    from dsa_b200 import _capi as capi
+    from dsa_b200.indexer import stream_ptr
+    from dsa_b200.paged import paged_workspace
+
+    c = Case([n], [1], seed=78)
+    out, lse = torch.zeros_like(c.qd), torch.zeros(n, 8, device="cuda")
+    rows = [capi.TdsaTokenRows(t.data_ptr(), *t.stride()[:2]) for t in (c.qd, out)]
+    ws = paged_workspace(c.cache.device, 128)
+    rc = capi.lib().tdsa_paged_attention(
+        c.cache._ref, c.batch._for(n), C.byref(rows[0]), 8, 128 ** -0.5, 2 ** 31 - 1,
+        C.byref(rows[1]), lse.data_ptr(), ws[1], ws[2], stream_ptr(c.cache.device))
+    assert rc == 0
+    _check(c, (out, lse), c.reference())

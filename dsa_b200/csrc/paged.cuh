@@ -35,6 +35,7 @@ struct SeqSpan {
   int q0;   // first row of the sequence's new tokens
   int n;    // new tokens
   int len;  // positions with them, as far as the page table reaches
+  int pos;  // position of the first new token, by the length as it stands
 };
 
 // The batch arrays come from the device, so every value is clamped to what its buffer holds; a
@@ -49,6 +50,7 @@ __device__ __forceinline__ SeqSpan load_span(const PagedView& p, int b) {
   const int l = __ldg(p.lengths + b);
   load_rows(p, b, s.q0, s.n);
   s.len = min(max(l, 0), p.max_pages << p.page_shift);  // the host bounds this product
+  s.pos = max(l, 0) - s.n;
   if (s.len != l) atomicOr(p.status, TDSA_STATUS_RANGE);
   return s;
 }
@@ -200,10 +202,10 @@ __device__ __forceinline__ void paged_range_item(const PagedQuery& q, const SeqS
   it.tok0 = s.q0;
   it.r0 = rt * kRows;
   it.rows = min(kRows, s.n * g - it.r0);
-  it.pos0 = s.len - s.n;
+  it.pos0 = s.pos;
   const int first = it.pos0 + it.r0 / g;
   const int last = it.pos0 + (it.r0 + it.rows - 1) / g;
-  it.k1 = max(0, last + 1);
+  it.k1 = min(max(0, last + 1), s.len);
   it.k0 = q.window > 0 ? max(0, first - (q.window - 1)) : 0;
   it.k0 = min(it.k0, it.k1);
   it.u0 = it.k0 / kUnit;

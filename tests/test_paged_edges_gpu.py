@@ -272,3 +272,27 @@ def test_a_window_of_the_c_ints_range(n):
         C.byref(rows[1]), lse.data_ptr(), ws[1], ws[2], stream_ptr(c.cache.device))
     assert rc == 0
     _check(c, (out, lse), c.reference())
+
+
+@pytest.mark.parametrize("n", [1, 7, 40])
+@pytest.mark.parametrize("window", [None, 38])
+@pytest.mark.parametrize("past", [1, 5, 2 ** 31 - 1 - 128])
+def test_a_length_past_the_page_table_keeps_the_tokens_positions(n, window, past):
+    # positions from the table's end on are absent; the tokens stay where the length puts them
+    from dsa_b200 import _capi as capi
+    from dsa_b200 import device_status
+
+    c = Case([n, 2], [96, 30], page=32, window=window, seed=68)
+    length = 128 + past  # the table reaches 128, of which the last page is not one of the cache's
+    c.batch.lengths[0] = length
+    got = _attend(c)
+    assert device_status() & capi.TDSA_STATUS_RANGE
+    rows = []
+    for b, (new, end) in enumerate(((n, length), (2, 30))):
+        for i in range(new):
+            pos = end - new + i
+            lo = 0 if window is None else max(0, pos - window + 1)
+            rows.append(list(range(min(lo, 96), min(pos + 1, 96))))
+    width = max(map(len, rows))
+    ind = torch.tensor([r + [-1] * (width - len(r)) for r in rows]).view(len(rows), width)
+    _check(c, got, c.reference(indices=ind))

@@ -82,7 +82,7 @@ __global__ void __launch_bounds__(kPaThreads, kPaThreads == kPaShort ? 5 : 9)
     if (t >= q0 && t < q0 + n) {
       const int64_t pos = static_cast<int64_t>(len) - n + (t - q0);
       const bool in = pos >= 0 && (pos >> a.p.page_shift) < a.p.max_pages;
-      s_pos = static_cast<int>(max(int64_t(-1), min(pos, int64_t(0x7FFFFFFF))));
+      s_pos = static_cast<int>(max(int64_t(-0x7FFFFFFF), pos));  // at most len - 1
       s_page = in ? __ldg(a.p.table + b * a.p.table_stride + (pos >> a.p.page_shift)) : -1;
       found = true;
     }

@@ -9,7 +9,7 @@ import math
 import pytest
 import torch
 
-from tests._paged_util import ROUND, Case
+from tests._paged_util import ROUND, Case, rotate
 
 pytestmark = pytest.mark.gpu
 BF16, F16 = torch.bfloat16, torch.float16
@@ -296,3 +296,21 @@ def test_a_length_past_the_page_table_keeps_the_tokens_positions(n, window, past
     width = max(map(len, rows))
     ind = torch.tensor([r + [-1] * (width - len(r)) for r in rows]).view(len(rows), width)
     _check(c, got, c.reference(indices=ind))
+
+
+def test_append_turns_queries_by_positions_before_the_first():
+    # more new tokens than positions: no slot for the first ones, but a position all the same
+    from dsa_b200 import _capi as capi
+    from dsa_b200 import device_status
+    from dsa_b200.paged import PagedAppender
+
+    c = Case([9, 1], [4, 20], hq=4, hkv=2, seed=69)
+    k = torch.randn(10, 2, 128, generator=torch.Generator().manual_seed(2)).to(BF16).cuda()
+    app = PagedAppender(c.cache, rope_dim=128)
+    got = app.append(c.batch, k, k, c.qd)
+    assert device_status() & capi.TDSA_STATUS_RANGE
+    pos = torch.cat((torch.arange(-5, 4), torch.tensor([19])))
+    want = rotate(c.q, pos, app.inv_freq.cpu(), False)
+    size = c.q.double().abs().amax(-1, keepdim=True)
+    err = (got.double().cpu() - want).abs()
+    assert bool((err <= ROUND[BF16] * want.abs() + 2.0 ** -19 * size + 2.0 ** -25).all())

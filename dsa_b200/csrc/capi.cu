@@ -1,5 +1,6 @@
 // extern "C" entry points of libtdsa: argument checks on the host, then the launchers.
 #include <algorithm>
+#include <cstdlib>
 #include <mutex>
 #include <string>
 #include <utility>
@@ -273,6 +274,45 @@ int check_token_rows(const tdsa_token_rows* r, int heads, int dim, const char* n
   return TDSA_OK;
 }
 
+// Whether rows of a (ha heads) and of b (hb heads) share memory, where that can be told: apart
+// from address ranges that do not meet, their strides have to be the same.  Strides are checked and not
+// negative.  self: a and b are one, and only different rows count.
+bool rows_overlap(const tdsa_token_rows* a, int ha, const tdsa_token_rows* b, int hb, int tokens,
+                  int dim, bool self) {
+  const int64_t ts = tokens > 1 ? a->token_stride : 0;
+  const int64_t hsa = ha > 1 ? a->head_stride : 0, hsb = hb > 1 ? b->head_stride : 0;
+  const int64_t tsb = tokens > 1 ? b->token_stride : 0, last = tokens - 1;
+  const int64_t from = (reinterpret_cast<intptr_t>(b->data) - reinterpret_cast<intptr_t>(a->data)) / 2;
+  const int64_t wide_a = (ha - 1) * hsa + dim, wide_b = (hb - 1) * hsb + dim;  // of one token
+  if (!self) {
+    if (from >= last * ts + wide_a || -from >= last * tsb + wide_b) return false;
+    if (ts != tsb || (ha > 1 && hb > 1 && hsa != hsb)) return false;  // not told
+    // parts of the same wider rows
+    const int64_t r = ts ? ((from % ts) + ts) % ts : 0;
+    if (ts && r >= wide_a && r + wide_b <= ts) return false;
+  } else if ((tokens == 1 || ts >= wide_a) && (ha == 1 || hsa >= dim)) {
+    return false;
+  }
+  // row (t, h) of b begins from + dt ts + dh hs after row (t - dt, h - dh) of a
+  const int64_t hs = ha > 1 ? hsa : hsb;
+  for (int64_t dh = self ? 0 : 1 - ha; dh < hb; ++dh) {
+    const int64_t x = from + dh * hs;
+    const int64_t q = ts ? -x / ts : 0;  // dt near q brings it nearest
+    for (int64_t dt = q - 1; dt <= q + 1; ++dt) {
+      const int64_t t = std::max(-last, std::min(last, dt));
+      if (self && dh == 0 && t == 0) continue;
+      if (std::abs(x + t * ts) < dim) return true;
+    }
+  }
+  return false;
+}
+
+int check_output_rows(const tdsa_token_rows* out, int heads, int tokens, int dim, const char* name) {
+  if (rows_overlap(out, heads, out, heads, tokens, dim, true))
+    return fail(TDSA_ERR_INVALID, std::string(name) + "'s rows overlap each other");
+  return TDSA_OK;
+}
+
 int paged_query(const tdsa_paged_cache* c, int tokens, const tdsa_token_rows* q, int q_heads,
                 float scale,
                 const tdsa_token_rows* out, float* lse, void* ws, size_t ws_bytes,
@@ -284,8 +324,14 @@ int paged_query(const tdsa_paged_cache* c, int tokens, const tdsa_token_rows* q,
   int rc = check_token_rows(q, q_heads, c->head_dim, "q");
   if (!rc) rc = check_token_rows(out, q_heads, c->head_dim, "out");
   if (rc) return rc;
-  if (q->data == out->data)
-    return fail(TDSA_ERR_INVALID, "out must not be q: a row may be read after others are written");
+  d.group = q_heads / c->kv_heads;
+  if (d.group > 1024)
+    return fail(TDSA_ERR_UNSUPPORTED, "at most 1024 query heads per key/value head");
+  if (q->data == out->data || rows_overlap(q, q_heads, out, q_heads, tokens, c->head_dim, false))
+    return fail(TDSA_ERR_INVALID,
+                "out must not overlap q: a row may be read after others are written");
+  rc = check_output_rows(out, q_heads, tokens, c->head_dim, "out");
+  if (rc) return rc;
   if (!(scale > 0.f) || scale > 1e30f)
     return fail(TDSA_ERR_INVALID, "scale must be positive and finite");
   if (!ws || ws_bytes < tdsa_paged_workspace_bytes(c->head_dim) ||
@@ -301,9 +347,6 @@ int paged_query(const tdsa_paged_cache* c, int tokens, const tdsa_token_rows* q,
   d.o_hs = out->head_stride;
   d.lse = lse;
   d.heads = q_heads;
-  d.group = q_heads / c->kv_heads;
-  if (d.group > 1024)
-    return fail(TDSA_ERR_UNSUPPORTED, "at most 1024 query heads per key/value head");
   d.group_magic = d.group > 1 ? static_cast<uint32_t>((uint64_t(1) << 32) / d.group + 1) : 0u;
   d.scale_log2 = scale * 1.4426950408889634f;
   d.window = 0;
@@ -1198,6 +1241,17 @@ int tdsa_paged_append(const tdsa_paged_cache* cache, const tdsa_paged_batch* bat
     if (q_heads < 1) return fail(TDSA_ERR_INVALID, "q_heads must be >= 1");
     rc = check_token_rows(q, q_heads, cache->head_dim, "q");
     if (!rc) rc = check_token_rows(q_out, q_heads, cache->head_dim, "q_out");
+    if (!rc) rc = check_output_rows(q_out, q_heads, batch->tokens, cache->head_dim, "q_out");
+    const auto meets = [&](const tdsa_token_rows* r, int heads) {
+      return rows_overlap(r, heads, q_out, q_heads, batch->tokens, cache->head_dim, false);
+    };
+    const bool in_place = !rc && q->data == q_out->data &&
+                          (batch->tokens == 1 || q->token_stride == q_out->token_stride) &&
+                          (q_heads == 1 || q->head_stride == q_out->head_stride);
+    if (!rc && !in_place && (q->data == q_out->data || meets(q, q_heads)))
+      return fail(TDSA_ERR_INVALID, "q_out must be q or not overlap it");
+    if (!rc && (meets(k, cache->kv_heads) || meets(v, cache->kv_heads)))
+      return fail(TDSA_ERR_INVALID, "q_out must not overlap k or v");
   }
   if (rc) return rc;
   int* status = device_status_ptr();

@@ -296,7 +296,7 @@ def paged_attention(q: torch.Tensor, cache: PagedKV, batch: PagedBatch, *,
     ``return_lse`` the float32 log-sum-exp ``[tokens, heads]``.  ``window``: a token sees only
     the last ``window`` positions up to its own.  ``scale`` defaults to ``head_dim ** -0.5``.
     A token that sees nothing gets zeros and ``-inf``.  The tokens must be in the cache already
-    (``PagedAppender.append``).
+    (``PagedAppender.append``).  ``out`` must not share memory with ``q``.
     """
     if window is None:
         window = 0

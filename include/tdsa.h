@@ -642,7 +642,8 @@ typedef struct tdsa_token_rows {
 
 /*
  * Writes the keys (rotated) and values of every new token into its slot of the cache and, when
- * q is not NULL, its rotated queries into q_out (which may be q).  The rotation turns the
+ * q is not NULL, its rotated queries into q_out (q itself with its strides, or rows that share no
+ * memory with q, k, v or each other; refused where that can be told, as below).  The rotation turns the
  * pairs of the leading rope_dim features (0, or a multiple of 16 up to head_dim), the halves'
  * j and j + rope_dim / 2 or, with interleaved != 0, neighbours 2 j and 2 j + 1, by the angle
  * position * inv_freq[j] (device float32 [rope_dim / 2]); positions (device int64 [tokens])
@@ -663,7 +664,8 @@ int tdsa_paged_append(const tdsa_paged_cache* cache, const tdsa_paged_batch* bat
  *   out[t][h] = sum_j softmax_j(scale * q[t][h] . K[j][h / g]) V[j][h / g],  g = q_heads /
  *   kv_heads;  lse[t][h] = log sum_j exp(scale * q . K[j]) (float32, [tokens][q_heads], NULL:
  *   not wanted).
- * A token that sees no key gets out 0 and lse -inf.  out must not overlap q.  float32 scores,
+ * A token that sees no key gets out 0 and lse -inf.  out's rows must not overlap q or each other;
+ * that is refused where both have the same strides (other pairs are not looked into).  float32 scores,
  * maxima and sums; in long chunks the softmax weights are rounded to the cache's type for the
  * product with V.  scale > 0.
  * workspace: tdsa_paged_workspace_bytes bytes, 256-byte aligned, its first

@@ -314,3 +314,29 @@ def test_append_turns_queries_by_positions_before_the_first():
     size = c.q.double().abs().amax(-1, keepdim=True)
     err = (got.double().cpu() - want).abs()
     assert bool((err <= ROUND[BF16] * want.abs() + 2.0 ** -19 * size + 2.0 ** -25).all())
+
+
+# ------------------------------------------------------------------ outputs beside their inputs
+
+@pytest.mark.parametrize("n", [1, 40])
+@pytest.mark.parametrize("way", ["heads", "features", "tokens", "head-major"])
+def test_outputs_in_the_same_buffer_as_queries(n, way):
+    # interleaved in every way, and nowhere the same memory
+    c = Case([n, 2], [90, 30], hq=8, hkv=2, seed=79)
+    t = c.tokens
+    if way == "heads":
+        room = torch.zeros(t, 16, 128, dtype=BF16, device="cuda")
+        q, out = room[:, :8], room[:, 8:]
+    elif way == "features":
+        room = torch.zeros(t, 8, 2, 128, dtype=BF16, device="cuda")
+        q, out = room[:, :, 0], room[:, :, 1]
+    elif way == "tokens":
+        room = torch.zeros(t, 2, 8, 128, dtype=BF16, device="cuda")
+        q, out = room[:, 1], room[:, 0]
+    else:
+        room = torch.zeros(8, 2, t, 128, dtype=BF16, device="cuda")
+        q, out = room[:, 0].transpose(0, 1), room[:, 1].transpose(0, 1)
+    q.copy_(c.qd)
+    c.qd = q
+    _check(c, _attend(c, out=out), c.reference())
+    assert torch.equal(q.cpu(), c.q)

@@ -340,3 +340,36 @@ def test_outputs_in_the_same_buffer_as_queries(n, way):
     c.qd = q
     _check(c, _attend(c, out=out), c.reference())
     assert torch.equal(q.cpu(), c.q)
+
+
+# ------------------------------------------------------------------ values that are not finite
+
+@pytest.mark.parametrize("dtype,dim", [(BF16, 128), (F16, 64), (F16, 128)])
+@pytest.mark.parametrize("n", [1, 8, 40])
+def test_an_infinite_value_is_infinite_where_it_is_seen(dtype, dim, n):
+    # +inf in one feature, -inf in another, both in a third: inf, -inf and NaN
+    c = Case([n, 3], [170, 40], dtype=dtype, dim=dim, seed=70)
+    for pos in (0, 17, 100, 135, 150, 160, 169):
+        _set(c, "v", 0, pos, 1, 5, math.inf)
+    for pos in (150, 168):
+        _set(c, "v", 0, pos, 1, 6, math.inf)
+    for pos in (3, 120, 140, 165):
+        _set(c, "v", 0, pos, 1, 9, -math.inf)
+    _set(c, "v", 0, 20, 0, 30, math.inf)
+    _set(c, "v", 0, 151, 0, 30, -math.inf)
+    _set(c, "v", 0, 155, 0, 31, math.nan)
+    _check(c, _attend(c), c.reference())
+
+
+@pytest.mark.parametrize("tokens", [3, 400])
+def test_an_infinite_value_among_selected_positions(tokens):
+    from dsa_b200.paged import selected_attention
+
+    c = Case([tokens], [450], hq=16, hkv=8, dim=64, seed=71)
+    for head in range(8):
+        _set(c, "v", 0, 7 * head + 30, head, 5, math.inf)
+        _set(c, "v", 0, 7 * head + 31, head, 5 + head, -math.inf)
+    g = torch.Generator().manual_seed(72)
+    ind = torch.stack([torch.randperm(450, generator=g)[:60] for _ in range(tokens)])
+    got = selected_attention(c.qd, c.cache, c.batch, ind.cuda(), return_lse=True)
+    _check(c, got, c.reference(indices=ind))

@@ -373,3 +373,54 @@ def test_an_infinite_value_among_selected_positions(tokens):
     ind = torch.stack([torch.randperm(450, generator=g)[:60] for _ in range(tokens)])
     got = selected_attention(c.qd, c.cache, c.batch, ind.cuda(), return_lse=True)
     _check(c, got, c.reference(indices=ind))
+
+
+# ------------------------------------------------------------------ long chunks
+
+def _torch_reference(c):
+    """Case.reference a head at a time for all tokens of a sequence, on the GPU in float64."""
+    g = c.hq // c.hkv
+    out = torch.zeros(c.tokens, c.hq, c.dim, dtype=torch.float64)
+    mag, lse = torch.zeros_like(out), torch.full((c.tokens, c.hq), -math.inf, dtype=torch.float64)
+    for b, (n, length) in enumerate(zip(c.news, c.lens)):
+        pos = torch.arange(length - n, length, device="cuda")[:, None]
+        j = torch.arange(length, device="cuda")
+        sees = (j <= pos) & c.there[b].cuda()
+        if c.window is not None:
+            sees &= j > pos - c.window
+        rows = slice(c.starts[b], c.starts[b] + n)
+        for h in range(c.hq):
+            k, v = c.k[b][:, h // g].cuda(), c.v[b][:, h // g].cuda()
+            z = (c.q[rows, h].double().cuda() @ k.T * c.dim ** -0.5).masked_fill(~sees, -math.inf)
+            w = torch.softmax(z, -1).nan_to_num(0.0)
+            out[rows, h], mag[rows, h] = (w @ v).cpu(), (w @ v.abs()).cpu()
+            lse[rows, h] = torch.logsumexp(z, -1).cpu()
+    return out, mag, lse
+
+
+@pytest.mark.parametrize("dtype,dim,hq,hkv,page", [
+    (BF16, 128, 8, 1, 16), (F16, 64, 8, 1, 64), (BF16, 64, 16, 8, 32), (F16, 128, 24, 8, 128)])
+@pytest.mark.parametrize("window", [None, 2500])
+@pytest.mark.parametrize("gone", [False, True])
+def test_chunks_over_long_sequences(dtype, dim, hq, hkv, page, window, gone):
+    # rings and rows of absent pages that wrap many times, split items, several items per CTA
+    from dsa_b200 import _capi as capi
+    from dsa_b200 import device_status
+
+    c = Case([300, 37, 513], [6001, 5200, 7003], dtype=dtype, dim=dim, hq=hq, hkv=hkv, page=page,
+             window=window, seed=73)
+    c.there = [torch.ones(n, dtype=torch.bool) for n in c.lens]
+    if gone:
+        for b, at in ((0, 4200), (0, 5990), (1, 3000), (2, 6480), (2, 6999)):
+            p = at // page
+            c.batch.page_table[b, p] = -1
+            c.there[b][p * page:(p + 1) * page] = False
+    got = _attend(c)
+    assert bool(device_status() & capi.TDSA_STATUS_RANGE) == gone
+    _check(c, got, _torch_reference(c))
+
+
+def test_many_long_items_of_two_tiles():
+    c = Case([700] * 6, [2100 + 97 * i for i in range(6)], dim=64, hq=32, hkv=4, page=64, seed=74)
+    c.there = [torch.ones(n, dtype=torch.bool) for n in c.lens]
+    _check(c, _attend(c), _torch_reference(c))

@@ -219,6 +219,9 @@ __global__ void __launch_bounds__(kPrWarps * 32, RowsCfg<D, MT, kSel, kPrWarps>:
   const uint32_t lm_vc = lane >> 4;
   bool bad = false;  // a position or page outside the cache was named
 
+  // The second term of P is p + second * (p rounded): what the rounding left, or, when a segment
+  // is formed again because that left something that is not finite (see there), the first once more.
+  float second = -1.f;
   for (int64_t u = u_begin; u < u_end;) {
     const int n_units = it.u1 - it.u0;
     const int seg = static_cast<int>(min(static_cast<int64_t>(n_units - off), u_end - u));
@@ -277,262 +280,259 @@ __global__ void __launch_bounds__(kPrWarps * 32, RowsCfg<D, MT, kSel, kPrWarps>:
       if (r < 0) bad = true;
       return r;
     };
+    int64_t row_now, row_next;
+    int raw2, entry2, raw3;  // of the pairs after row_next's
+    {
+      const int raw0 = load_raw(0), raw1 = load_raw(1);
+      raw2 = load_raw(2);
+      raw3 = load_raw(3);
+      const int e0 = load_entry(raw0), e1 = load_entry(raw1);
+      entry2 = load_entry(raw2);
+      row_now = to_row(raw0, e0);
+      row_next = to_row(raw1, e1);
+    }
+    int load_pair = 0;  // the pair of row_now
+    uint32_t valid_now = __ballot_sync(0xffffffffu, row_now >= 0);
+
+    // issue the copies of tile i of the segment (one group, empty past the end)
+    auto issue = [&](int i) {
+      if (i < n_tiles) {
+        const int pr = i >> 1;
+        if (pr != load_pair) {
+          load_pair = pr;
+          row_now = row_next;
+          row_next = to_row(raw2, entry2);
+          raw2 = raw3;
+          entry2 = load_entry(raw2);
+          raw3 = load_raw(pr + 3);
+          valid_now = __ballot_sync(0xffffffffu, row_now >= 0);
+        }
+        if (lane == 0) s_valid[i % kStages] = (valid_now >> ((i & 1) * 16)) & 0xFFFFu;
+        const uint32_t st = ring_u + (i % kStages) * C::kStageBytes;
+        const int chunk = lane % kLanesPerRow;
+#pragma unroll
+        for (int c = 0; c < kPrTile / kRowsPerCopy; ++c) {
+          const int r = c * kRowsPerCopy + lane / kLanesPerRow;
+          const int64_t row = __shfl_sync(0xffffffffu, row_now, (i & 1) * 16 + r);
+          const bool ok = row >= 0;
+          const int64_t at = (ok ? row : 0) + head_off + chunk * 8;
+          const uint32_t dst = st + r * C::kRowBytes + ((chunk ^ (r & 7)) << 4);
+          cp_async16_fill(dst, a.p.keys + at, ok);
+          cp_async16_fill(dst + C::kTileBytes, a.p.values + at, ok);
+        }
+      }
+      cp_async_commit();
+    };
+
+#pragma unroll
+    for (int i = 0; i < kStages - 1; ++i) issue(i);
+
+    // ------------------------------------------------------------ query fragments
+    uint32_t qf[MT][kKs][4];
+#pragma unroll
+    for (int m = 0; m < MT; ++m) {
+      const int ra = it.r0 + m * 16 + quad, rb = ra + 8;
+      const int lim = it.r0 + it.rows;
+      const int ta = kSel ? 0 : ra / g, tb = kSel ? 0 : rb / g;
+      const uint16_t* pa = a.q.q + static_cast<int64_t>(it.tok0 + ta) * a.q.q_ts +
+                           (it.head * g + ra - ta * g) * a.q.q_hs + ql * 2;
+      const uint16_t* pb = a.q.q + static_cast<int64_t>(it.tok0 + tb) * a.q.q_ts +
+                           (it.head * g + rb - tb * g) * a.q.q_hs + ql * 2;
+#pragma unroll
+      for (int k = 0; k < kKs; ++k) {
+        qf[m][k][0] = ra < lim ? *reinterpret_cast<const uint32_t*>(pa + k * 16) : 0u;
+        qf[m][k][1] = rb < lim ? *reinterpret_cast<const uint32_t*>(pb + k * 16) : 0u;
+        qf[m][k][2] = ra < lim ? *reinterpret_cast<const uint32_t*>(pa + k * 16 + 8) : 0u;
+        qf[m][k][3] = rb < lim ? *reinterpret_cast<const uint32_t*>(pb + k * 16 + 8) : 0u;
+      }
+    }
+    // ------------------------------------------------------------ the key loop
     float o[MT][kNt][4];
     float mx[MT][2], sum[MT][2];
-    // Once, and again with one term of P when that leaves something that is not finite (see the
-    // end): a segment whose values hold infinities or NaN takes twice the time, others 1 % more
-    // (32 ragged sequences 161 us against 160, 683 x 512 selected positions 39.8 against 39.2).
-    for (bool one_term = false;; one_term = true) {
-      int64_t row_now, row_next;
-      int raw2, entry2, raw3;  // of the pairs after row_next's
-      {
-        const int raw0 = load_raw(0), raw1 = load_raw(1);
-        raw2 = load_raw(2);
-        raw3 = load_raw(3);
-        const int e0 = load_entry(raw0), e1 = load_entry(raw1);
-        entry2 = load_entry(raw2);
-        row_now = to_row(raw0, e0);
-        row_next = to_row(raw1, e1);
-      }
-      int load_pair = 0;  // the pair of row_now
-      uint32_t valid_now = __ballot_sync(0xffffffffu, row_now >= 0);
-
-      // issue the copies of tile i of the segment (one group, empty past the end)
-      auto issue = [&](int i) {
-        if (i < n_tiles) {
-          const int pr = i >> 1;
-          if (pr != load_pair) {
-            load_pair = pr;
-            row_now = row_next;
-            row_next = to_row(raw2, entry2);
-            raw2 = raw3;
-            entry2 = load_entry(raw2);
-            raw3 = load_raw(pr + 3);
-            valid_now = __ballot_sync(0xffffffffu, row_now >= 0);
-          }
-          if (lane == 0) s_valid[i % kStages] = (valid_now >> ((i & 1) * 16)) & 0xFFFFu;
-          const uint32_t st = ring_u + (i % kStages) * C::kStageBytes;
-          const int chunk = lane % kLanesPerRow;
 #pragma unroll
-          for (int c = 0; c < kPrTile / kRowsPerCopy; ++c) {
-            const int r = c * kRowsPerCopy + lane / kLanesPerRow;
-            const int64_t row = __shfl_sync(0xffffffffu, row_now, (i & 1) * 16 + r);
-            const bool ok = row >= 0;
-            const int64_t at = (ok ? row : 0) + head_off + chunk * 8;
-            const uint32_t dst = st + r * C::kRowBytes + ((chunk ^ (r & 7)) << 4);
-            cp_async16_fill(dst, a.p.keys + at, ok);
-            cp_async16_fill(dst + C::kTileBytes, a.p.values + at, ok);
-          }
-        }
-        cp_async_commit();
-      };
-
+    for (int m = 0; m < MT; ++m) {
 #pragma unroll
-      for (int i = 0; i < kStages - 1; ++i) issue(i);
-
-      // ------------------------------------------------------------ query fragments
-      uint32_t qf[MT][kKs][4];
+      for (int n = 0; n < kNt; ++n)
 #pragma unroll
-      for (int m = 0; m < MT; ++m) {
-        const int ra = it.r0 + m * 16 + quad, rb = ra + 8;
-        const int lim = it.r0 + it.rows;
-        const int ta = kSel ? 0 : ra / g, tb = kSel ? 0 : rb / g;
-        const uint16_t* pa = a.q.q + static_cast<int64_t>(it.tok0 + ta) * a.q.q_ts +
-                             (it.head * g + ra - ta * g) * a.q.q_hs + ql * 2;
-        const uint16_t* pb = a.q.q + static_cast<int64_t>(it.tok0 + tb) * a.q.q_ts +
-                             (it.head * g + rb - tb * g) * a.q.q_hs + ql * 2;
+        for (int e = 0; e < 4; ++e) o[m][n][e] = 0.f;
+      mx[m][0] = mx[m][1] = -INFINITY;
+      sum[m][0] = sum[m][1] = 0.f;
+    }
+    for (int i = 0; i < n_tiles; ++i) {
+      issue(i + kStages - 1);
+      cp_async_wait<kStages - 1>();
+      __syncwarp();
+      const uint32_t st = ring_u + (i % kStages) * C::kStageBytes;
+      const uint32_t vmask = s_valid[i % kStages];
+      const int base = tile_base(i);
+      float s[MT][2][4];
 #pragma unroll
-        for (int k = 0; k < kKs; ++k) {
-          qf[m][k][0] = ra < lim ? *reinterpret_cast<const uint32_t*>(pa + k * 16) : 0u;
-          qf[m][k][1] = rb < lim ? *reinterpret_cast<const uint32_t*>(pb + k * 16) : 0u;
-          qf[m][k][2] = ra < lim ? *reinterpret_cast<const uint32_t*>(pa + k * 16 + 8) : 0u;
-          qf[m][k][3] = rb < lim ? *reinterpret_cast<const uint32_t*>(pb + k * 16 + 8) : 0u;
+      for (int m = 0; m < MT; ++m)
+#pragma unroll
+        for (int n = 0; n < 2; ++n)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) s[m][n][e] = 0.f;
+#pragma unroll
+      for (int k = 0; k < kKs; ++k) {
+        uint32_t b[4];
+        ldsm4(b, st + lm_k * C::kRowBytes + (((2 * k + lm_kc) ^ (lm_k & 7)) << 4));
+#pragma unroll
+        for (int m = 0; m < MT; ++m) {
+          mma16816<kBF16>(s[m][0], qf[m][k], b[0], b[1]);
+          mma16816<kBF16>(s[m][1], qf[m][k], b[2], b[3]);
         }
       }
-      // ------------------------------------------------------------ the key loop
-#pragma unroll
-      for (int m = 0; m < MT; ++m) {
-#pragma unroll
-        for (int n = 0; n < kNt; ++n)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) o[m][n][e] = 0.f;
-        mx[m][0] = mx[m][1] = -INFINITY;
-        sum[m][0] = sum[m][1] = 0.f;
-      }
-      for (int i = 0; i < n_tiles; ++i) {
-        issue(i + kStages - 1);
-        cp_async_wait<kStages - 1>();
-        __syncwarp();
-        const uint32_t st = ring_u + (i % kStages) * C::kStageBytes;
-        const uint32_t vmask = s_valid[i % kStages];
-        const int base = tile_base(i);
-        float s[MT][2][4];
+      const bool whole = vmask == 0xFFFFu && base >= all_lo && base + kPrTile <= all_hi;
+      if (!whole) {
 #pragma unroll
         for (int m = 0; m < MT; ++m)
 #pragma unroll
           for (int n = 0; n < 2; ++n)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) s[m][n][e] = 0.f;
+            for (int e = 0; e < 4; ++e) {
+              const int c = n * 8 + ql * 2 + (e & 1);
+              const bool see = ((vmask >> c) & 1u) && base + c >= lo[m][e >> 1] &&
+                               base + c < hi[m][e >> 1];
+              if (!see) s[m][n][e] = -INFINITY;
+            }
+      }
+      // running maximum: the reference moves only when a row's maximum has grown by more than
+      // a factor 2^kGrow of weight, so most tiles rescale nothing and P stays below
+      // 2^(kGrow + kBias)
+      bool grow = false;
+      float top[MT][2];
 #pragma unroll
-        for (int k = 0; k < kKs; ++k) {
-          uint32_t b[4];
-          ldsm4(b, st + lm_k * C::kRowBytes + (((2 * k + lm_kc) ^ (lm_k & 7)) << 4));
+      for (int m = 0; m < MT; ++m)
 #pragma unroll
-          for (int m = 0; m < MT; ++m) {
-            mma16816<kBF16>(s[m][0], qf[m][k], b[0], b[1]);
-            mma16816<kBF16>(s[m][1], qf[m][k], b[2], b[3]);
-          }
+        for (int e = 0; e < 2; ++e) {
+          float t = fmaxf(fmaxf(s[m][0][2 * e], s[m][0][2 * e + 1]),
+                          fmaxf(s[m][1][2 * e], s[m][1][2 * e + 1]));
+          t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 1));
+          t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 2));
+          top[m][e] = t * a.q.scale_log2;
+          grow |= top[m][e] > mx[m][e] + kGrow ||
+                  (mx[m][e] == -INFINITY && top[m][e] > -INFINITY);
         }
-        const bool whole = vmask == 0xFFFFu && base >= all_lo && base + kPrTile <= all_hi;
-        if (!whole) {
-#pragma unroll
-          for (int m = 0; m < MT; ++m)
-#pragma unroll
-            for (int n = 0; n < 2; ++n)
-#pragma unroll
-              for (int e = 0; e < 4; ++e) {
-                const int c = n * 8 + ql * 2 + (e & 1);
-                const bool see = ((vmask >> c) & 1u) && base + c >= lo[m][e >> 1] &&
-                                 base + c < hi[m][e >> 1];
-                if (!see) s[m][n][e] = -INFINITY;
-              }
-        }
-        // running maximum: the reference moves only when a row's maximum has grown by more than
-        // a factor 2^kGrow of weight, so most tiles rescale nothing and P stays below
-        // 2^(kGrow + kBias)
-        bool grow = false;
-        float top[MT][2];
+      if (__any_sync(0xffffffffu, grow)) {
 #pragma unroll
         for (int m = 0; m < MT; ++m)
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
-            float t = fmaxf(fmaxf(s[m][0][2 * e], s[m][0][2 * e + 1]),
-                            fmaxf(s[m][1][2 * e], s[m][1][2 * e + 1]));
-            t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 1));
-            t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 2));
-            top[m][e] = t * a.q.scale_log2;
-            grow |= top[m][e] > mx[m][e] + kGrow ||
-                    (mx[m][e] == -INFINITY && top[m][e] > -INFINITY);
-          }
-        if (__any_sync(0xffffffffu, grow)) {
+            const float now = fmaxf(mx[m][e], top[m][e]);
+            const float f = now == mx[m][e] ? 1.f : exp2_approx(mx[m][e] - now);
+            mx[m][e] = now;
+            sum[m][e] *= f;
 #pragma unroll
-          for (int m = 0; m < MT; ++m)
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-              const float now = fmaxf(mx[m][e], top[m][e]);
-              const float f = now == mx[m][e] ? 1.f : exp2_approx(mx[m][e] - now);
-              mx[m][e] = now;
-              sum[m][e] *= f;
-#pragma unroll
-              for (int n = 0; n < kNt; ++n) {
-                o[m][n][2 * e] *= f;
-                o[m][n][2 * e + 1] *= f;
-              }
-            }
-        }
-        uint32_t pf[MT][4], pl[MT][4];  // P rounded, and what the rounding left
-#pragma unroll
-        for (int m = 0; m < MT; ++m) {
-#pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            const float ref = mx[m][e] == -INFINITY ? 0.f : mx[m][e] - kBias;
-#pragma unroll
-            for (int n = 0; n < 2; ++n)
-#pragma unroll
-              for (int x = 0; x < 2; ++x) {
-                const float p = exp2_approx(fmaf(s[m][n][2 * e + x], a.q.scale_log2, -ref));
-                s[m][n][2 * e + x] = p;
-                sum[m][e] += p;
-              }
-          }
-#pragma unroll
-          for (int x = 0; x < 4; ++x) {
-            const float u = s[m][x >> 1][2 * (x & 1)], w = s[m][x >> 1][2 * (x & 1) + 1];
-            pf[m][x] = pack16<kBF16>(u, w);
-            const float2 r = unpack16<kBF16>(pf[m][x]);
-            pl[m][x] = one_term ? pf[m][x] : pack16<kBF16>(u - r.x, w - r.y);
-          }
-        }
-        const uint32_t sv = st + C::kTileBytes;
-        bool slow = false;
-        if (!kSel && !whole) {
-          // does a value that only some rows see break the product with zero weights?
-          for (int c = lane; c < kPrTile * kLanesPerRow; c += 32) {
-            uint32_t x[4];
-            asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];"
-                         : "=r"(x[0]), "=r"(x[1]), "=r"(x[2]), "=r"(x[3])
-                         : "r"(sv + c * 16)
-                         : "memory");
-            slow |= nonfinite16<kBF16>(x[0]) || nonfinite16<kBF16>(x[1]) ||
-                    nonfinite16<kBF16>(x[2]) || nonfinite16<kBF16>(x[3]);
-          }
-          slow = __any_sync(0xffffffffu, slow);
-        }
-        if (!slow) {
-#pragma unroll
-          for (int c = 0; c < kKs; ++c) {
-            uint32_t b[4];
-            ldsm4t(b, sv + lm_v * C::kRowBytes + (((2 * c + lm_vc) ^ (lm_v & 7)) << 4));
-#pragma unroll
-            for (int m = 0; m < MT; ++m) {
-              mma16816<kBF16>(o[m][2 * c], pf[m], b[0], b[1]);
-              mma16816<kBF16>(o[m][2 * c + 1], pf[m], b[2], b[3]);
-              mma16816<kBF16>(o[m][2 * c], pl[m], b[0], b[1]);
-              mma16816<kBF16>(o[m][2 * c + 1], pl[m], b[2], b[3]);
+            for (int n = 0; n < kNt; ++n) {
+              o[m][n][2 * e] *= f;
+              o[m][n][2 * e + 1] *= f;
             }
           }
-        } else {
-          // element by element, only the keys a row sees (with the weight of both terms)
-          const float w_all = one_term ? 2.f : 1.f;
+      }
+      uint32_t pf[MT][4], pl[MT][4];  // P rounded, and what the rounding left
 #pragma unroll
-          for (int n2 = 0; n2 < 2; ++n2)
+      for (int m = 0; m < MT; ++m) {
 #pragma unroll
-            for (int x = 0; x < 2; ++x)
-              for (int src = 0; src < 4; ++src) {
-                const int c = n2 * 8 + src * 2 + x;
-                const bool there = (vmask >> c) & 1u;
+        for (int e = 0; e < 2; ++e) {
+          const float ref = mx[m][e] == -INFINITY ? 0.f : mx[m][e] - kBias;
 #pragma unroll
-                for (int m = 0; m < MT; ++m) {
-                  const float pa = w_all * __shfl_sync(0xffffffffu, s[m][n2][x], (lane & ~3) | src);
-                  const float pb =
-                      w_all * __shfl_sync(0xffffffffu, s[m][n2][2 + x], (lane & ~3) | src);
-                  const bool va = there && base + c >= lo[m][0] && base + c < hi[m][0];
-                  const bool vb = there && base + c >= lo[m][1] && base + c < hi[m][1];
+          for (int n = 0; n < 2; ++n)
 #pragma unroll
-                  for (int n = 0; n < kNt; ++n) {
-                    uint32_t w;
-                    asm volatile("ld.shared.u32 %0, [%1];"
-                                 : "=r"(w)
-                                 : "r"(sv + c * C::kRowBytes + ((n ^ (c & 7)) << 4) + ql * 4)
-                                 : "memory");
-                    const float2 v = unpack16<kBF16>(w);
-                    if (va) {
-                      o[m][n][0] = fmaf(pa, v.x, o[m][n][0]);
-                      o[m][n][1] = fmaf(pa, v.y, o[m][n][1]);
-                    }
-                    if (vb) {
-                      o[m][n][2] = fmaf(pb, v.x, o[m][n][2]);
-                      o[m][n][3] = fmaf(pb, v.y, o[m][n][3]);
-                    }
+            for (int x = 0; x < 2; ++x) {
+              const float p = exp2_approx(fmaf(s[m][n][2 * e + x], a.q.scale_log2, -ref));
+              s[m][n][2 * e + x] = p;
+              sum[m][e] += p;
+            }
+        }
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+          const float u = s[m][x >> 1][2 * (x & 1)], w = s[m][x >> 1][2 * (x & 1) + 1];
+          pf[m][x] = pack16<kBF16>(u, w);
+          const float2 r = unpack16<kBF16>(pf[m][x]);
+          pl[m][x] = pack16<kBF16>(fmaf(second, r.x, u), fmaf(second, r.y, w));
+        }
+      }
+      const uint32_t sv = st + C::kTileBytes;
+      bool slow = false;
+      if (!kSel && !whole) {
+        // does a value that only some rows see break the product with zero weights?
+        for (int c = lane; c < kPrTile * kLanesPerRow; c += 32) {
+          uint32_t x[4];
+          asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];"
+                       : "=r"(x[0]), "=r"(x[1]), "=r"(x[2]), "=r"(x[3])
+                       : "r"(sv + c * 16)
+                       : "memory");
+          slow |= nonfinite16<kBF16>(x[0]) || nonfinite16<kBF16>(x[1]) ||
+                  nonfinite16<kBF16>(x[2]) || nonfinite16<kBF16>(x[3]);
+        }
+        slow = __any_sync(0xffffffffu, slow);
+      }
+      if (!slow) {
+#pragma unroll
+        for (int c = 0; c < kKs; ++c) {
+          uint32_t b[4];
+          ldsm4t(b, sv + lm_v * C::kRowBytes + (((2 * c + lm_vc) ^ (lm_v & 7)) << 4));
+#pragma unroll
+          for (int m = 0; m < MT; ++m) {
+            mma16816<kBF16>(o[m][2 * c], pf[m], b[0], b[1]);
+            mma16816<kBF16>(o[m][2 * c + 1], pf[m], b[2], b[3]);
+            mma16816<kBF16>(o[m][2 * c], pl[m], b[0], b[1]);
+            mma16816<kBF16>(o[m][2 * c + 1], pl[m], b[2], b[3]);
+          }
+        }
+      } else {
+        // element by element, only the keys a row sees, with the weight of both terms
+        const float w_all = 2.f + second;
+#pragma unroll
+        for (int n2 = 0; n2 < 2; ++n2)
+#pragma unroll
+          for (int x = 0; x < 2; ++x)
+            for (int src = 0; src < 4; ++src) {
+              const int c = n2 * 8 + src * 2 + x;
+              const bool there = (vmask >> c) & 1u;
+#pragma unroll
+              for (int m = 0; m < MT; ++m) {
+                const float pa = w_all * __shfl_sync(0xffffffffu, s[m][n2][x], (lane & ~3) | src);
+                const float pb =
+                    w_all * __shfl_sync(0xffffffffu, s[m][n2][2 + x], (lane & ~3) | src);
+                const bool va = there && base + c >= lo[m][0] && base + c < hi[m][0];
+                const bool vb = there && base + c >= lo[m][1] && base + c < hi[m][1];
+#pragma unroll
+                for (int n = 0; n < kNt; ++n) {
+                  uint32_t w;
+                  asm volatile("ld.shared.u32 %0, [%1];"
+                               : "=r"(w)
+                               : "r"(sv + c * C::kRowBytes + ((n ^ (c & 7)) << 4) + ql * 4)
+                               : "memory");
+                  const float2 v = unpack16<kBF16>(w);
+                  if (va) {
+                    o[m][n][0] = fmaf(pa, v.x, o[m][n][0]);
+                    o[m][n][1] = fmaf(pa, v.y, o[m][n][1]);
+                  }
+                  if (vb) {
+                    o[m][n][2] = fmaf(pb, v.x, o[m][n][2]);
+                    o[m][n][3] = fmaf(pb, v.y, o[m][n][3]);
                   }
                 }
               }
-        }
-        __syncwarp();  // every lane is done with the stage before the next copies into it
+            }
       }
-      cp_async_wait<0>();
-      __syncwarp();
-      // An infinite value times the second term, which is zero or negative as often as not, is NaN
-      // where the average is infinite.  Twice the first term is right, and is halved here.
-      if (one_term) {
+      __syncwarp();  // every lane is done with the stage before the next copies into it
+    }
+    cp_async_wait<0>();
+    __syncwarp();
+    // An infinite value times what the rounding left, which is zero or negative as often as not, is
+    // NaN where the average is infinite.  Twice the first term is right, and is halved here.  A warp
+    // goes back alone: nothing up to here waits for other warps.  Segments whose output is finite pay
+    // for the look at it (one sequence of 32768 positions 36.8 us against 36.4).
+    if (second == 0.f) {
 #pragma unroll
-        for (int m = 0; m < MT; ++m)
+      for (int m = 0; m < MT; ++m)
 #pragma unroll
-          for (int n = 0; n < kNt; ++n)
+        for (int n = 0; n < kNt; ++n)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) o[m][n][e] *= 0.5f;
-        break;
-      }
+          for (int e = 0; e < 4; ++e) o[m][n][e] *= 0.5f;
+    } else {
       float odd[4] = {0.f, 0.f, 0.f, 0.f};  // stays 0 when all are finite
 #pragma unroll
       for (int m = 0; m < MT; ++m)
@@ -540,8 +540,12 @@ __global__ void __launch_bounds__(kPrWarps * 32, RowsCfg<D, MT, kSel, kPrWarps>:
         for (int n = 0; n < kNt; ++n)
 #pragma unroll
           for (int e = 0; e < 4; ++e) odd[e] = fmaf(o[m][n][e], 0.f, odd[e]);
-      if (!__any_sync(0xffffffffu, odd[0] + odd[1] + odd[2] + odd[3] != 0.f)) break;
+      if (__any_sync(0xffffffffu, odd[0] + odd[1] + odd[2] + odd[3] != 0.f)) {
+        second = 0.f;
+        continue;
+      }
     }
+    second = -1.f;
 
     // ------------------------------------------------------------ the warps' results meet
     float* wo = reinterpret_cast<float*>(ring);

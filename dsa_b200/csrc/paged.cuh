@@ -99,6 +99,22 @@ __device__ __forceinline__ float exp2_approx(float x) {
   return y;
 }
 
+// Two float32 in a register pair, and a * b + c of both in one issue slot.
+__device__ __forceinline__ uint64_t pair(float lo, float hi) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+  return r;
+}
+__device__ __forceinline__ float2 unpair(uint64_t v) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+  return r;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
 // A weight is held as 2^(x - ref + kBias), x the score and ref the running reference of its row (in
 // log2 units), which moves when a score exceeds it by more than kGrow.  The bias is in the sums,
 // the partials and the outputs alike and leaves with the division; a log-sum-exp takes it off.

@@ -8,10 +8,12 @@
 // read from the cache once.
 //
 // HBM bound: a key and its value are 4 D bytes for 4 D rows multiply-adds.  32 ragged sequences
-// (979 MB) take 161 us, 6.1 TB/s of the 6.55 that a copy reaches; 2048 selected positions for 64
-// sequences (537 MB in pieces of 256 bytes) 95 us, 5.7 TB/s; one sequence of 32768 positions (134
-// MB) 36 us, 9 of them before the first tile is there and after the last, and the slowest SM a
-// third later than the fastest.
+// (979 MB) take 161 to 171 us from one card to another, 6.1 to 5.7 TB/s of the 6.55 that a copy
+// reaches; 2048 selected positions for 64 sequences (537 MB in pieces of 256 bytes) 93 to 98 us,
+// 5.8 to 5.5 TB/s; one sequence of 32768 positions (134 MB) 37 us, 9 of them before the first tile is
+// there and after the last, and the slowest SM a third later than the fastest.  17 to 32 rows (16
+// sequences of 8192, 537 MB) take 127 us at 128 features, 4.2 TB/s, and 90 at 64, 3.0 TB/s: the
+// instructions of two row tiles a key tile no longer hide behind the loads.
 //
 // Layout.  A CTA is four or eight warps.  Each warp runs its own stream of 16-key tiles (a unit is
 // a tile per warp) with its own ring of tiles in shared memory, filled by 16-byte asynchronous
@@ -25,8 +27,9 @@
 //
 // Scores, maxima, sums and O are float32.  P enters the second product as a 16-bit value and a
 // second one that holds what its rounding left (2^-16 relative in bf16; in f16 2^-22, or 2^-36 of
-// the row's largest weight where that is more): twice the products, which are not what bounds this kernel -- 161 us against
-// 160 with one term at 128 features, 149 against 142 at 64 -- for errors 0.7 times as large.
+// the row's largest weight where that is more): twice the products, which are not what bounds this
+// kernel -- 161 us against 160 with one term at 128 features, 149 against 142 at 64 -- for errors
+// 0.7 times as large.
 //
 // Values of keys that no row of the item sees (past the length, or of a page that is not one)
 // are zero-filled on arrival.  In a tile that some rows see and others do not, a value that is
@@ -50,7 +53,7 @@ struct RowsArgs {
   int* status;
 };
 
-template <int D, int MT, bool kSel, int kWarps>
+template <int D, int MT, bool kSel, int kWarps, bool kSolo = false>
 struct RowsCfg {
   static constexpr int kRowBytes = D * 2;
   static constexpr int kTileBytes = kPrTile * kRowBytes;       // K or V tile
@@ -66,7 +69,13 @@ struct RowsCfg {
   static constexpr int kMergeO = kRows * D * 4;                // a warp's output, float32
   static constexpr int kRing = kWarps * kWarpBytes;
   static constexpr int kMl = kWarps * kRows * 8;
-  static constexpr int kSmem = kRing + kMl + 256 + kWarps * kStages * 4;
+  // Queries are in registers where they fit beside the output.  32 rows of 128 features do not, and
+  // a team reads them from shared memory for every tile (16 sequences of 8192, 4 tokens x 8 heads per
+  // group: 127 us, 161 to 168 with registers that spill 370 bytes).
+  static constexpr bool kQShared = MT == 2 && D == 128 && !kSolo;
+  static constexpr int kQ = (kRing + kMl + 256 + kWarps * kStages * 4 + 127) / 128 * 128;
+  static constexpr int kSmem =
+      kQShared ? kQ + kRows * kRowBytes : kRing + kMl + 256 + kWarps * kStages * 4;
   static_assert(kMergeO <= kWarpBytes, "a warp's output fits its ring");
 };
 
@@ -116,9 +125,9 @@ __device__ __forceinline__ void cp_async_wait() {
 // kSolo (selected attention): a warp takes items of its own instead of a quarter of the CTA's, so
 // that nothing waits for the other warps where items are short and many.
 template <bool kBF16, int D, int MT, bool kSel, bool kSolo, int kPrWarps>
-__global__ void __launch_bounds__(kPrWarps * 32, RowsCfg<D, MT, kSel, kPrWarps>::kCtas)
+__global__ void __launch_bounds__(kPrWarps * 32, RowsCfg<D, MT, kSel, kPrWarps, kSolo>::kCtas)
     paged_rows_kernel(const RowsArgs a) {
-  using C = RowsCfg<D, MT, kSel, kPrWarps>;
+  using C = RowsCfg<D, MT, kSel, kPrWarps, kSolo>;
   constexpr int kPrThreads = kPrWarps * 32;
   constexpr int kPrUnit = kPrWarps * kPrTile;      // keys per unit of work
   static_assert(kSel || !kSolo, "");
@@ -219,8 +228,8 @@ __global__ void __launch_bounds__(kPrWarps * 32, RowsCfg<D, MT, kSel, kPrWarps>:
   const uint32_t lm_vc = lane >> 4;
   bool bad = false;  // a position or page outside the cache was named
 
-  // The second term of P is p + second * (p rounded): what the rounding left, or, when a segment
-  // is formed again because that left something that is not finite (see there), the first once more.
+  // The second term of P is p + second * (p rounded): what the rounding left, or the first once
+  // more when a segment is formed again because its output was not finite (see there).
   float second = -1.f;
   for (int64_t u = u_begin; u < u_end;) {
     const int n_units = it.u1 - it.u0;
@@ -328,22 +337,37 @@ __global__ void __launch_bounds__(kPrWarps * 32, RowsCfg<D, MT, kSel, kPrWarps>:
     for (int i = 0; i < kStages - 1; ++i) issue(i);
 
     // ------------------------------------------------------------ query fragments
-    uint32_t qf[MT][kKs][4];
+    uint32_t qf[C::kQShared ? 1 : MT][C::kQShared ? 1 : kKs][4];
+    const uint32_t s_q = smem_u32(smem + C::kQ);
+    if (C::kQShared) {
+      if (second != 0.f) {  // a warp that goes over its segment again finds them there
+        for (int x = tid; x < kRows * kLanesPerRow; x += kPrThreads) {
+          const int r = x / kLanesPerRow, c = x % kLanesPerRow;
+          const int rr = it.r0 + r, tk = kSel ? 0 : rr / g;
+          const uint16_t* from = a.q.q + static_cast<int64_t>(it.tok0 + tk) * a.q.q_ts +
+                                 (it.head * g + rr - tk * g) * a.q.q_hs + c * 8;
+          *reinterpret_cast<uint4*>(smem + C::kQ + r * C::kRowBytes + ((c ^ (r & 7)) << 4)) =
+              r < it.rows ? *reinterpret_cast<const uint4*>(from) : make_uint4(0u, 0u, 0u, 0u);
+        }
+        __syncthreads();
+      }
+    } else {
 #pragma unroll
-    for (int m = 0; m < MT; ++m) {
-      const int ra = it.r0 + m * 16 + quad, rb = ra + 8;
-      const int lim = it.r0 + it.rows;
-      const int ta = kSel ? 0 : ra / g, tb = kSel ? 0 : rb / g;
-      const uint16_t* pa = a.q.q + static_cast<int64_t>(it.tok0 + ta) * a.q.q_ts +
-                           (it.head * g + ra - ta * g) * a.q.q_hs + ql * 2;
-      const uint16_t* pb = a.q.q + static_cast<int64_t>(it.tok0 + tb) * a.q.q_ts +
-                           (it.head * g + rb - tb * g) * a.q.q_hs + ql * 2;
+      for (int m = 0; m < MT; ++m) {
+        const int ra = it.r0 + m * 16 + quad, rb = ra + 8;
+        const int lim = it.r0 + it.rows;
+        const int ta = kSel ? 0 : ra / g, tb = kSel ? 0 : rb / g;
+        const uint16_t* pa = a.q.q + static_cast<int64_t>(it.tok0 + ta) * a.q.q_ts +
+                             (it.head * g + ra - ta * g) * a.q.q_hs + ql * 2;
+        const uint16_t* pb = a.q.q + static_cast<int64_t>(it.tok0 + tb) * a.q.q_ts +
+                             (it.head * g + rb - tb * g) * a.q.q_hs + ql * 2;
 #pragma unroll
-      for (int k = 0; k < kKs; ++k) {
-        qf[m][k][0] = ra < lim ? *reinterpret_cast<const uint32_t*>(pa + k * 16) : 0u;
-        qf[m][k][1] = rb < lim ? *reinterpret_cast<const uint32_t*>(pb + k * 16) : 0u;
-        qf[m][k][2] = ra < lim ? *reinterpret_cast<const uint32_t*>(pa + k * 16 + 8) : 0u;
-        qf[m][k][3] = rb < lim ? *reinterpret_cast<const uint32_t*>(pb + k * 16 + 8) : 0u;
+        for (int k = 0; k < kKs; ++k) {
+          qf[m][k][0] = ra < lim ? *reinterpret_cast<const uint32_t*>(pa + k * 16) : 0u;
+          qf[m][k][1] = rb < lim ? *reinterpret_cast<const uint32_t*>(pb + k * 16) : 0u;
+          qf[m][k][2] = ra < lim ? *reinterpret_cast<const uint32_t*>(pa + k * 16 + 8) : 0u;
+          qf[m][k][3] = rb < lim ? *reinterpret_cast<const uint32_t*>(pb + k * 16 + 8) : 0u;
+        }
       }
     }
     // ------------------------------------------------------------ the key loop
@@ -378,8 +402,12 @@ __global__ void __launch_bounds__(kPrWarps * 32, RowsCfg<D, MT, kSel, kPrWarps>:
         ldsm4(b, st + lm_k * C::kRowBytes + (((2 * k + lm_kc) ^ (lm_k & 7)) << 4));
 #pragma unroll
         for (int m = 0; m < MT; ++m) {
-          mma16816<kBF16>(s[m][0], qf[m][k], b[0], b[1]);
-          mma16816<kBF16>(s[m][1], qf[m][k], b[2], b[3]);
+          uint32_t qs[4];
+          if (C::kQShared)
+            ldsm4(qs, s_q + (m * 16 + lm_v) * C::kRowBytes + (((2 * k + lm_vc) ^ (lm_v & 7)) << 4));
+          const uint32_t(&qa)[4] = C::kQShared ? qs : qf[C::kQShared ? 0 : m][C::kQShared ? 0 : k];
+          mma16816<kBF16>(s[m][0], qa, b[0], b[1]);
+          mma16816<kBF16>(s[m][1], qa, b[2], b[3]);
         }
       }
       const bool whole = vmask == 0xFFFFu && base >= all_lo && base + kPrTile <= all_hi;
@@ -521,10 +549,11 @@ __global__ void __launch_bounds__(kPrWarps * 32, RowsCfg<D, MT, kSel, kPrWarps>:
     }
     cp_async_wait<0>();
     __syncwarp();
-    // An infinite value times what the rounding left, which is zero or negative as often as not, is
-    // NaN where the average is infinite.  Twice the first term is right, and is halved here.  A warp
-    // goes back alone: nothing up to here waits for other warps.  Segments whose output is finite pay
-    // for the look at it (one sequence of 32768 positions 36.8 us against 36.4).
+    // An infinite value times what the rounding left, which is zero or negative as often as not,
+    // is NaN where the average is infinite.  Twice the first term is right, and is halved here.  A
+    // warp goes back alone: the second time nothing up to here waits for other warps.  Segments
+    // whose output is finite pay for the look at it (one sequence of 32768 positions 36.8 us
+    // against 36.4).
     if (second == 0.f) {
 #pragma unroll
       for (int m = 0; m < MT; ++m)
@@ -533,14 +562,18 @@ __global__ void __launch_bounds__(kPrWarps * 32, RowsCfg<D, MT, kSel, kPrWarps>:
 #pragma unroll
           for (int e = 0; e < 4; ++e) o[m][n][e] *= 0.5f;
     } else {
-      float odd[4] = {0.f, 0.f, 0.f, 0.f};  // stays 0 when all are finite
+      uint64_t zero[2] = {0ull, 0ull};  // stays that when all are finite
 #pragma unroll
       for (int m = 0; m < MT; ++m)
 #pragma unroll
-        for (int n = 0; n < kNt; ++n)
+        for (int e = 0; e < 2; ++e)
+          if (m * 16 + 8 * e < it.rows) {
 #pragma unroll
-          for (int e = 0; e < 4; ++e) odd[e] = fmaf(o[m][n][e], 0.f, odd[e]);
-      if (__any_sync(0xffffffffu, odd[0] + odd[1] + odd[2] + odd[3] != 0.f)) {
+            for (int n = 0; n < kNt; ++n)
+              zero[n & 1] = fma2(pair(o[m][n][2 * e], o[m][n][2 * e + 1]), 0ull, zero[n & 1]);
+          }
+      const float2 z0 = unpair(zero[0]), z1 = unpair(zero[1]);
+      if (__any_sync(0xffffffffu, z0.x + z0.y + z1.x + z1.y != 0.f)) {
         second = 0.f;
         continue;
       }
@@ -729,7 +762,7 @@ __global__ void __launch_bounds__(kPrWarps * 32, RowsCfg<D, MT, kSel, kPrWarps>:
 
 template <bool kBF16, int D, int MT, bool kSel, bool kSolo, int kWarps>
 int launch_rows_t(RowsArgs a, void* ws, cudaStream_t stream) {
-  using C = RowsCfg<D, MT, kSel, kWarps>;
+  using C = RowsCfg<D, MT, kSel, kWarps, kSolo>;
   const int ctas = C::kCtas * device_sm_count(current_device());
   a.part = paged_partials(ws, ctas * (kSolo ? kWarps : 1), C::kRows);
   auto kern = paged_rows_kernel<kBF16, D, MT, kSel, kSolo, kWarps>;

@@ -287,7 +287,7 @@ __global__ void __launch_bounds__(kPcThreads, 1)
     paged_chunk_kernel(const __grid_constant__ CUtensorMap kmap,
                        const __grid_constant__ CUtensorMap vmap, const ChunkArgs a) {
   using C = ChunkCfg<D>;
-  constexpr float kGrow = WeightRange<kBF16>::kGrow, kBias = WeightRange<kBF16>::kBias;
+  constexpr float kTop = WeightRange<kBF16>::kTop, kBias = WeightRange<kBF16>::kBias;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>(
       (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -576,8 +576,8 @@ __global__ void __launch_bounds__(kPcThreads, 1)
             tops[c] = max2_nan(tops[c], __uint_as_float(x[15]));
           }
           const float top = max2_nan(max3_nan(tops[0], tops[1], tops[2]), tops[3]) * scale;
-          if (__any_sync(0xffffffffu, top > ref + kGrow)) {
-            const float now = fmaxf(ref, top);
+          if (__any_sync(0xffffffffu, top > ref + kTop)) {
+            const float now = fmaxf(ref, top - kBias);
             const float f = now == ref ? 1.f : exp2_approx(ref - now);
             ref = now;
             sum *= f;
@@ -600,7 +600,7 @@ __global__ void __launch_bounds__(kPcThreads, 1)
           // A score that is NaN or +infinity makes the whole row NaN: the polynomial below would
           // drop it, so it is the reference that carries it into every weight of the part.
           const float neg = !(top < INFINITY) ? __int_as_float(0x7FFFFFFF)
-                                              : (ref == -INFINITY ? 0.f : kBias - ref);
+                                              : (ref == -INFINITY ? 0.f : -ref);
           const uint64_t scale2 = pair(scale, scale), neg2 = pair(neg, neg);
           uint64_t part[2] = {0ull, 0ull};
           // a third of the pairs take the polynomial
@@ -781,7 +781,7 @@ __global__ void __launch_bounds__(kPcThreads, 1)
         if (valid && a.q.lse) {
           const int rl = sg->sub + r_item, tk = row_token(a.q, rl);
           a.q.lse[static_cast<int64_t>(sg->tok + tk) * a.q.heads + sg->head0 + rl - tk * g] =
-              none ? -INFINITY : (m - kBias + log2f(l)) * 0.6931471805599453f;
+              none ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f;
         }
       }
       tc_fence_before();

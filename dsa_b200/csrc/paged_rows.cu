@@ -134,7 +134,7 @@ __global__ void __launch_bounds__(kPrWarps * 32, RowsCfg<D, MT, kSel, kPrWarps, 
   constexpr int kTeam = kSolo ? 1 : kPrWarps;      // warps that share an item
   constexpr int kUnitTiles = kPrWarps / kTeam;     // tiles of a unit per warp
   constexpr int kRows = C::kRows, kStages = C::kStages;
-  constexpr float kGrow = WeightRange<kBF16>::kGrow, kBias = WeightRange<kBF16>::kBias;
+  constexpr float kTop = WeightRange<kBF16>::kTop, kBias = WeightRange<kBF16>::kBias;
   constexpr int kKs = D / 16;   // 16-wide steps of the head dimension
   constexpr int kNt = D / 8;    // 8-wide output tiles
   constexpr int kLanesPerRow = D / 8;
@@ -424,9 +424,8 @@ __global__ void __launch_bounds__(kPrWarps * 32, RowsCfg<D, MT, kSel, kPrWarps, 
               if (!see) s[m][n][e] = -INFINITY;
             }
       }
-      // running maximum: the reference moves only when a row's maximum has grown by more than
-      // a factor 2^kGrow of weight, so most tiles rescale nothing and P stays below
-      // 2^(kGrow + kBias)
+      // running reference (see WeightRange): it moves only when a row's maximum has grown by more
+      // than a factor of 2^8 or 2^4 of weight, so most tiles rescale nothing
       bool grow = false;
       float top[MT][2];
 #pragma unroll
@@ -438,7 +437,7 @@ __global__ void __launch_bounds__(kPrWarps * 32, RowsCfg<D, MT, kSel, kPrWarps, 
           t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 1));
           t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 2));
           top[m][e] = t * a.q.scale_log2;
-          grow |= top[m][e] > mx[m][e] + kGrow ||
+          grow |= top[m][e] > mx[m][e] + kTop ||
                   (mx[m][e] == -INFINITY && top[m][e] > -INFINITY);
         }
       if (__any_sync(0xffffffffu, grow)) {
@@ -446,7 +445,7 @@ __global__ void __launch_bounds__(kPrWarps * 32, RowsCfg<D, MT, kSel, kPrWarps, 
         for (int m = 0; m < MT; ++m)
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
-            const float now = fmaxf(mx[m][e], top[m][e]);
+            const float now = fmaxf(mx[m][e], top[m][e] - kBias);
             const float f = now == mx[m][e] ? 1.f : exp2_approx(mx[m][e] - now);
             mx[m][e] = now;
             sum[m][e] *= f;
@@ -462,7 +461,7 @@ __global__ void __launch_bounds__(kPrWarps * 32, RowsCfg<D, MT, kSel, kPrWarps, 
       for (int m = 0; m < MT; ++m) {
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          const float ref = mx[m][e] == -INFINITY ? 0.f : mx[m][e] - kBias;
+          const float ref = mx[m][e] == -INFINITY ? 0.f : mx[m][e];
 #pragma unroll
           for (int n = 0; n < 2; ++n)
 #pragma unroll
@@ -642,7 +641,7 @@ __global__ void __launch_bounds__(kPrWarps * 32, RowsCfg<D, MT, kSel, kPrWarps, 
           *reinterpret_cast<uint2*>(a.q.out + t * a.q.o_ts + h * a.q.o_hs + col * 4) = w;
           if (a.q.lse && col == 0)
             a.q.lse[t * a.q.heads + h] =
-                l == 0.f ? -INFINITY : (m - kBias + log2f(l)) * 0.6931471805599453f;
+                l == 0.f ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f;
         } else {
           if (col == 0) a.part.ml[static_cast<int64_t>(slot) * kRows + r] = make_float2(m, l);
           *reinterpret_cast<float4*>(a.part.o + (static_cast<int64_t>(slot) * kRows + r) * D +

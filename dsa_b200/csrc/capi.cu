@@ -274,9 +274,9 @@ int check_token_rows(const tdsa_token_rows* r, int heads, int dim, const char* n
   return TDSA_OK;
 }
 
-// Whether rows of a (ha heads) and of b (hb heads) share memory, where that can be told: apart
-// from address ranges that do not meet, their strides have to be the same.  Strides are checked and not
-// negative.  self: a and b are one, and only different rows count.
+// Whether rows of a (ha heads) and of b (hb heads) share memory: exact where both have the same
+// strides, false where they differ (the caller's promise then).  Strides are not negative.  self:
+// a and b are one array, of which only different rows count.
 bool rows_overlap(const tdsa_token_rows* a, int ha, const tdsa_token_rows* b, int hb, int tokens,
                   int dim, bool self) {
   const int64_t ts = tokens > 1 ? a->token_stride : 0;

@@ -24,13 +24,14 @@
 //
 // What bounds it.  A unit of both tiles is 2048 cycles of tensor work (2560 with S in parts of 64,
 // whose operands shared memory delivers in 48 cycles instead of 32) and 3600 cycles of the rows'
-// warps: 64 scores of a row and part are read, compared and exponentiated in 1830 cycles with two
-// warps on an SM quarter, 1150 of them the exponentials, where the special-function pipe, the fma
-// pipe (a third of the exponentials) and the latency of either add up.  Sixteen warps of rows with
-// half a part each, and turns between the two tiles' exponentials, both measured the same.  4096
-// tokens over 16384 positions (32 heads in groups of 4, 128 features, 962 GFLOP): 0.86 ms alone,
-// 1.12 PFLOP/s against the 1.67 of a library product; 0.99 ms, 0.97 PFLOP/s, in a loop that holds
-// the card at its power limit, where the library product reaches 1.39.
+// warps (3800 with clocks read in between): 64 scores of a row and part are read, compared and
+// exponentiated in 1710 cycles with two warps on an SM quarter, 940 of them the exponentials, where
+// the special-function pipe, the fma pipe (a third of the exponentials) and the latency of either
+// add up.  Sixteen warps of rows with half a part each, and turns between the two tiles'
+// exponentials, both measured the same.  4096 tokens over 16384 positions (32 heads in groups of
+// 4, 128 features, 962 GFLOP): 0.86 ms alone, 1.12 PFLOP/s against the 1.67 of a library product;
+// 0.99 ms, 0.97 PFLOP/s, in a loop that holds the card at its power limit, where the library
+// product reaches 1.39.
 //
 // Scores, maxima, sums and O are float32.  P is rounded to the cache's type for the second
 // product (2^-8 relative in bf16, 2^-11 in f16 or 2^-36 of the row's largest weight where that is

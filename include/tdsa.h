@@ -599,8 +599,9 @@ int tdsa_query_prep(const void* qraw, int64_t qraw_stride, const void* hidden,
  * stride table_stride (position p of sequence b is row p % page_size of page
  * page_table[b][p / page_size]); query_starts [batch + 1] device int32, the sequences' new
  * tokens are rows query_starts[b] .. query_starts[b + 1] - 1 of the packed [tokens] arrays
- * (ascending; rows outside every sequence are neither read nor written); lengths [batch]
- * device int32, positions of each sequence with its new tokens, which are its last ones.
+ * (ascending; rows outside every sequence are not written and what they hold does not matter,
+ * but the append may read them); lengths [batch] device int32, positions of each sequence with
+ * its new tokens, which are its last ones.
  * max_new is the host's bound on a sequence's new tokens: it chooses a kernel, which changes
  * results by rounding at most.  max_pages * page_size <= 2^30.  Table entries are read only where a
  * position is needed; a page outside [0, pages) raises TDSA_STATUS_RANGE and its positions
@@ -643,8 +644,8 @@ typedef struct tdsa_token_rows {
 /*
  * Writes the keys (rotated) and values of every new token into its slot of the cache and, when
  * q is not NULL, its rotated queries into q_out (q itself with its strides, or rows that share no
- * memory with q, k, v or each other; refused where that can be told, as below).  The rotation turns the
- * pairs of the leading rope_dim features (0, or a multiple of 16 up to head_dim), the halves'
+ * memory with q, k, v or each other; refused where that can be told, as below).  The rotation
+ * turns the pairs of the leading rope_dim features (0, or a multiple of 16 up to head_dim), the halves'
  * j and j + rope_dim / 2 or, with interleaved != 0, neighbours 2 j and 2 j + 1, by the angle
  * position * inv_freq[j] (device float32 [rope_dim / 2]); positions (device int64 [tokens])
  * replaces the tokens' positions in the angle, NULL keeps them.  The angle is reduced in
@@ -664,10 +665,12 @@ int tdsa_paged_append(const tdsa_paged_cache* cache, const tdsa_paged_batch* bat
  *   out[t][h] = sum_j softmax_j(scale * q[t][h] . K[j][h / g]) V[j][h / g],  g = q_heads /
  *   kv_heads;  lse[t][h] = log sum_j exp(scale * q . K[j]) (float32, [tokens][q_heads], NULL:
  *   not wanted).
- * A token that sees no key gets out 0 and lse -inf.  out's rows must not overlap q or each other;
- * that is refused where both have the same strides (other pairs are not looked into).  float32 scores,
- * maxima and sums; in long chunks the softmax weights are rounded to the cache's type for the
- * product with V.  scale > 0.
+ * A token that sees no key gets out 0 and lse -inf; one with a score that is NaN or +infinity gets
+ * NaN.  out's rows must not overlap q or each other, which is refused where both have the same
+ * strides (other pairs are not looked into).  float32 scores, maxima and sums; in long chunks the
+ * softmax weights are rounded to the cache's type for the product with V (in float16 to 2^-11 or
+ * 2^-36 of the row's largest, whichever is more).  scale > 0; a window past the positions that a
+ * table can have is none.
  * workspace: tdsa_paged_workspace_bytes bytes, 256-byte aligned, its first
  * TDSA_PAGED_COUNTER_BYTES zero before its first use; every call leaves it ready for the next
  * one on the same stream (after a TDSA_ERR_TIMEOUT, zero them again).

@@ -115,17 +115,17 @@ __device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
   asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
   return r;
 }
-// A weight is held as 2^(x - ref), x the score and ref the running reference of its row (in log2
-// units), and no weight is above 2^kTop: when a score would give one, ref moves to kBias below
-// the row's maximum, so it moves when the maximum has grown by kTop - kBias, 8 or 4.  Sums, partial
-// results and outputs are all relative to ref.  bfloat16 has float32's exponents, so no weight
-// needs to be above 1, and with none above it a value near the type's largest does not overflow a
-// product.  float16 would lose every weight below 2^-25 of the largest, which a long row has many
-// of: up to 2^15 of float16's 2^16, weights above 2^-25 of the row's largest keep 11 bits, and a
-// smaller one is off by no more than 2^-36 of it.
+// A weight is held as 2^((s - t) scale + kBias), s the score and t the score of the row's maximum
+// as it stood when t was last moved, which happens when it has grown by kGrow log2 units, so no
+// weight is above 2^(kBias + kGrow).  (The difference comes before the product: t scale alone, once
+// its rounding is worth a power of two, would make a largest weight infinite or nothing.)
+// bfloat16 has float32's exponents, so no weight needs to be above 1, and with none above it a
+// value near the type's largest does not overflow a product.  float16 would lose every weight below
+// 2^-25 of the largest, which a long row has many of: up to 2^15 of float16's 2^16, weights above
+// 2^-25 of the row's largest keep 11 bits, and a smaller one is off by no more than 2^-36 of it.
 template <bool kBF16>
 struct WeightRange {
-  static constexpr float kTop = kBF16 ? 0.f : 15.f, kBias = kBF16 ? -8.f : 11.f;
+  static constexpr float kGrow = kBF16 ? 8.f : 4.f, kBias = kBF16 ? -8.f : 11.f;
 };
 
 // Slice of CTA c of `ctas` (at most `units`) over `units`, and the CTA whose slice holds unit u:
@@ -150,7 +150,7 @@ __device__ __forceinline__ int slice_owner(int64_t units, int ctas, int64_t u) {
 constexpr int kPagedCounters = TDSA_PAGED_COUNTER_BYTES / 4;
 struct PagedPartials {
   uint32_t* counters;
-  float2* ml;   // [slot][rows]: running reference (log2 units), sum
+  float2* ml;   // [slot][rows]: running maximum (few rows: t; chunks: t scale - kBias), sum
   float* o;     // [slot][rows][dim]
 };
 

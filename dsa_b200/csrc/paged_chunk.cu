@@ -29,8 +29,8 @@
 // the special-function pipe, the fma pipe (a third of the exponentials) and the latency of either
 // add up.  Sixteen warps of rows with half a part each, and turns between the two tiles'
 // exponentials, both measured the same.  4096 tokens over 16384 positions (32 heads in groups of
-// 4, 128 features, 962 GFLOP): 0.86 ms alone, 1.12 PFLOP/s against the 1.67 of a library product;
-// 0.99 ms, 0.97 PFLOP/s, in a loop that holds the card at its power limit, where the library
+// 4, 128 features, 962 GFLOP): 0.87 ms alone, 1.11 PFLOP/s against the 1.67 of a library product;
+// 1.00 ms, 0.96 PFLOP/s, in a loop that holds the card at its power limit, where the library
 // product reaches 1.39.
 //
 // Scores, maxima, sums and O are float32.  P is rounded to the cache's type for the second
@@ -272,6 +272,52 @@ __device__ __forceinline__ float2 exp2_poly2(uint64_t x2) {
                      __int_as_float(max(__float_as_int(pv.y) + (__float_as_int(rv.y) << 23), 0)));
 }
 
+// The keys of a part (from `base` on) that a row sees of [lo, hi), a bit each; gone: bit x is set
+// when keys 16 x .. 16 x + 15 are of no page.
+__device__ __forceinline__ uint64_t seen_keys(int lo, int hi, int base, uint32_t gone) {
+  const int from = max(0, lo - base), to = min(kPcPart, hi - base);
+  const uint64_t below_to = to >= 64 ? ~0ull : (to <= 0 ? 0ull : (1ull << to) - 1);
+  const uint64_t below_from = from >= 64 ? ~0ull : (1ull << from) - 1;
+  uint64_t seen = below_to & ~below_from;
+#pragma unroll
+  for (int x = 0; x < 4; ++x)
+    if ((gone >> x) & 1u) seen &= ~(0xFFFFull << (16 * x));
+  return seen;
+}
+
+// A part's weights of one row, the maximum taken off the scores before the product (see
+// WeightRange): S from TMEM, P to TMEM, their sum returned.  Not inlined: the code in the loop over
+// parts cost every call 2 to 4 %.
+template <bool kBF16>
+__device__ __noinline__ float far_weights(uint32_t s_addr, int lo, int hi, uint32_t gone, float mx,
+                                          float scale) {
+  const uint64_t seen = seen_keys(lo, hi, 0, gone);
+  const float t = mx == -INFINITY ? 0.f : mx;
+  float sum = 0.f;
+  for (int c = 0; c < 2; ++c) {
+    uint32_t s[32], p[16];
+    __syncwarp();
+    tmem_ld32(s_addr + c * 32, s);
+    tmem_wait_ld();
+    const uint32_t w = static_cast<uint32_t>(seen >> (32 * c));
+#pragma unroll
+    for (int j = 0; j < 16; ++j) {
+      float e[2];
+#pragma unroll
+      for (int x = 0; x < 2; ++x) {
+        const float d = __uint_as_float(s[2 * j + x]) - t;
+        e[x] = (w >> (2 * j + x)) & 1u
+                   ? exp2_approx(fmaf(d, scale, WeightRange<kBF16>::kBias))
+                   : 0.f;
+        sum += e[x];
+      }
+      p[j] = pack16<kBF16>(e[0], e[1]);
+    }
+    tmem_st16(s_addr + c * 16, p);
+  }
+  return sum;
+}
+
 // A segment of an item, published by the copy warp to the others.
 struct ChunkSegment {
   int unit0, units;    // first unit and number of units (0: the CTA's list ends)
@@ -288,7 +334,7 @@ __global__ void __launch_bounds__(kPcThreads, 1)
     paged_chunk_kernel(const __grid_constant__ CUtensorMap kmap,
                        const __grid_constant__ CUtensorMap vmap, const ChunkArgs a) {
   using C = ChunkCfg<D>;
-  constexpr float kTop = WeightRange<kBF16>::kTop, kBias = WeightRange<kBF16>::kBias;
+  constexpr float kBias = WeightRange<kBF16>::kBias;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>(
       (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -458,7 +504,7 @@ __global__ void __launch_bounds__(kPcThreads, 1)
     const uint32_t lane_base = static_cast<uint32_t>(warp & 3) << 21;
     const uint32_t s_addr = tmem + lane_base + t * 128;
     const uint32_t o_addr = tmem + lane_base + C::kOCol + t * D;
-    const float scale = a.q.scale_log2;
+    const float scale = a.q.scale_log2, grow = WeightRange<kBF16>::kGrow / scale;
     // one bit per buffer: the parity of its next S, and whether its last product was the threads'
     uint32_t s_ph = 0, was_alone = 0;
     uint32_t n_unit = 0;  // units of the CTA's list before the segment
@@ -526,7 +572,12 @@ __global__ void __launch_bounds__(kPcThreads, 1)
         all_hi = min(sg->k1, first + 1);
         all_lo = w > 0 ? max(sg->k0, last - (w - 1)) : sg->k0;
       }
-      float ref = -INFINITY, sum = 0.f;
+      float mx = -INFINITY, sum = 0.f;  // the running maximum, a score
+      // A weight is 2^(s scale + add), the difference from the maximum formed by one fma.  Where
+      // the rounding of mx scale would show, past 2^20 units in any row of the warp, far_weights
+      // forms them; every part then counts as past the limit, so that others pay nothing for it.
+      float add = 0.f;
+      float limit = -INFINITY;  // a score above it moves the maximum
       int base = sg->unit0 * kPcUnit;
       bool ok = true;
       for (int i = 0; i < units && ok; ++i) {
@@ -549,14 +600,7 @@ __global__ void __launch_bounds__(kPcThreads, 1)
           }
           tmem_wait_ld();
           if (masked) {
-            // the keys of the part that the row sees, a bit each
-            const int from = max(0, lo - base), to = min(kPcPart, hi - base);
-            const uint64_t below_to = to >= 64 ? ~0ull : (to <= 0 ? 0ull : (1ull << to) - 1);
-            const uint64_t below_from = from >= 64 ? ~0ull : (1ull << from) - 1;
-            uint64_t seen = below_to & ~below_from;
-#pragma unroll
-            for (int x = 0; x < 4; ++x)
-              if ((gone >> x) & 1u) seen &= ~(0xFFFFull << (16 * x));
+            const uint64_t seen = seen_keys(lo, hi, base, gone);
 #pragma unroll
             for (int c = 0; c < 2; ++c) {
               const uint32_t w = static_cast<uint32_t>(seen >> (32 * c));
@@ -576,11 +620,14 @@ __global__ void __launch_bounds__(kPcThreads, 1)
               tops[c] = max3_nan(tops[c], __uint_as_float(x[j]), __uint_as_float(x[j + 1]));
             tops[c] = max2_nan(tops[c], __uint_as_float(x[15]));
           }
-          const float top = max2_nan(max3_nan(tops[0], tops[1], tops[2]), tops[3]) * scale;
-          if (__any_sync(0xffffffffu, top > ref + kTop)) {
-            const float now = fmaxf(ref, top - kBias);
-            const float f = now == ref ? 1.f : exp2_approx(ref - now);
-            ref = now;
+          const float top = max2_nan(max3_nan(tops[0], tops[1], tops[2]), tops[3]);
+          if (__any_sync(0xffffffffu, top > limit)) {
+            const float now = fmaxf(mx, top);
+            const float f = now == mx ? 1.f : exp2_approx((mx - now) * scale);
+            mx = now;
+            const float ref = fmaf(mx, scale, -kBias);
+            add = mx == -INFINITY ? 0.f : -ref;
+            limit = mx + grow;
             sum *= f;
             if (i > 0 || b > 0) {
               // O += P V of the part before is complete with the S after this one
@@ -597,38 +644,45 @@ __global__ void __launch_bounds__(kPcThreads, 1)
                 tmem_st16(o_addr + c * 16, o);
               }
             }
-          }
-          // A score that is NaN or +infinity makes the whole row NaN: the polynomial below would
-          // drop it, so it is the reference that carries it into every weight of the part.
-          const float neg = !(top < INFINITY) ? __int_as_float(0x7FFFFFFF)
-                                              : (ref == -INFINITY ? 0.f : -ref);
-          const uint64_t scale2 = pair(scale, scale), neg2 = pair(neg, neg);
-          uint64_t part[2] = {0ull, 0ull};
-          // a third of the pairs take the polynomial
-#pragma unroll
-          for (int c = 0; c < 2; ++c) {
-            uint32_t p[16];
-#pragma unroll
-            for (int j = 0; j < 16; ++j) {
-              const uint64_t x2 =
-                  fma2(pair(__uint_as_float(s[c][2 * j]), __uint_as_float(s[c][2 * j + 1])), scale2,
-                       neg2);
-              float2 e;
-              if (j % 3 == 1) {
-                e = exp2_poly2(x2);
-              } else {
-                const float2 x = unpair(x2);
-                e = make_float2(exp2_approx(x.x), exp2_approx(x.y));
-              }
-              part[j & 1] = add2(part[j & 1], pair(e.x, e.y));
-              p[j] = pack16<kBF16>(e.x, e.y);
+            if (__any_sync(0xffffffffu, fabsf(add) > 0x1p20f)) {
+              sum += far_weights<kBF16>(sb, lo - base, hi - base, gone, mx, scale);
+              limit = -INFINITY;
+              goto weighed;
             }
-            tmem_st16(sb + c * 16, p);
           }
           {
-            const float2 x = unpair(add2(part[0], part[1]));
-            sum += x.x + x.y;
+            // A score that is NaN or +infinity makes the whole row NaN: the polynomial below would
+            // drop it, so it is carried into every weight of the part.
+            const float neg = top < INFINITY ? add : __int_as_float(0x7FFFFFFF);
+            const uint64_t scale2 = pair(scale, scale), neg2 = pair(neg, neg);
+            uint64_t part[2] = {0ull, 0ull};
+            // a third of the pairs take the polynomial
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+              uint32_t p[16];
+#pragma unroll
+              for (int j = 0; j < 16; ++j) {
+                const uint64_t x2 =
+                    fma2(pair(__uint_as_float(s[c][2 * j]), __uint_as_float(s[c][2 * j + 1])),
+                         scale2, neg2);
+                float2 e;
+                if (j % 3 == 1) {
+                  e = exp2_poly2(x2);
+                } else {
+                  const float2 x = unpair(x2);
+                  e = make_float2(exp2_approx(x.x), exp2_approx(x.y));
+                }
+                part[j & 1] = add2(part[j & 1], pair(e.x, e.y));
+                p[j] = pack16<kBF16>(e.x, e.y);
+              }
+              tmem_st16(sb + c * 16, p);
+            }
+            {
+              const float2 x = unpair(add2(part[0], part[1]));
+              sum += x.x + x.y;
+            }
           }
+        weighed:
           tmem_wait_st();
           if (masked) {
             // A value that only some rows see and that is not finite: zero weights times it
@@ -688,7 +742,7 @@ __global__ void __launch_bounds__(kPcThreads, 1)
         // a part of the item: float32, the rows of a column quad side by side
         const int cta = blockIdx.x;
         const int64_t slot = 2 * cta + (cta == c_first ? 1 : 0);
-        a.part.ml[slot * kPcRows + r_item] = make_float2(ref, sum);
+        a.part.ml[slot * kPcRows + r_item] = make_float2(fmaf(mx, scale, -kBias), sum);
         float4* dst = reinterpret_cast<float4*>(a.part.o + slot * kPcRows * D) + r_item;
 #pragma unroll 1
         for (int c = 0; c < D / 32; ++c) {
@@ -709,7 +763,7 @@ __global__ void __launch_bounds__(kPcThreads, 1)
         write = s_last[t] != 0;
       }
       if (write) {
-        float m = ref, l = sum;
+        float m = fmaf(mx, scale, -kBias), l = sum;
         const bool split = units != sg->item_units;
         auto slot_of = [&](int c) { return (2 * static_cast<int64_t>(c) + (c == c_first)) * kPcRows; };
         if (split) {  // the last to arrive adds the parts up, in the CTAs' order

@@ -134,7 +134,7 @@ __global__ void __launch_bounds__(kPrWarps * 32, RowsCfg<D, MT, kSel, kPrWarps, 
   constexpr int kTeam = kSolo ? 1 : kPrWarps;      // warps that share an item
   constexpr int kUnitTiles = kPrWarps / kTeam;     // tiles of a unit per warp
   constexpr int kRows = C::kRows, kStages = C::kStages;
-  constexpr float kTop = WeightRange<kBF16>::kTop, kBias = WeightRange<kBF16>::kBias;
+  constexpr float kGrow = WeightRange<kBF16>::kGrow, kBias = WeightRange<kBF16>::kBias;
   constexpr int kKs = D / 16;   // 16-wide steps of the head dimension
   constexpr int kNt = D / 8;    // 8-wide output tiles
   constexpr int kLanesPerRow = D / 8;
@@ -424,8 +424,8 @@ __global__ void __launch_bounds__(kPrWarps * 32, RowsCfg<D, MT, kSel, kPrWarps, 
               if (!see) s[m][n][e] = -INFINITY;
             }
       }
-      // running reference (see WeightRange): it moves only when a row's maximum has grown by more
-      // than a factor of 2^8 or 2^4 of weight, so most tiles rescale nothing
+      // running maximum mx (a score): it moves only when a row's has grown by a factor of 2^8 or
+      // 2^4 of weight (see WeightRange), so most tiles rescale nothing
       bool grow = false;
       float top[MT][2];
 #pragma unroll
@@ -436,17 +436,17 @@ __global__ void __launch_bounds__(kPrWarps * 32, RowsCfg<D, MT, kSel, kPrWarps, 
                           fmaxf(s[m][1][2 * e], s[m][1][2 * e + 1]));
           t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 1));
           t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 2));
-          top[m][e] = t * a.q.scale_log2;
-          grow |= top[m][e] > mx[m][e] + kTop ||
-                  (mx[m][e] == -INFINITY && top[m][e] > -INFINITY);
+          top[m][e] = t;
+          grow |= (t - mx[m][e]) * a.q.scale_log2 > kGrow;
         }
       if (__any_sync(0xffffffffu, grow)) {
 #pragma unroll
         for (int m = 0; m < MT; ++m)
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
-            const float now = fmaxf(mx[m][e], top[m][e] - kBias);
-            const float f = now == mx[m][e] ? 1.f : exp2_approx(mx[m][e] - now);
+            const float now = fmaxf(mx[m][e], top[m][e]);
+            const float f =
+                now == mx[m][e] ? 1.f : exp2_approx((mx[m][e] - now) * a.q.scale_log2);
             mx[m][e] = now;
             sum[m][e] *= f;
 #pragma unroll
@@ -466,7 +466,7 @@ __global__ void __launch_bounds__(kPrWarps * 32, RowsCfg<D, MT, kSel, kPrWarps, 
           for (int n = 0; n < 2; ++n)
 #pragma unroll
             for (int x = 0; x < 2; ++x) {
-              const float p = exp2_approx(fmaf(s[m][n][2 * e + x], a.q.scale_log2, -ref));
+              const float p = exp2_approx(fmaf(s[m][n][2 * e + x] - ref, a.q.scale_log2, kBias));
               s[m][n][2 * e + x] = p;
               sum[m][e] += p;
             }
@@ -618,7 +618,7 @@ __global__ void __launch_bounds__(kPrWarps * 32, RowsCfg<D, MT, kSel, kPrWarps, 
 #pragma unroll
         for (int w = 0; w < kTeam; ++w) {
           const float2 ml = s_ml[w * kRows + r];
-          const float f = exp2_approx(ml.x - ref);
+          const float f = exp2_approx((ml.x - ref) * a.q.scale_log2);
           const uint8_t* from = kSolo ? ring : smem + w * C::kWarpBytes;
           const float4 x = *reinterpret_cast<const float4*>(
               reinterpret_cast<const float*>(from) + r * D + col * 4);
@@ -641,7 +641,8 @@ __global__ void __launch_bounds__(kPrWarps * 32, RowsCfg<D, MT, kSel, kPrWarps, 
           *reinterpret_cast<uint2*>(a.q.out + t * a.q.o_ts + h * a.q.o_hs + col * 4) = w;
           if (a.q.lse && col == 0)
             a.q.lse[t * a.q.heads + h] =
-                l == 0.f ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f;
+                l == 0.f ? -INFINITY
+                         : (fmaf(m, a.q.scale_log2, -kBias) + log2f(l)) * 0.6931471805599453f;
         } else {
           if (col == 0) a.part.ml[static_cast<int64_t>(slot) * kRows + r] = make_float2(m, l);
           *reinterpret_cast<float4*>(a.part.o + (static_cast<int64_t>(slot) * kRows + r) * D +
@@ -697,8 +698,8 @@ __global__ void __launch_bounds__(kPrWarps * 32, RowsCfg<D, MT, kSel, kPrWarps, 
                 now = fmaxf(now, __shfl_xor_sync(0xffffffffu, now, o2));
               now = fmaxf(now, m[x]);
               const float ref = now == -INFINITY ? 0.f : now;
-              const float keep = exp2_approx(m[x] - ref);
-              f[x] = exp2_approx(ml[x].x - ref);
+              const float keep = exp2_approx((m[x] - ref) * a.q.scale_log2);
+              f[x] = exp2_approx((ml[x].x - ref) * a.q.scale_log2);
               l[x] = l[x] * keep + ml[x].y * f[x];  // this lane's partials
               v[x].x *= keep, v[x].y *= keep, v[x].z *= keep, v[x].w *= keep;
               m[x] = now;

@@ -424,3 +424,46 @@ def test_many_long_items_of_two_tiles():
     c = Case([700] * 6, [2100 + 97 * i for i in range(6)], dim=64, hq=32, hkv=4, page=64, seed=74)
     c.there = [torch.ones(n, dtype=torch.bool) for n in c.lens]
     _check(c, _attend(c), _torch_reference(c))
+
+
+# ------------------------------------------------------------------ scores of any size
+
+@pytest.mark.parametrize("dtype,size", [(BF16, 300.0), (BF16, 1e4), (BF16, 1e6), (BF16, 1e12),
+                                        (F16, 300.0), (F16, 5e3), (F16, 1.2e4)])
+@pytest.mark.parametrize("n", [1, 8, 40])
+def test_scores_of_any_size(dtype, size, n):
+    # queries and keys of ``size``: scores up to 1e25, each off by 2^-17 of sum |q k|, so a row is
+    # its best key's value where that leads by more; float32 holds them all
+    from dsa_b200.paged import selected_attention
+
+    c = Case([n, 3], [700, 90], dtype=dtype, dim=128, seed=80)
+    c.q = (c.q.double() * size).to(dtype)
+    c.qd = c.q.cuda()
+    for b, length in enumerate(c.lens):
+        c.k[b] = (c.k[b] * size).to(dtype).double()
+        pages = c.table[b, :-(-length // c.page)].long().cuda()
+        room = torch.zeros(pages.numel() * c.page, 2, 128, dtype=dtype)
+        room[:length] = c.k[b].to(dtype)
+        c.cache.keys[pages] = room.view(-1, c.page, 2, 128).cuda()
+    out, mag, lse = c.reference()
+    clear = torch.zeros(c.tokens, 8, dtype=torch.bool)
+    for b, (new, length) in enumerate(zip(c.news, c.lens)):
+        for i in range(new):
+            t, keys = c.starts[b] + i, c.k[b][:length - new + i + 1]
+            for h in range(8):
+                z = keys[:, h // 4] @ c.q[t, h].double()
+                best = z.topk(2).values
+                room = (keys[:, h // 4].abs() @ c.q[t, h].double().abs()).max() * 2.0 ** -16
+                # by so much that the second key's weight is nothing
+                clear[t, h] = best[0] - best[1] > room + 40 * 128 ** 0.5
+    assert clear.float().mean() > 0.8
+    ind = torch.arange(700).repeat(c.tokens, 1)
+    ind[ind > torch.cat([torch.arange(m - k, m) for k, m in zip(c.news, c.lens)])[:, None]] = -1
+    for got, got_lse in (_attend(c), selected_attention(c.qd, c.cache, c.batch, ind.cuda(),
+                                                        return_lse=True)):
+        err = (got.double().cpu() - out).abs()
+        u = ROUND[dtype]
+        lim = (u + 2.0 ** -12) * mag + u * (1 + u) * out.abs() + 2.0 ** -24
+        assert bool((err <= lim)[clear].all())
+        assert bool(torch.isfinite(got).all())
+        assert bool(((got_lse.double().cpu() - lse).abs() <= 2.0 ** -14 * lse.abs()).all())

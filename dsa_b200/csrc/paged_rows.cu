@@ -8,12 +8,12 @@
 // read from the cache once.
 //
 // HBM bound: a key and its value are 4 D bytes for 4 D rows multiply-adds.  32 ragged sequences
-// (979 MB) take 161 to 171 us from one card to another, 6.1 to 5.7 TB/s of the 6.55 that a copy
-// reaches; 2048 selected positions for 64 sequences (537 MB in pieces of 256 bytes) 93 to 98 us,
-// 5.8 to 5.5 TB/s; one sequence of 32768 positions (134 MB) 37 us, 9 of them before the first tile
-// is there and after the last, and the slowest SM a third later than the fastest.  17 to 32 rows
-// (16 sequences of 8192, 537 MB) take 127 us at 128 features, 4.2 TB/s, and 90 at 64 (half the
-// bytes), 3.0 TB/s: the instructions of two row tiles a key tile do not hide behind the loads.
+// (979 MB) take 168 us, 5.8 TB/s of the 6.55 that a copy reaches, and up to 6 % less on other
+// cards; 2048 selected positions for 64 sequences (537 MB in pieces of 256 bytes) 96 us, 5.6
+// TB/s; one sequence of 32768 positions (134 MB) 36 us, 9 of them before the first tile is there
+// and after the last, and the slowest SM a third later than the fastest.  17 to 32 rows (16
+// sequences of 8192, 537 MB) take 125 us at 128 features, 4.3 TB/s, and 80 at 64 (half the bytes),
+// 3.4 TB/s: the instructions of two row tiles a key tile do not hide behind the loads.
 //
 // Layout.  A CTA is four or eight warps.  Each warp runs its own stream of 16-key tiles (a unit is
 // a tile per warp) with its own ring of tiles in shared memory, filled by 16-byte asynchronous
@@ -71,7 +71,7 @@ struct RowsCfg {
   static constexpr int kMl = kWarps * kRows * 8;
   // Queries are in registers where they fit beside the output.  32 rows of 128 features do not,
   // and a team reads them from shared memory for every tile (16 sequences of 8192, 4 tokens x 8
-  // heads per group: 127 us, 168 with registers, of which 370 bytes spill).
+  // heads per group: 125 us, 168 with registers, of which 370 bytes spill).
   static constexpr bool kQShared = MT == 2 && D == 128 && !kSolo;
   static constexpr int kQ = (kRing + kMl + 256 + kWarps * kStages * 4 + 127) / 128 * 128;
   static constexpr int kSmem =
@@ -551,8 +551,8 @@ __global__ void __launch_bounds__(kPrWarps * 32, RowsCfg<D, MT, kSel, kPrWarps, 
     // An infinite value times what the rounding left, which is zero or negative as often as not,
     // is NaN where the average is infinite.  Twice the first term is right, and is halved here.  A
     // warp goes back alone: the second time nothing up to here waits for other warps.  Segments
-    // whose output is finite pay for the look at it (one sequence of 32768 positions 36.8 us
-    // against 36.4).
+    // whose output is finite pay 1 to 2 % for the look at it where items are short, and nothing
+    // that shows where they are long.
     if (second == 0.f) {
 #pragma unroll
       for (int m = 0; m < MT; ++m)
